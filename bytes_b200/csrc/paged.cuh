@@ -1,0 +1,58 @@
+// Pieces shared by the paged-cache kernels: the cache's geometry and its host checks.
+#pragma once
+#include "common.cuh"
+
+namespace bd {
+
+// A paged cache as the kernels address it: pages [num_blocks, Hk, block, D], any strides
+// (elements; the innermost one too), and the block table that maps a sequence's logical
+// pages to them. Entries outside [0, num_blocks) name no page.
+struct PagedGeometry {
+  int B, Hk, D, num_blocks, block, wide;  // wide: columns of the block table
+  const int* table; int64_t t_sb, t_si;
+  const int* lens; int64_t l_s;
+  int64_t k_sb, k_sh, k_st, k_sd;
+  int64_t v_sb, v_sh, v_st, v_sd;
+};
+
+// Tokens a sequence holds: its length, cut to what the block table can address.
+__device__ __forceinline__ int paged_len(const PagedGeometry& g, int b) {
+  const int n = g.lens[int64_t(b) * g.l_s];
+  const int64_t cap = int64_t(g.wide) * g.block;
+  return n < 0 ? 0 : (int64_t(n) > cap ? int(cap) : n);
+}
+
+// Physical page of logical page j (0 <= j < wide) of sequence b, or -1.
+__device__ __forceinline__ int paged_block(const PagedGeometry& g, int b, int j) {
+  const int p = g.table[int64_t(b) * g.t_sb + int64_t(j) * g.t_si];
+  return p >= 0 && p < g.num_blocks ? p : -1;
+}
+
+// Checks of cache, block table and lengths that every paged entry point makes.
+int check_paged(const bd_tensor* k_cache, const bd_tensor* v_cache, const bd_tensor* block_table,
+                const bd_tensor* context_lens, PagedGeometry* g);
+
+inline bool is_float16_32(int dt) { return dt == BD_BF16 || dt == BD_F16 || dt == BD_F32; }
+
+// Runs the body of an extern "C" entry point: nothing thrown in it (an allocation that fails
+// while a message is built) crosses the C boundary.
+template <typename F>
+int guarded(F&& body) noexcept {
+  try {
+    return body();
+  } catch (...) {
+    return BD_ERR_CUDA;
+  }
+}
+
+// Loads and stores by element type, for the forms that take any of them.
+__device__ __forceinline__ float load_as(const void* base, int dt, int64_t off) {
+  switch (dt) {
+    case BD_BF16: return to_f32(reinterpret_cast<const __nv_bfloat16*>(base)[off]);
+    case BD_F16: return to_f32(reinterpret_cast<const __half*>(base)[off]);
+    case BD_F8E4M3: return to_f32(reinterpret_cast<const __nv_fp8_e4m3*>(base)[off]);
+    default: return reinterpret_cast<const float*>(base)[off];
+  }
+}
+
+}  // namespace bd

@@ -128,6 +128,99 @@ std::tuple<int64_t, at::Tensor> decode_attn_nq(const at::Tensor& q, const at::Te
   return {rc, out};
 }
 
+// ---- the paged cache. Optional tensors: an undefined one becomes a NULL descriptor.
+using Opt = c10::optional<at::Tensor>;
+
+struct OptDesc {
+  bd_tensor d{};
+  const bd_tensor* p = nullptr;
+  OptDesc(const Opt& t, int device) {
+    if (t.has_value() && t->defined()) {
+      d = desc(*t, device);
+      p = &d;
+    }
+  }
+};
+
+// A decode query or output: [B, H, D], or [B, H, 1, D] viewed so.
+bd_tensor desc_row(const at::Tensor& t, int device) {
+  return t.dim() == 4 && t.size(2) == 1 ? desc_drop2(t, device) : desc(t, device);
+}
+
+// bd_paged_append, then bd_paged_block_summary of the touched pages when a summary is kept
+// -> (status, rotated queries or None).
+std::tuple<int64_t, Opt> paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
+                                      const at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& lens,
+                                      const Opt& q, const Opt& cos, const Opt& sin, bool interleaved, const Opt& cu,
+                                      double k_scale, double v_scale, const Opt& summary, const Opt& summary_scale) {
+  const int dev = k.get_device();
+  const bd_tensor dk = desc(k, dev), dv = desc(v, dev), dkc = desc(k_cache, dev), dvc = desc(v_cache, dev),
+                  dt = desc(table, dev), dl = desc(lens, dev);
+  const OptDesc dq(q, dev), dcos(cos, dev), dsin(sin, dev), dcu(cu, dev), ds(summary, dev), dss(summary_scale, dev);
+  const c10::cuda::CUDAGuard guard(k.device());
+  const auto st = at::cuda::getCurrentCUDAStream(dev).stream();
+  Opt q_out;
+  if (dq.p) q_out = at::empty(q->sizes(), q->options());
+  const OptDesc dqo(q_out, dev);
+  int rc = bd_paged_append(&dk, &dv, dq.p, dcos.p, dsin.p, interleaved, dcu.p, &dt, &dl, float(k_scale),
+                           float(v_scale), &dkc, &dvc, dqo.p, st);
+  if (rc == 0 && ds.p && k.size(0) > 0)
+    rc = bd_paged_block_summary(&dkc, &dt, &dl, dcu.p, int(k.size(0)), float(k_scale), ds.p, dss.p, st);
+  return {rc, q_out};
+}
+
+int64_t paged_block_summary(const at::Tensor& k_cache, const at::Tensor& table, const at::Tensor& lens,
+                            double k_scale, const at::Tensor& summary, const at::Tensor& summary_scale) {
+  const int dev = k_cache.get_device();
+  const bd_tensor dkc = desc(k_cache, dev), dt = desc(table, dev), dl = desc(lens, dev), ds = desc(summary, dev),
+                  dss = desc(summary_scale, dev);
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  return bd_paged_block_summary(&dkc, &dt, &dl, nullptr, 0, float(k_scale), &ds, &dss,
+                                at::cuda::getCurrentCUDAStream(dev).stream());
+}
+
+// -> (status, selected int32 [B, Hk, budget])
+std::tuple<int64_t, at::Tensor> paged_select(const at::Tensor& q, const at::Tensor& summary,
+                                             const at::Tensor& summary_scale, const at::Tensor& table,
+                                             const at::Tensor& lens, int64_t block_size, int64_t budget, int64_t sink,
+                                             int64_t recent) {
+  const int dev = q.get_device();
+  const bd_tensor dq = desc_row(q, dev), ds = desc(summary, dev), dss = desc(summary_scale, dev),
+                  dt = desc(table, dev), dl = desc(lens, dev);
+  if (summary.dim() != 4) return {BD_ERR_SHAPE, at::Tensor()};
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor sel = at::empty({q.size(0), summary.size(1), budget}, q.options().dtype(at::kInt));
+  const bd_tensor dsel = desc(sel, dev);
+  const size_t nws = bd_paged_select_workspace(&dq, &ds, &dt);
+  const at::Tensor ws = workspace(nws, q);
+  const int rc = bd_paged_select(&dq, &ds, &dss, &dt, &dl, int(block_size), int(sink), int(recent), &dsel,
+                                 ws.data_ptr(), nws, at::cuda::getCurrentCUDAStream(dev).stream());
+  return {rc, sel};
+}
+
+// -> (status, out like q, lse [B, Hq] or None)
+std::tuple<int64_t, at::Tensor, Opt> paged_decode_attn(const at::Tensor& q, const at::Tensor& k_cache,
+                                                       const at::Tensor& v_cache, const at::Tensor& table,
+                                                       const at::Tensor& lens, const Opt& selected, double scaling,
+                                                       double k_scale, double v_scale, bool want_lse) {
+  const int dev = q.get_device();
+  const bd_tensor dq = desc_row(q, dev), dk = desc(k_cache, dev), dv = desc(v_cache, dev), dt = desc(table, dev),
+                  dl = desc(lens, dev);
+  const OptDesc dsel(selected, dev);
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  const bd_tensor dout = desc_row(out, dev);
+  Opt lse;
+  if (want_lse) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  const OptDesc dlse(lse, dev);
+  const size_t nws = bd_paged_decode_attn_workspace(&dq, &dk, &dv, &dt, &dl, dsel.p);
+  const at::Tensor ws = workspace(nws, q);
+  const int rc = bd_paged_decode_attn(&dq, &dk, &dv, &dt, &dl, dsel.p, float(scaling), float(k_scale),
+                                      float(v_scale), &dout, dlse.p, ws.data_ptr(), nws,
+                                      at::cuda::getCurrentCUDAStream(dev).stream());
+  return {rc, out, lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -136,4 +229,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attn", &decode_attn, "bd_decode_attn on the current CUDA stream");
   m.def("kivi_decode_attn", &kivi_decode_attn, "the drop-in KIVI decode step: (status, out [B,Hq,1,D])");
   m.def("decode_attn_nq", &decode_attn_nq, "decode_attn_bf16 / decode_attn_fp8: (status, out [B,Hq,1,D])");
+  m.def("paged_append", &paged_append, "bd_paged_append (+ summaries): (status, rotated queries)");
+  m.def("paged_block_summary", &paged_block_summary, "bd_paged_block_summary of every page");
+  m.def("paged_select", &paged_select, "bd_paged_select: (status, selected)");
+  m.def("paged_decode_attn", &paged_decode_attn, "bd_paged_decode_attn: (status, out, lse)");
 }

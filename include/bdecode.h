@@ -331,6 +331,63 @@ int bd_pq_encode(const bd_tensor* x, const bd_tensor* centroids, const bd_tensor
  *      quantize_key / quantize_value  src/quantization.py:468-501 */
 int bd_asym_fakequant(const bd_tensor* x, int levels, const bd_tensor* y, bd_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged key-value cache: pages k_cache, v_cache [num_blocks,Hk,block,D] of one type (bf16, f16,
+ * f32 or fp8 e4m3; D <= 256; any strides), block_table int32 [B,W] (logical page -> page), and
+ * context_lens int32 [B]. Entries outside [0,num_blocks) name no page: nothing is written
+ * there, and its tokens do not count. Lengths are cut to [0, W*block]. An fp8 cache holds
+ * x / k_scale and x / v_scale; the other types take scales of 1.
+ *
+ * bd_paged_append writes new tokens into their pages, the keys rotated by their position, and
+ * writes the rotated queries to q_out (q and q_out NULL: none). k,v [T,Hk,D], q,q_out [T,Hq,D]
+ * bf16/f16/f32 of one type, any strides. Token t belongs to sequence b with cu_seqlens[b] <= t <
+ * cu_seqlens[b+1] (int32 [B+1]; NULL: T = B, one token each); the last n_b tokens of a sequence
+ * are the new ones, so token i of them has position context_lens[b] - n_b + i. cos, sin f32
+ * [positions, r/2] (NULL: no rotation) rotate the first r channels by pairs (i, i + r/2), or
+ * (2i, 2i+1) if interleaved: y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin in fp32, each product and
+ * sum rounded. A token without a place (past cu_seqlens[B], a position below 0, past the block
+ * table or past the rows of cos, or no page) is not written and its q_out row is zeros.
+ *
+ * bd_paged_block_summary writes the 8-bit summary of pages' keys: summary i8 [num_blocks,Hk,2,D]
+ * (last two dims contiguous) holds rint(min / s) and rint(max / s) over the page's tokens of each
+ * channel of k_scale * key, summary_scale f32 [num_blocks,Hk] s = max|.| / 127. new_tokens = 0:
+ * every page that holds tokens; T > 0: the pages that the last T appended tokens (cu_seqlens as
+ * above) lie in.
+ *
+ * bd_paged_select chooses pages for one new token a sequence from the summaries. With q8 =
+ * rint(q * (127 / max|q|)), s_q = max|q| / 127 per query head: I = sum_d max(q8 min8, q8 max8),
+ * score(page) = (max over the KV head's query heads of float(I) * s_q) * s, in fp32. The first
+ * `sink` and last `recent` pages of a sequence are taken first, then the largest scores, the
+ * lower page on ties. selected int32 [B,Hk,budget]: logical pages in ascending order, -1 after
+ * the last.
+ *
+ * bd_paged_decode_attn: out [B,Hq,D] (bf16/f16/f32) = softmax(scaling * k_scale * q.k) . v *
+ * v_scale over a sequence's tokens, or over those of its chosen pages (selected int32
+ * [B,Hk,pages], NULL: all; entries that hold no token do not count, duplicates count once per
+ * occurrence). lse f32 [B,Hq] (may be NULL) = natural log of the softmax denominator. A row
+ * without a token gives zeros and lse = -inf. q [B,Hq,D] bf16/f16/f32.
+ * ref: none -- the reference pages its PQ caches only (paged_attn_pq_lut_kv,
+ *      src/attention_kernels.py:588); Quest's pages (benchmarks/sparse_attention.py:328-364) are
+ *      ranges of a contiguous cache, with a choice per query head. */
+int bd_paged_append(const bd_tensor* k, const bd_tensor* v, const bd_tensor* q, const bd_tensor* cos,
+                    const bd_tensor* sin, int interleaved, const bd_tensor* cu_seqlens, const bd_tensor* block_table,
+                    const bd_tensor* context_lens, float k_scale, float v_scale, const bd_tensor* k_cache,
+                    const bd_tensor* v_cache, const bd_tensor* q_out, bd_stream_t stream);
+int bd_paged_block_summary(const bd_tensor* k_cache, const bd_tensor* block_table, const bd_tensor* context_lens,
+                           const bd_tensor* cu_seqlens, int new_tokens, float k_scale, const bd_tensor* summary,
+                           const bd_tensor* summary_scale, bd_stream_t stream);
+size_t bd_paged_select_workspace(const bd_tensor* q, const bd_tensor* summary, const bd_tensor* block_table);
+int bd_paged_select(const bd_tensor* q, const bd_tensor* summary, const bd_tensor* summary_scale,
+                    const bd_tensor* block_table, const bd_tensor* context_lens, int block_size, int sink, int recent,
+                    const bd_tensor* selected, void* workspace, size_t workspace_bytes, bd_stream_t stream);
+size_t bd_paged_decode_attn_workspace(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_cache,
+                                      const bd_tensor* block_table, const bd_tensor* context_lens,
+                                      const bd_tensor* selected);
+int bd_paged_decode_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_cache,
+                         const bd_tensor* block_table, const bd_tensor* context_lens, const bd_tensor* selected,
+                         float scaling, float k_scale, float v_scale, const bd_tensor* out, const bd_tensor* lse,
+                         void* workspace, size_t workspace_bytes, bd_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
