@@ -8,6 +8,8 @@
 #include "decode_shared.cuh"
 
 #include <algorithm>
+#include <cfloat>
+#include <type_traits>
 
 namespace bd {
 
@@ -25,6 +27,8 @@ struct AttnParams {
   float scale_log2, v_scale;
   int n_splits; int64_t split_tokens;
   float* part_o; float* part_m; float* part_l;  // [B*Hq][n_splits]([D]); m in log2 units
+  // tile form: warps of the grid, its partials [2 * warps][heads]([D])
+  int warps, heads, block_shift;
   void* out; int out_dtype; int64_t o_sb, o_sh, o_sd;
   float* lse; int64_t e_sb, e_sh;
 };
@@ -130,6 +134,626 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const AttnParams p) {
   if (p.lse && threadIdx.x == 0) p.lse[b * p.e_sb + h * p.e_sh] = M == -INFINITY ? -INFINITY : M * kLn2 + logf(L);
 }
 
+// ------------------------------------------------------------------ tensor-core tiles
+//
+// The work is one list of 16-token units: for every sequence, every KV head (and chunk of 8 or 16
+// of its query heads), the units of its tokens, or of its chosen pages. Warp w of the grid's n takes
+// units [w T / n, (w + 1) T / n): equal shares whatever the lengths, which only the device knows. A
+// warp works alone, with no barrier of the CTA: its lane 0 brings units ahead of use into the warp's
+// own ring of shared memory by TMA (one box of a page's 16 rows for keys and one for values, 128-byte
+// swizzle, so that ldmatrix reads without bank conflicts), and each unit is
+//   S^T[16 x heads] = K Q^T, running maximum and sum, O^T[D x heads] += V^T P^T
+// in mma.sync m16n8k16 with 32-bit sums (the query heads of a KV head are the n of the product, so
+// every key and value is read once). Rows that a warp has whole are written at once; the others'
+// (maximum, sum, numerator) go to the workspace, two at most for a warp, and paged_join_kernel joins
+// them.
+
+constexpr int kUnit = 16;
+
+enum { kBf16 = 0, kF16 = 1, kFp8 = 2 };
+
+template <int D, int KIND>
+struct TileShape {
+  static constexpr int ELT = KIND == kFp8 ? 1 : 2;
+  static constexpr int ROWB = D * ELT;
+  static constexpr int SW = ROWB < 128 ? ROWB : 128;  // bytes of a row in one slab (the swizzle's span)
+  static constexpr int SLABS = ROWB / SW;
+  static constexpr int HALF = kUnit * ROWB;           // keys (or values) of a unit
+  static constexpr int WARPS = HALF * 2 > 8192 ? 4 : 8;
+  static constexpr int STAGES = (200 * 1024 / (WARPS * HALF * 2)) < 8 ? (200 * 1024 / (WARPS * HALF * 2)) : 8;
+  static constexpr int SMEM = WARPS * STAGES * HALF * 2 + WARPS * STAGES * 8 + 1024;
+};
+
+// waits on tile copies that ran past their limit (a result is then NaN)
+__device__ unsigned int g_paged_timeouts = 0;
+
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
+// Units of a row (one sequence and KV head), and of all rows.
+__device__ __forceinline__ int row_units(const AttnParams& p, int len) {
+  if (p.n_sel >= 0) return len > 0 ? int((int64_t(p.n_sel) * p.g.block + kUnit - 1) / kUnit) : 0;
+  return (len + kUnit - 1) / kUnit;
+}
+
+__device__ __forceinline__ int64_t total_units(const AttnParams& p, int lane) {
+  int64_t n = 0;
+  for (int b = lane; b < p.g.B; b += 32) n += row_units(p, paged_len(p.g, b));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n * (p.g.Hk * p.chunks);
+}
+
+// First unit of warp w's share.
+__device__ __forceinline__ int64_t share(int64_t total, int w, int n) {
+  const int64_t each = total / n, rest = total % n;
+  return each * w + min(int64_t(w), rest);
+}
+
+// Warp whose share holds unit u.
+__device__ __forceinline__ int owner(int64_t total, int64_t u, int n) {
+  const int64_t each = total / n, rest = total % n;
+  const int64_t cut = (each + 1) * rest;
+  return u < cut ? int(u / (each + 1)) : int(rest + (u - cut) / each);
+}
+
+// A place in the list of units.
+struct Place {
+  int b, hc, u, units, len;
+  // Goes to unit `at` of the list (a warp's lanes together).
+  __device__ __forceinline__ void find(const AttnParams& p, int64_t at, int lane) {
+    const int per = p.g.Hk * p.chunks;
+    for (int b0 = 0; b0 < p.g.B; b0 += 32) {
+      const int mine = b0 + lane < p.g.B ? paged_len(p.g, b0 + lane) : 0;
+      const int64_t n = int64_t(row_units(p, mine)) * per;
+      int64_t sum = n;  // inclusive prefix
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, sum > at);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        b = b0 + l;
+        len = __shfl_sync(0xffffffffu, mine, l);
+        const int64_t in = at - __shfl_sync(0xffffffffu, sum - n, l);
+        units = row_units(p, len);
+        hc = int(in / units);
+        u = int(in % units);
+        return;
+      }
+      at -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+  }
+  // Goes to the first unit of the next row that has any; there has to be one.
+  __device__ __forceinline__ void next_row(const AttnParams& p) {
+    u = 0;
+    if (++hc < p.g.Hk * p.chunks) return;
+    hc = 0;
+    do {
+      ++b;
+      len = paged_len(p.g, b);
+      units = row_units(p, len);
+    } while (units == 0 && b + 1 < p.g.B);
+  }
+};
+
+template <int D, int KIND, int NT>
+__global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
+    paged_attn_tile_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
+                           const __grid_constant__ CUtensorMap vmap) {
+  using T = TileShape<D, KIND>;
+  constexpr bool FP8 = KIND == kFp8;
+  constexpr int KSTEPS = D / 16, NH = 8 * NT;
+  // weights are kept 2^kUp above 1 where they are rounded to f16, so that small ones stay normal
+  constexpr float kUp = KIND == kBf16 ? 0.f : 14.f;
+  extern __shared__ uint8_t smem_raw[];
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + uint32_t(warp) * T::STAGES * 2 * T::HALF;
+  const uint32_t bars = ((smem_u32(smem_raw) + 1023u) & ~1023u) + uint32_t(T::WARPS) * T::STAGES * 2 * T::HALF +
+                        uint32_t(warp) * T::STAGES * 8;
+  const int w = blockIdx.x * T::WARPS + warp;
+  const int64_t total = total_units(p, lane);
+  const int64_t first = share(total, w, p.warps);
+  int left = int(share(total, w + 1, p.warps) - first);
+  if (left == 0) return;
+  if (lane < T::STAGES) mbar_init(bars + lane * 8, 1);
+  if (lane == 0) mbar_fence_init();
+  __syncwarp();
+
+  Place in;  // the next unit to bring in
+  in.find(p, first, lane);
+  Place at = in;  // the unit at hand
+  int to_issue = left;
+  // list positions held by the lanes: entry_first + lane of the row in.b, in.hc
+  int entry_first = -1, entry_page = -1, entry_logical = 0;
+  unsigned long long live = 0;  // a byte a stage: live rows of the unit's first and second eight
+  // rows of a box, and where in a unit's keys row r of slab c starts: (r / 8) * step8 + c * slab + (r % 8) * SW
+  const bool small_page = p.block_shift == 3;
+  const uint32_t step8 = (small_page ? T::SLABS : 1) * 8 * T::SW, slab = (small_page ? 8 : 16) * T::SW;
+
+  auto issue = [&](int stage) {
+    if (to_issue == 0) return;
+    const int idx = small_page ? in.u * 2 : in.u >> (p.block_shift - 4);
+    const int hk = in.hc / p.chunks;
+    if (entry_first < 0 || idx - entry_first >= 32) {
+      entry_first = idx;
+      int j = idx + lane;
+      if (p.n_sel >= 0)
+        j = j < p.n_sel ? p.selected[in.b * p.s_sb + hk * p.s_sh + j * p.s_si] : -1;
+      entry_logical = j;
+      entry_page = j >= 0 && j < p.g.wide && (int64_t(j) << p.block_shift) < in.len ? paged_block(p.g, in.b, j) : -1;
+    }
+    const uint32_t dst = ring + stage * 2 * T::HALF, bar = bars + stage * 8;
+    unsigned rows = 0;
+    if (!small_page) {
+      const int page = __shfl_sync(0xffffffffu, entry_page, idx - entry_first);
+      const int j = __shfl_sync(0xffffffffu, entry_logical, idx - entry_first);
+      const int off = (in.u & ((1 << (p.block_shift - 4)) - 1)) * kUnit;
+      const int64_t n = int64_t(in.len) - ((int64_t(j) << p.block_shift) + off);
+      if (page >= 0 && n > 0) {
+        rows = unsigned(n >= 8 ? 8 : n) | unsigned(n >= 16 ? 8 : n > 8 ? n - 8 : 0) << 4;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, 2 * T::HALF);
+          tma_load_5d(dst, &kmap, 0, off, 0, hk, page, bar);
+          tma_load_5d(dst + T::HALF, &vmap, 0, off, 0, hk, page, bar);
+        }
+      }
+    } else {
+      uint32_t bytes = 0;
+      int page[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        page[i] = __shfl_sync(0xffffffffu, entry_page, idx - entry_first + i);
+        const int j = __shfl_sync(0xffffffffu, entry_logical, idx - entry_first + i);
+        const int64_t n = int64_t(in.len) - (int64_t(j) << 3);
+        if (page[i] >= 0 && n > 0) {
+          rows |= unsigned(n >= 8 ? 8 : n) << (4 * i);
+          bytes += T::HALF;
+        } else {
+          page[i] = -1;
+        }
+      }
+      if (rows && lane == 0) {
+        mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (page[i] >= 0) {
+            tma_load_5d(dst + i * T::HALF / 2, &kmap, 0, 0, 0, hk, page[i], bar);
+            tma_load_5d(dst + T::HALF + i * T::HALF / 2, &vmap, 0, 0, 0, hk, page[i], bar);
+          }
+      }
+    }
+    if (!rows && lane == 0) mbar_arrive_expect_tx(bar, 0);  // nothing to bring: the phase ends at once
+    live = (live & ~(0xffull << (8 * stage))) | (static_cast<unsigned long long>(rows) << (8 * stage));
+    if (--to_issue && ++in.u == in.units) {
+      in.next_row(p);
+      entry_first = -1;
+    }
+  };
+
+#pragma unroll 1
+  for (int s = 0; s < T::STAGES; ++s) issue(s);
+
+  int stage = 0;
+  unsigned phase = 0;
+  bool lost = false;
+  const int64_t list_first = first;
+  int64_t seg_first = first;
+  while (left > 0) {
+    const int n = min(left, at.units - at.u);  // this warp's units of the row
+    const int hk = at.hc / p.chunks, h0 = (at.hc % p.chunks) * NH;
+    const int nheads = min(NH, p.G - h0);
+    // ---- query fragments (B operand of K Q^T)
+    uint32_t qb[KSTEPS][NT][2];
+    float mul = p.scale_log2;
+    {
+      float qv[KSTEPS][NT][4], amax = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int hl = nt * 8 + g;
+          const bool ok = hl < nheads;
+          const int64_t off = at.b * p.q_sb + int64_t(hk * p.G + h0 + (ok ? hl : 0)) * p.q_sh;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // 16-bit tiles: channels 2tq, 2tq+1, 2tq+8, 2tq+9 of a step; 8-bit: 4tq..4tq+3
+            const int c = FP8 ? kk * 16 + 4 * tq + e : kk * 16 + 2 * tq + (e & 1) + (e >> 1) * 8;
+            float x = 0.f;
+            if (ok) x = KIND == kBf16 ? to_f32(reinterpret_cast<const __nv_bfloat16*>(p.q)[off + c * p.q_sd])
+                                      : load_as(p.q, p.q_dtype, off + c * p.q_sd);
+            qv[kk][nt][e] = x;
+            amax = fmaxf(amax, fabsf(x));
+          }
+        }
+      float qscale = 1.f;
+      if (FP8) {  // a power of two that keeps |q| within f16 (exact)
+        amax = warp_max(amax);
+        int ex = 0;
+        frexpf(amax, &ex);
+        const int shift = ex > 15 && amax <= FLT_MAX ? ex - 15 : 0;
+        qscale = ldexpf(1.f, -shift);
+        mul = ldexpf(p.scale_log2, shift);
+      }
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            qb[kk][nt][i] = KIND == kBf16 ? pack_bf16x2(qv[kk][nt][2 * i], qv[kk][nt][2 * i + 1])
+                                          : pack_f16x2(qv[kk][nt][2 * i] * qscale, qv[kk][nt][2 * i + 1] * qscale);
+    }
+    float o[KSTEPS][NT][4], mrow[NT][2], lrow[NT][2];
+#pragma unroll
+    for (int mt = 0; mt < KSTEPS; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][nt][e] = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) mrow[nt][0] = mrow[nt][1] = -INFINITY, lrow[nt][0] = lrow[nt][1] = 0.f;
+
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      if (!lost && !mbar_wait(bars + stage * 8, phase)) {
+        lost = true;
+        to_issue = 0;
+        if (lane == 0) atomicAdd(&g_paged_timeouts, 1u);
+      }
+      lost = __any_sync(0xffffffffu, lost);
+      if (lost) break;
+      const unsigned rows = unsigned(live >> (8 * stage)) & 0xffu;
+      const int nv0 = rows & 15, nv1 = rows >> 4;
+      if (rows) {
+        const uint32_t ks = ring + stage * 2 * T::HALF, vs = ks + T::HALF;
+        if (rows != 0x88u) {
+          // rows past the sequence's end hold whatever was there: their weights are zero, and so must
+          // their values be (zero times infinity is not zero)
+          for (int e = lane; e < kUnit * T::ROWB / 16; e += 32) {
+            const int r = e / (T::ROWB / 16), c = e % (T::ROWB / 16);
+            const uint32_t a = vs + (r >> 3) * step8 + (c * 16 / T::SW) * slab + (r & 7) * T::SW + c * 16 % T::SW;
+            if ((r & 7) >= (r < 8 ? nv0 : nv1))  // whole rows: the swizzle moves chunks within a row only
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(a), "r"(0) : "memory");
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+        // ---- S^T = K Q^T
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+        // a lane's 16-byte chunk of its row is chunk ^ (row % 8) (128-byte rows), or
+        // chunk ^ (row / 2 % 4) (64-byte rows)
+        const uint32_t x = (T::SW == 128 ? lane & 7 : (lane >> 1) & 3) * 16;
+        {
+          const uint32_t base = ks + ((lane >> 3) & 1) * step8 + (lane & 7) * T::SW, hi = uint32_t(lane >> 4) * 16;
+#pragma unroll
+          for (int c = 0; c < T::ROWB / 32; ++c) {
+            uint32_t r0, r1, r2, r3;
+            ldmatrix_x4(r0, r1, r2, r3, base + (c * 32 / T::SW) * slab + ((c * 32 % T::SW) ^ (hi ^ x)));
+            if (!FP8) {
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                if (KIND == kBf16) mma_bf16(s[nt], r0, r1, r2, r3, qb[c][nt][0], qb[c][nt][1]);
+                else mma_f16(s[nt], r0, r1, r2, r3, qb[c][nt][0], qb[c][nt][1]);
+            } else {
+              const uint32_t x0 = e4m3x2_to_f16x2(r0), x1 = e4m3x2_to_f16x2(r1);
+              const uint32_t x2 = e4m3x2_to_f16x2(r0 >> 16), x3 = e4m3x2_to_f16x2(r1 >> 16);
+              const uint32_t y0 = e4m3x2_to_f16x2(r2), y1 = e4m3x2_to_f16x2(r3);
+              const uint32_t y2 = e4m3x2_to_f16x2(r2 >> 16), y3 = e4m3x2_to_f16x2(r3 >> 16);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_f16(s[nt], x0, x1, x2, x3, qb[2 * c % KSTEPS][nt][0], qb[2 * c % KSTEPS][nt][1]);
+                mma_f16(s[nt], y0, y1, y2, y3, qb[(2 * c + 1) % KSTEPS][nt][0], qb[(2 * c + 1) % KSTEPS][nt][1]);
+              }
+            }
+          }
+        }
+        // ---- running maximum and sum; P^T fragments
+        const bool v0 = g < nv0, v1 = g < nv1;
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float a[2], c[2], mx[2], pv[4];
+          bool grow = false;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            a[j] = v0 ? s[nt][j] * mul : -INFINITY;
+            c[j] = v1 ? s[nt][2 + j] * mul : -INFINITY;
+            mx[j] = fmaxf(a[j], c[j]);
+            grow |= mx[j] > mrow[nt][j];
+          }
+          if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 4));
+              mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 8));
+              mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 16));
+              const float mnew = fmaxf(mrow[nt][j], mx[j]);
+              const float alpha = mrow[nt][j] == -INFINITY ? 0.f : fast_exp2(mrow[nt][j] - mnew);
+              mrow[nt][j] = mnew;
+              lrow[nt][j] *= alpha;
+#pragma unroll
+              for (int mt = 0; mt < KSTEPS; ++mt) {
+                o[mt][nt][j] *= alpha;
+                o[mt][nt][2 + j] *= alpha;
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float ref = mrow[nt][j] == -INFINITY ? 0.f : mrow[nt][j] - kUp;
+            pv[j] = fast_exp2(a[j] - ref);
+            pv[2 + j] = fast_exp2(c[j] - ref);
+            lrow[nt][j] += pv[j] + pv[2 + j];
+          }
+          if (KIND == kBf16) {
+            pb[nt][0] = movmatrix_trans(pack_bf16x2(pv[0], pv[1]));
+            pb[nt][1] = movmatrix_trans(pack_bf16x2(pv[2], pv[3]));
+          } else {
+            pb[nt][0] = movmatrix_trans(pack_f16x2(pv[0], pv[1]));
+            pb[nt][1] = movmatrix_trans(pack_f16x2(pv[2], pv[3]));
+          }
+        }
+        // ---- O^T += V^T P^T
+        if (!FP8) {
+          const uint32_t base = vs + (lane >> 4) * step8 + (lane & 7) * T::SW, hi = uint32_t((lane >> 3) & 1) * 16;
+#pragma unroll
+          for (int mt = 0; mt < KSTEPS; ++mt) {
+            uint32_t a0, a1, a2, a3;
+            ldmatrix_x4_trans(a0, a1, a2, a3, base + (mt * 32 / T::SW) * slab + ((mt * 32 % T::SW) ^ (hi ^ x)));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              if (KIND == kBf16) mma_bf16(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+              else mma_f16(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+          }
+        } else {
+          const uint32_t base = vs + ((lane >> 3) & 1) * step8 + (lane & 7) * T::SW, hi = uint32_t(lane >> 4) * 16;
+#pragma unroll
+          for (int m2 = 0; m2 < KSTEPS / 2; ++m2) {
+            uint32_t r0, r1, r2, r3;
+            ldmatrix_x4_trans(r0, r1, r2, r3, base + (m2 * 32 / T::SW) * slab + ((m2 * 32 % T::SW) ^ (hi ^ x)));
+            // r0, r1: tokens 0-7, 8-15 of channels [32 m2, +16); r2, r3: of the next 16; each holds
+            // (token 2tq: channels 2g, 2g+1 | token 2tq+1: the same)
+            const uint32_t a0 = e4m3x2_to_f16x2(prmt(r0, 0, 0x0020)), a1 = e4m3x2_to_f16x2(prmt(r0, 0, 0x0031));
+            const uint32_t a2 = e4m3x2_to_f16x2(prmt(r1, 0, 0x0020)), a3 = e4m3x2_to_f16x2(prmt(r1, 0, 0x0031));
+            const uint32_t c0 = e4m3x2_to_f16x2(prmt(r2, 0, 0x0020)), c1 = e4m3x2_to_f16x2(prmt(r2, 0, 0x0031));
+            const uint32_t c2 = e4m3x2_to_f16x2(prmt(r3, 0, 0x0020)), c3 = e4m3x2_to_f16x2(prmt(r3, 0, 0x0031));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(o[2 * m2][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+              mma_f16(o[2 * m2 + 1][nt], c0, c1, c2, c3, pb[nt][0], pb[nt][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();  // the unit is read: its place may be filled again
+      issue(stage);
+      if (++stage == T::STAGES) stage = 0, phase ^= 1;
+    }
+
+    // ---- the row's result, or this warp's part of it
+    const bool whole = n == at.units;
+    const int64_t slot = 2 * int64_t(w) + (seg_first != list_first);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float l = lrow[nt][j];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        if (lost) l = NAN;
+        const int h = nt * 8 + 2 * tq + j;
+        if (h >= nheads) continue;
+        const float m = lost ? 0.f : mrow[nt][j] - kUp;  // of sums that are 2^kUp times as large
+        if (whole) {
+          const int hq = hk * p.G + h0 + h;
+          const float f = m == -INFINITY ? 0.f : p.v_scale / l;
+          const int64_t off = at.b * p.o_sb + int64_t(hq) * p.o_sh;
+#pragma unroll
+          for (int mt = 0; mt < KSTEPS; ++mt) {
+            const int ca = FP8 ? mt * 16 + 2 * g : mt * 16 + g, cb = FP8 ? ca + 1 : ca + 8;
+            store_as(p.out, p.out_dtype, off + ca * p.o_sd, o[mt][nt][j] * f);
+            store_as(p.out, p.out_dtype, off + cb * p.o_sd, o[mt][nt][2 + j] * f);
+          }
+          if (p.lse && g == 0)
+            p.lse[at.b * p.e_sb + hq * p.e_sh] = m == -INFINITY ? -INFINITY : m * kLn2 + logf(l);
+        } else {
+          float* po = p.part_o + (slot * NH + h) * D;
+#pragma unroll
+          for (int mt = 0; mt < KSTEPS; ++mt) {
+            const int ca = FP8 ? mt * 16 + 2 * g : mt * 16 + g, cb = FP8 ? ca + 1 : ca + 8;
+            po[ca] = o[mt][nt][j];
+            po[cb] = o[mt][nt][2 + j];
+          }
+          if (g == 0) {
+            p.part_m[slot * NH + h] = m;
+            p.part_l[slot * NH + h] = l;
+          }
+        }
+      }
+    left -= n;
+    seg_first += n;
+    if (left > 0) at.next_row(p);
+  }
+  // a copy that was given up is still waited for (again with a limit) before the memory goes
+  if (lost)
+    for (int s = 0; s < T::STAGES; ++s) mbar_wait(bars + s * 8, s < stage ? phase ^ 1 : phase);
+}
+
+// Joins the parts of the rows that more than one warp had, and writes the rows that have no token.
+// One CTA per (query head, sequence); a thread has 4 channels of every eighth (D = 64), fourth or
+// second (256) part.
+constexpr int kJoinThreads = 128;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) paged_tile_join_kernel(const AttnParams p) {
+  constexpr int PER = D / 4, SLICES = kJoinThreads / PER;
+  __shared__ float4 red[SLICES][PER];
+  const int hq = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31;
+  const int hk = hq / p.G, hl = hq % p.G, hc = hk * p.chunks + hl / p.heads, h = hl % p.heads;
+  const int units = row_units(p, paged_len(p.g, b));
+  const int64_t out = b * p.o_sb + hq * p.o_sh;
+  const int part = threadIdx.x % PER, slice = threadIdx.x / PER;
+  if (units == 0) {
+    if (slice == 0)
+      for (int i = 0; i < 4; ++i) store_as(p.out, p.out_dtype, out + (4 * part + i) * p.o_sd, 0.f);
+    if (p.lse && threadIdx.x == 0) p.lse[b * p.e_sb + hq * p.e_sh] = -INFINITY;
+    griddep_wait();  // a kernel that waits for this one then finds the tile kernel done as well
+    return;
+  }
+  // units of all sequences, and of those before this one
+  int64_t all = 0, before = 0;
+  for (int i = lane; i < p.g.B; i += 32) {
+    const int n = row_units(p, paged_len(p.g, i));
+    all += n;
+    if (i < b) before += n;
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, s);
+    before += __shfl_xor_sync(0xffffffffu, before, s);
+  }
+  const int per = p.g.Hk * p.chunks;
+  all *= per;
+  const int64_t u0 = before * per + int64_t(hc) * units;
+  const int w0 = owner(all, u0, p.warps), w1 = owner(all, u0 + units - 1, p.warps);
+  griddep_wait();
+  if (w0 == w1) return;  // one warp had the whole row
+  auto slot = [&](int w) { return (2 * int64_t(w) + (share(all, w, p.warps) < u0)) * p.heads + h; };
+  float M = -INFINITY;
+  for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, p.part_m[slot(w)]);
+  M = warp_max(M);
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int w = w0 + slice; w <= w1; w += SLICES) {
+    const int64_t s = slot(w);
+    const float m = p.part_m[s], f = m == -INFINITY ? 0.f : exp2f(m - M);
+    const float4 x = reinterpret_cast<const float4*>(p.part_o + s * D)[part];
+    L = fmaf(p.part_l[s], f, L);
+    acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
+    acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+  }
+  __shared__ float sums[SLICES];
+  red[slice][part] = acc;
+  if (part == 0) sums[slice] = L;
+  __syncthreads();
+  if (slice) return;
+  for (int i = 1; i < SLICES; ++i) {
+    const float4 x = red[i][part];
+    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+    L += sums[i];
+  }
+  const float f = M == -INFINITY ? 0.f : p.v_scale / L;
+  store_as(p.out, p.out_dtype, out + 4 * part * p.o_sd, acc.x * f);
+  store_as(p.out, p.out_dtype, out + (4 * part + 1) * p.o_sd, acc.y * f);
+  store_as(p.out, p.out_dtype, out + (4 * part + 2) * p.o_sd, acc.z * f);
+  store_as(p.out, p.out_dtype, out + (4 * part + 3) * p.o_sd, acc.w * f);
+  if (p.lse && part == 0) p.lse[b * p.e_sb + hq * p.e_sh] = M == -INFINITY ? -INFINITY : M * kLn2 + logf(L);
+}
+
+// Whether the tiles can take a call: 16-bit queries and caches of one type, or 8-bit caches; pages of
+// 8, 16, 32, ... tokens; rows that TMA can address.
+bool tile_layout(const bd_tensor* t) {
+  const size_t es = dtype_size(t->dtype);
+  if ((reinterpret_cast<uintptr_t>(t->data) & 15) || t->stride[3] != 1) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t->shape[i] > 1 && (t->stride[i] <= 0 || (size_t(t->stride[i]) * es) % 16 ||
+                            size_t(t->stride[i]) * es >= (size_t(1) << 40)))
+      return false;
+  return true;
+}
+
+bool use_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v_cache) {
+  const int D = p.g.D;
+  if (D != 64 && D != 128 && D != 256) return false;
+  const bool types = (p.kv_dtype == BD_BF16 && p.q_dtype == BD_BF16) || (p.kv_dtype == BD_F16 && p.q_dtype == BD_F16) ||
+                     (p.kv_dtype == BD_F8E4M3 && p.q_dtype != BD_F32);
+  if (!types || p.g.block < 8 || p.g.block > 65536 || (p.g.block & (p.g.block - 1))) return false;
+  return p.g.num_blocks > 0 && tile_layout(k_cache) && tile_layout(v_cache);
+}
+
+// Warps of the grid: the CTAs fill the GPU once, if the block table has work for them.
+void plan_tiles(AttnParams* p, int warps_per_cta) {
+  p->heads = p->G > 8 && p->g.D <= 128 ? 16 : 8;
+  p->chunks = (p->G + p->heads - 1) / p->heads;
+  const int64_t tokens = int64_t(p->n_sel >= 0 ? p->n_sel : p->g.wide) * p->g.block;
+  const int64_t units = (tokens + kUnit - 1) / kUnit * p->g.B * p->g.Hk * p->chunks;
+  const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(num_sms(), units));
+  p->warps = int(ctas) * warps_per_cta;
+  p->block_shift = 31 - __builtin_clz(unsigned(p->g.block));
+}
+
+size_t tile_bytes(const AttnParams& p) {
+  return size_t(2) * p.warps * p.heads * (size_t(p.g.D) + 2) * sizeof(float) + 256;
+}
+
+bool tile_map(CUtensorMap* m, const bd_tensor* t, int sw) {
+  const size_t es = dtype_size(t->dtype);
+  const int rowb = int(t->shape[3] * es), slabs = rowb / sw, box_rows = t->shape[2] < kUnit ? int(t->shape[2]) : kUnit;
+  const cuuint64_t dims[5] = {cuuint64_t(sw / es), cuuint64_t(t->shape[2]), cuuint64_t(slabs), cuuint64_t(t->shape[1]),
+                              cuuint64_t(t->shape[0])};
+  // the stride of a dim of one entry is free: give it one that TMA takes
+  auto st = [&](int i) { return cuuint64_t(t->shape[i] > 1 ? t->stride[i] * es : rowb); };
+  const cuuint64_t strides[4] = {st(2), cuuint64_t(sw), st(1), st(0)};
+  const cuuint32_t box[5] = {cuuint32_t(sw / es), cuuint32_t(box_rows), cuuint32_t(slabs), 1, 1};
+  const CUtensorMapDataType dt = t->dtype == BD_F8E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : t->dtype == BD_F16  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode_map(m, dt, 5, t->data, dims, strides, box,
+                    sw == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+template <int D, int KIND, int NT>
+int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v_cache, cudaStream_t st) {
+  using T = TileShape<D, KIND>;
+  CUtensorMap km, vm;
+  if (!tile_map(&km, k_cache, T::SW) || !tile_map(&vm, v_cache, T::SW))
+    return fail(BD_ERR_CUDA, "cuTensorMapEncodeTiled refused the cache's layout");
+  auto kern = paged_attn_tile_kernel<D, KIND, NT>;
+  static bool set[64] = {false};  // dynamic shared memory allowed, per device
+  int dev = 0, rc;
+  cudaGetDevice(&dev);
+  if (!set[dev & 63]) {
+    if ((rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM),
+                         "cudaFuncSetAttribute(paged_attn_tile_kernel)")))
+      return rc;
+    set[dev & 63] = true;
+  }
+  kern<<<p.warps / T::WARPS, T::WARPS * 32, T::SMEM, st>>>(p, km, vm);
+  if ((rc = cuda_check(cudaGetLastError(), "paged_attn_tile_kernel launch"))) return rc;
+  return launch_programmatic(paged_tile_join_kernel<D>, dim3(p.Hq, p.g.B), dim3(kJoinThreads), 0, st, p,
+                             "paged_tile_join_kernel launch");
+}
+
+template <int D, int KIND>
+int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v_cache, cudaStream_t st) {
+  if constexpr (D <= 128)
+    if (p.heads == 16) return launch_tiles<D, KIND, 2>(p, k_cache, v_cache, st);
+  return launch_tiles<D, KIND, 1>(p, k_cache, v_cache, st);
+}
+
+template <int D>
+int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v_cache, cudaStream_t st) {
+  switch (p.kv_dtype) {
+    case BD_BF16: return launch_tiles<D, kBf16>(p, k_cache, v_cache, st);
+    case BD_F16: return launch_tiles<D, kF16>(p, k_cache, v_cache, st);
+    default: return launch_tiles<D, kFp8>(p, k_cache, v_cache, st);
+  }
+}
+
+int tile_warps(int D, int kv_dtype) {
+  auto of = [&](auto d) {
+    constexpr int N = decltype(d)::value;
+    return kv_dtype == BD_F8E4M3 ? TileShape<N, kFp8>::WARPS : TileShape<N, kBf16>::WARPS;
+  };
+  return D == 64 ? of(std::integral_constant<int, 64>()) : D == 128 ? of(std::integral_constant<int, 128>())
+                                                                   : of(std::integral_constant<int, 256>());
+}
+
 // Splits of the generic form: about four CTAs an SM, of 64 tokens at least.
 void plan_generic(AttnParams* p) {
   const int64_t cap = int64_t(p->n_sel >= 0 ? p->n_sel : p->g.wide) * p->g.block;
@@ -173,6 +797,13 @@ int check_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_
 }
 
 }  // namespace
+
+// host read of this file's wait-timeout counter (-1 on failure)
+long long paged_wait_timeouts() {
+  unsigned int v = 0;
+  return cudaMemcpyFromSymbol(&v, g_paged_timeouts, sizeof v) == cudaSuccess ? (long long)v : -1;
+}
+
 }  // namespace bd
 
 extern "C" {
@@ -186,6 +817,11 @@ size_t bd_paged_decode_attn_workspace(const bd_tensor* q, const bd_tensor* k_cac
     AttnParams p{};
     const int rc = check_attn(q, k_cache, v_cache, block_table, context_lens, selected, &p);
     if (rc) return rc;
+    if (use_tiles(p, k_cache, v_cache)) {
+      plan_tiles(&p, tile_warps(p.g.D, p.kv_dtype));
+      n = tile_bytes(p);
+      return BD_OK;
+    }
     plan_generic(&p);
     n = join_bytes(p);
     return BD_OK;
@@ -220,12 +856,19 @@ int bd_paged_decode_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_
     p.scale_log2 = scaling * k_scale * kLog2e;
     p.v_scale = v_scale;
     if (p.g.B == 0) return BD_OK;
-    plan_generic(&p);
-    const size_t need = join_bytes(p);
+    const bool tiles = use_tiles(p, k_cache, v_cache);
+    if (tiles) plan_tiles(&p, tile_warps(p.g.D, p.kv_dtype));
+    else plan_generic(&p);
+    const size_t need = tiles ? tile_bytes(p) : join_bytes(p);
     if (!workspace || workspace_bytes < need)
       return fail(BD_ERR_WORKSPACE, "need " + std::to_string(need) + " workspace bytes");
-    const Partials part = carve_partials(workspace, size_t(p.g.B) * p.Hq, p.n_splits, p.g.D);
+    const Partials part = tiles ? carve_partials(workspace, size_t(2) * p.warps * p.heads, 1, p.g.D)
+                                : carve_partials(workspace, size_t(p.g.B) * p.Hq, p.n_splits, p.g.D);
     p.part_o = part.o; p.part_m = part.m; p.part_l = part.l;
+    if (tiles)
+      return p.g.D == 64    ? launch_tiles<64>(p, k_cache, v_cache, stream)
+             : p.g.D == 128 ? launch_tiles<128>(p, k_cache, v_cache, stream)
+                            : launch_tiles<256>(p, k_cache, v_cache, stream);
     if (int64_t(p.g.Hk) * p.chunks > 65535) return fail(BD_ERR_SHAPE, "more than 65535 head chunks");
     paged_attn_generic_kernel<<<dim3(p.n_splits, p.g.Hk * p.chunks, p.g.B), kGenWarps * 32, 0, stream>>>(p);
     if ((rc = cuda_check(cudaGetLastError(), "paged_attn_generic_kernel launch"))) return rc;
