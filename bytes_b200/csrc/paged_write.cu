@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 namespace bd {
 
@@ -70,25 +71,34 @@ struct AppendParams {
   const float* cos; const float* sin; int64_t c_s, s_s; int positions, half, interleaved;
   const int* cu;
   float k_inv, v_inv;
+  int parts, each;  // vector form: warps of a token, and how often each goes on to further heads
 };
 
-// Sequence of packed token t: cu[s] <= t < cu[s + 1], or -1 past the last one.
+// Sequence of packed token t: cu[s] <= t < cu[s + 1], or -1 past the last one. The lanes of a warp ask
+// together, for one t: each step cuts the range by 32.
 __device__ __forceinline__ int sequence_of(const int* cu, int B, int t) {
-  if (t < cu[0] || t >= cu[B]) return -1;
+  if (B == 0 || t < cu[0] || t >= cu[B]) return -1;
+  const int lane = threadIdx.x & 31;
   int lo = 0, hi = B;  // cu[lo] <= t < cu[hi]
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid;
+    const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, i < hi && cu[i] <= t);
+    lo += (__popc(below) - 1) * step;
+    hi = min(hi, lo + step);
   }
   return lo;
 }
 
-// Page-table position of packed token t: (sequence, position), position -1 if it has no place.
+// Position of packed token t of sequence s (t < 0: of its newest token): -1 if it has no place.
+__device__ __forceinline__ int position_of(const PagedGeometry& g, const int* cu, int s, int t) {
+  const int64_t pos = int64_t(g.lens[int64_t(s) * g.l_s]) - (cu && t >= 0 ? int64_t(cu[s + 1]) - t : 1);
+  return pos < 0 || pos >= int64_t(g.wide) * g.block ? -1 : int(pos);
+}
+
+// (sequence, position) of packed token t, for a warp together.
 __device__ __forceinline__ int2 place_of(const PagedGeometry& g, const int* cu, int t) {
   const int s = cu ? sequence_of(cu, g.B, t) : t;
-  if (s < 0) return make_int2(-1, -1);
-  const int64_t pos = int64_t(g.lens[int64_t(s) * g.l_s]) - (cu ? int64_t(cu[s + 1]) - t : 1);
-  return make_int2(s, pos < 0 || pos >= int64_t(g.wide) * g.block ? -1 : int(pos));
+  return s < 0 ? make_int2(-1, -1) : make_int2(s, position_of(g, cu, s, t));
 }
 
 __device__ __forceinline__ void store_cache(void* base, int dt, int64_t off, float x, float inv) {
@@ -99,8 +109,8 @@ __device__ __forceinline__ void store_cache(void* base, int dt, int64_t off, flo
     store_as(base, dt, off, x);
 }
 
-// One CTA per token.
-__global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p) {
+// Any type, stride and head dim: one CTA per token, a thread a channel.
+__global__ void __launch_bounds__(128) paged_append_generic_kernel(const AppendParams p) {
   const int t = blockIdx.x;
   const int2 place = place_of(p.g, p.cu, t);
   int page = -1;
@@ -136,6 +146,169 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const AppendParams p)
   }
 }
 
+// Eight channels as 32-bit numbers, from and to each type.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+  static __device__ __forceinline__ void load(const void* p, float* x) {
+    const float4 a = __ldg(static_cast<const float4*>(p)), b = __ldg(static_cast<const float4*>(p) + 1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+  static __device__ __forceinline__ void store(void* p, const float* x) {
+    static_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    static_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+};
+template <> struct Eight<__nv_bfloat16> {
+  static __device__ __forceinline__ void load(const void* p, float* x) {
+    const uint4 a = __ldg(static_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void store(void* p, const float* x) {
+    *static_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                         pack_bf16x2(x[6], x[7]));
+  }
+};
+template <> struct Eight<__half> {
+  static __device__ __forceinline__ void load(const void* p, float* x) {
+    const uint4 a = __ldg(static_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x; x[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ void store(void* p, const float* x) {
+    *static_cast<uint4*>(p) = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]),
+                                         pack_f16x2(x[6], x[7]));
+  }
+};
+template <> struct Eight<__nv_fp8_e4m3> {
+  static __device__ __forceinline__ void store(void* p, const float* x) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+      w[i] = lo | hi << 16;
+    }
+    *static_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+};
+
+// Vector form. An item is 16 channels of one head of one token, two loads and two stores of eight: the
+// pairs' first and second halves (8c.., r/2 + 8c..), or 16 neighbours where pairs are neighbours or
+// nothing turns. A head has D / 16 items, a power of two up to 16, so a lane has the same channels of
+// every head it visits and holds their eight cosines and sines in registers. A warp takes one token's
+// items it, it + 1, ... `each` times; the heads run over queries, keys and values.
+constexpr int kAppendWarps = 8;
+
+template <typename TI, typename TC>
+__global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(const AppendParams p) {
+  const int64_t w = int64_t(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, t = int(w / p.parts), part = int(w % p.parts);
+  if (t >= p.T) return;
+  const int2 place = place_of(p.g, p.cu, t);
+  const int pos = place.y;
+  int page = -1;
+  if (pos >= 0 && (!p.cos || pos < p.positions)) page = paged_block(p.g, place.x, pos / p.g.block);
+  const int row = page >= 0 ? pos % p.g.block : 0;
+  const int items = p.g.D >> 4, shift = __ffs(items) - 1, c = lane & (items - 1), heads = 32 >> shift;
+  const bool turns = p.cos && 16 * c < 2 * p.half;
+  float cs[8], sn[8];
+  if (turns && page >= 0) {
+    Eight<float>::load(p.cos + int64_t(pos) * p.c_s + 8 * c, cs);
+    Eight<float>::load(p.sin + int64_t(pos) * p.s_s + 8 * c, sn);
+  }
+  const bool apart = turns && !p.interleaved;
+  const int a_off = apart ? 8 * c : 16 * c, b_off = apart ? p.half + 8 * c : 16 * c + 8;
+  const int all = p.q.H + p.k.H + p.v.H;
+  const int first = part * p.each * heads + (lane >> shift);
+#pragma unroll 4
+  for (int i = 0; i < p.each; ++i) {
+    int h = first + i * heads;
+    if (h >= all) break;
+    const bool is_q = h < p.q.H, is_v = h >= p.q.H + p.k.H;
+    if (!is_q && page < 0) break;
+    h -= is_q ? 0 : is_v ? p.q.H + p.k.H : p.q.H;
+    const TI* src = is_q   ? static_cast<const TI*>(p.q.data) + t * p.q.st + h * p.q.sh
+                    : is_v ? static_cast<const TI*>(p.v.data) + t * p.v.st + h * p.v.sh
+                           : static_cast<const TI*>(p.k.data) + t * p.k.st + h * p.k.sh;
+    float x[16], y[16];
+    Eight<TI>::load(src + a_off, x);
+    Eight<TI>::load(src + b_off, x + 8);
+    if (!turns || is_v) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[e] = x[e];
+    } else if (p.interleaved) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[2 * e] = __fsub_rn(__fmul_rn(x[2 * e], cs[e]), __fmul_rn(x[2 * e + 1], sn[e]));
+        y[2 * e + 1] = __fadd_rn(__fmul_rn(x[2 * e + 1], cs[e]), __fmul_rn(x[2 * e], sn[e]));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = __fsub_rn(__fmul_rn(x[e], cs[e]), __fmul_rn(x[8 + e], sn[e]));
+        y[8 + e] = __fadd_rn(__fmul_rn(x[8 + e], cs[e]), __fmul_rn(x[e], sn[e]));
+      }
+    }
+    if (is_q) {
+      if (page < 0)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = 0.f;
+      TI* dst = static_cast<TI*>(p.q_out) + t * p.o_st + h * p.o_sh;
+      Eight<TI>::store(dst + a_off, y);
+      Eight<TI>::store(dst + b_off, y + 8);
+    } else {
+      if (sizeof(TC) == 1) {
+        const float inv = is_v ? p.v_inv : p.k_inv;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = __fmul_rn(y[e], inv);
+      }
+      TC* dst = is_v ? static_cast<TC*>(p.v_cache) + page * p.g.v_sb + h * p.g.v_sh + row * p.g.v_st
+                     : static_cast<TC*>(p.k_cache) + page * p.g.k_sb + h * p.g.k_sh + row * p.g.k_st;
+      Eight<TC>::store(dst + a_off, y);
+      Eight<TC>::store(dst + b_off, y + 8);
+    }
+  }
+}
+
+// Warps that the vector form spreads a call over before it gives each of them more items of its token:
+// about 16 an SM.
+int launch_append(AppendParams p, cudaStream_t st) {
+  const int heads = 32 / (p.g.D >> 4), all = (p.q.H + 2 * p.k.H + heads - 1) / heads;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(all, int64_t(16) * num_sms() / p.T));
+  p.each = int((all + parts - 1) / parts);
+  p.parts = (all + p.each - 1) / p.each;
+  const int64_t ctas = (int64_t(p.T) * p.parts + kAppendWarps - 1) / kAppendWarps;
+  auto go = [&](auto kern) {
+    kern<<<unsigned(ctas), kAppendWarps * 32, 0, st>>>(p);
+    return cuda_check(cudaGetLastError(), "paged_append_kernel launch");
+  };
+  auto with = [&](auto in) {
+    using TI = decltype(in);
+    switch (p.cache_dtype) {
+      case BD_BF16: return go(paged_append_kernel<TI, __nv_bfloat16>);
+      case BD_F16: return go(paged_append_kernel<TI, __half>);
+      case BD_F8E4M3: return go(paged_append_kernel<TI, __nv_fp8_e4m3>);
+      default: return go(paged_append_kernel<TI, float>);
+    }
+  };
+  return p.in_dtype == BD_BF16 ? with(__nv_bfloat16()) : p.in_dtype == BD_F16 ? with(__half()) : with(float());
+}
+
+// Rows of contiguous channels on boundaries of eight of them (16 bytes at most).
+bool by_eight(const bd_tensor* t) {
+  const size_t es = dtype_size(t->dtype), align = std::min<size_t>(16, 8 * es);
+  if (reinterpret_cast<uintptr_t>(t->data) % align || t->stride[t->ndim - 1] != 1) return false;
+  for (int i = 0; i + 1 < t->ndim; ++i)
+    if (t->shape[i] > 1 && size_t(t->stride[i]) * es % align) return false;
+  return true;
+}
+
 struct SummaryParams {
   PagedGeometry g;
   const void* k_cache; int dtype;
@@ -145,27 +318,55 @@ struct SummaryParams {
   const int* cu; int T;  // T > 0: only the pages of the last appended tokens
 };
 
-// One warp per (page, KV head).
-__global__ void __launch_bounds__(128) paged_summary_kernel(const SummaryParams p) {
+// Which page a warp summarises: item / Hk counts the pages. All pages: (sequence, column of the block
+// table). Pages of the last T appended tokens: of every sequence its first and last touched page, then
+// the page of every block-th packed token where that is neither (whole pages between the two hold
+// exactly one such token). Sets b and j; false: nothing to do.
+__device__ __forceinline__ bool page_of_item(const SummaryParams& p, int64_t item, int& b, int& j) {
+  if (p.T == 0) {
+    b = int(item / p.g.wide); j = int(item % p.g.wide);
+    return b < p.g.B;
+  }
+  if (!p.cu) {
+    b = int(item);
+    if (b >= p.g.B) return false;
+    const int pos = position_of(p.g, p.cu, b, -1);
+    j = pos / p.g.block;
+    return pos >= 0;
+  }
+  const bool edge = item < 2 * int64_t(p.g.B);
+  const int64_t t = edge ? 0 : (item - 2 * int64_t(p.g.B)) * p.g.block;
+  if (!edge && t >= p.T) return false;
+  b = edge ? int(item >> 1) : sequence_of(p.cu, p.g.B, int(t));
+  if (b < 0 || p.cu[b + 1] <= p.cu[b]) return false;
+  const int last = position_of(p.g, p.cu, b, p.cu[b + 1] - 1);
+  // the first touched page is that of the first new token with a place
+  const int n = p.cu[b + 1] - p.cu[b];
+  const int64_t start = int64_t(p.g.lens[int64_t(b) * p.g.l_s]) - n;
+  const int first_page = int(max(start, int64_t(0)) / p.g.block);
+  const int last_page = last >= 0 ? last / p.g.block : (start + n > 0 ? p.g.wide - 1 : -1);
+  if (last_page < first_page) return false;
+  if (edge) {
+    j = item & 1 ? last_page : first_page;
+    return !(item & 1) || last_page != first_page;
+  }
+  const int pos = position_of(p.g, p.cu, b, int(t));
+  j = pos / p.g.block;
+  return pos >= 0 && j != first_page && j != last_page;
+}
+
+__device__ __forceinline__ int8_t code_of(float x, float s, bool some) {
+  return some ? int8_t(max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))))) : int8_t(0);
+}
+
+// Any type, stride and head dim: one warp per (page, KV head), a lane every 32nd channel.
+__global__ void __launch_bounds__(128) paged_summary_generic_kernel(const SummaryParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int h = int(w % p.g.Hk);
-  const int64_t item = w / p.g.Hk;
   int b, j;
-  if (p.T > 0) {
-    if (item >= p.T) return;
-    const int2 at = place_of(p.g, p.cu, int(item));
-    if (at.y < 0) return;
-    // the first appended token of each page acts for it
-    const bool first = at.y % p.g.block == 0 || !p.cu || item == p.cu[at.x];
-    // a token before it may have had no place (a position below zero)
-    if (!first) return;
-    b = at.x; j = at.y / p.g.block;
-  } else {
-    if (item >= int64_t(p.g.B) * p.g.wide) return;
-    b = int(item / p.g.wide); j = int(item % p.g.wide);
-  }
-  const int n = min(p.g.block, paged_len(p.g, b) - j * p.g.block);
+  if (!page_of_item(p, w / p.g.Hk, b, j)) return;
+  const int n = min(int64_t(p.g.block), paged_len(p.g, b) - int64_t(j) * p.g.block);
   if (n <= 0) return;
   const int page = paged_block(p.g, b, j);
   if (page < 0) return;
@@ -189,12 +390,133 @@ __global__ void __launch_bounds__(128) paged_summary_kernel(const SummaryParams 
   for (int i = 0; i < 8; ++i) {
     const int d = lane + 32 * i;
     if (d >= p.g.D) continue;
-    const int a = top > 0.f ? __float2int_rn(__fdiv_rn(lo[i], s)) : 0;
-    const int c = top > 0.f ? __float2int_rn(__fdiv_rn(hi[i], s)) : 0;
-    code[d] = int8_t(max(-127, min(127, a)));
-    code[p.g.D + d] = int8_t(max(-127, min(127, c)));
+    code[d] = code_of(lo[i], s, top > 0.f);
+    code[p.g.D + d] = code_of(hi[i], s, top > 0.f);
   }
   if (lane == 0) p.scale[page * p.s_sb + h * p.s_sh] = s;
+}
+
+// Minima and maxima by pairs in the cache's 16-bit type (8-bit ones as f16, which holds them all).
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> {
+  using V = __nv_bfloat162;
+  static __device__ __forceinline__ V bits(uint32_t x) { return *reinterpret_cast<V*>(&x); }
+  static __device__ __forceinline__ float2 wide(V x) { return __bfloat1622float2(x); }
+};
+template <> struct Pair<__half> {
+  using V = __half2;
+  static __device__ __forceinline__ V bits(uint32_t x) { return *reinterpret_cast<V*>(&x); }
+  static __device__ __forceinline__ float2 wide(V x) { return __half22float2(x); }
+};
+
+// 16- and 8-bit caches with 16-byte aligned rows: one warp per (page, KV head). A row is LPR lanes of 16
+// bytes, so a load instruction takes 32 / LPR rows; eight are in flight at a time. The row groups
+// then meet by shuffles; the first of them writes the minima, the second the maxima.
+template <typename T, bool FP8, int LPR>
+__global__ void __launch_bounds__(256) paged_summary_kernel(const SummaryParams p) {
+  using P = Pair<T>;
+  using V = typename P::V;
+  constexpr int NP = FP8 ? 8 : 4, GROUPS = 32 / LPR, D = LPR * NP * 2;
+  const int lane = threadIdx.x & 31, part = lane % LPR, group = lane / LPR;
+  const int64_t w = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int h = int(w % p.g.Hk);
+  int b, j;
+  if (!page_of_item(p, w / p.g.Hk, b, j)) return;
+  const int n = int(min(int64_t(p.g.block), paged_len(p.g, b) - int64_t(j) * p.g.block));
+  if (n <= 0) return;
+  const int page = paged_block(p.g, b, j);
+  if (page < 0) return;
+  constexpr int ES = FP8 ? 1 : 2;
+  const uint8_t* base = static_cast<const uint8_t*>(p.k_cache) + (page * p.g.k_sb + h * p.g.k_sh) * ES + part * 16;
+  V lo[NP], hi[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    lo[i] = P::bits(std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u);
+    hi[i] = P::bits(std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
+  }
+  for (int r0 = 0; r0 < n; r0 += 8 * GROUPS) {
+    uint4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // rows past the last are read as the last one again
+      const int r = min(r0 + i * GROUPS + group, n - 1);
+      x[i] = *reinterpret_cast<const uint4*>(base + int64_t(r) * p.g.k_st * ES);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int e = 0; e < NP; ++e) {
+        const V v = P::bits(FP8 ? e4m3x2_to_f16x2(u[e / 2] >> (16 * (e & 1))) : u[e]);
+        lo[e] = __hmin2(lo[e], v);
+        hi[e] = __hmax2(hi[e], v);
+      }
+    }
+  }
+  float lof[2 * NP], hif[2 * NP], top = 0.f;
+#pragma unroll
+  for (int e = 0; e < NP; ++e) {
+#pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) {
+      lo[e] = __hmin2(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
+      hi[e] = __hmax2(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
+    }
+    const float2 a = P::wide(lo[e]), c = P::wide(hi[e]);
+    lof[2 * e] = __fmul_rn(a.x, p.k_scale); lof[2 * e + 1] = __fmul_rn(a.y, p.k_scale);
+    hif[2 * e] = __fmul_rn(c.x, p.k_scale); hif[2 * e + 1] = __fmul_rn(c.y, p.k_scale);
+    top = fmaxf(top, fmaxf(fmaxf(fabsf(lof[2 * e]), fabsf(lof[2 * e + 1])), fmaxf(fabsf(hif[2 * e]), fabsf(hif[2 * e + 1]))));
+  }
+  top = fminf(warp_max(top), FLT_MAX);
+  const float s = __fdiv_rn(top, 127.f);
+  int8_t* code = p.code + page * p.c_sb + h * p.c_sh;
+  auto put = [&](const float* x, int8_t* to) {
+    uint32_t u[NP / 2];
+#pragma unroll
+    for (int e = 0; e < NP / 2; ++e) {
+      u[e] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[e] |= uint32_t(uint8_t(code_of(x[4 * e + i], s, top > 0.f))) << (8 * i);
+    }
+    if (FP8) *reinterpret_cast<uint4*>(to + part * 16) = make_uint4(u[0], u[1], u[NP / 2 - 2], u[NP / 2 - 1]);
+    else *reinterpret_cast<uint2*>(to + part * 8) = make_uint2(u[0], u[1]);
+  };
+  if (GROUPS == 1) {
+    put(lof, code);
+    put(hif, code + D);
+  } else if (group < 2) {
+#pragma unroll
+    for (int e = 0; e < 2 * NP; ++e) lof[e] = group ? hif[e] : lof[e];
+    put(lof, code + group * D);
+  }
+  if (lane == 0) p.scale[page * p.s_sb + h * p.s_sh] = s;
+}
+
+int launch_summary(const SummaryParams& p, bool vector, cudaStream_t st) {
+  const int64_t items = p.T == 0 ? int64_t(p.g.B) * p.g.wide
+                        : !p.cu  ? int64_t(p.g.B)
+                                 : 2 * int64_t(p.g.B) + (int64_t(p.T) + p.g.block - 1) / p.g.block;
+  const int per = vector ? 8 : 4;
+  const int64_t ctas = (items * p.g.Hk + per - 1) / per;
+  if (ctas == 0) return BD_OK;
+  if (ctas > 0x7fffffff) return fail(BD_ERR_SHAPE, "too many pages for one launch");
+  auto go = [&](auto kern) {
+    kern<<<unsigned(ctas), per * 32, 0, st>>>(p);
+    return cuda_check(cudaGetLastError(), "paged_summary_kernel launch");
+  };
+  if (!vector) return go(paged_summary_generic_kernel);
+  switch (p.dtype) {
+    case BD_BF16:
+      return p.g.D == 64 ? go(paged_summary_kernel<__nv_bfloat16, false, 8>)
+             : p.g.D == 128 ? go(paged_summary_kernel<__nv_bfloat16, false, 16>)
+                            : go(paged_summary_kernel<__nv_bfloat16, false, 32>);
+    case BD_F16:
+      return p.g.D == 64 ? go(paged_summary_kernel<__half, false, 8>)
+             : p.g.D == 128 ? go(paged_summary_kernel<__half, false, 16>)
+                            : go(paged_summary_kernel<__half, false, 32>);
+    default:
+      return p.g.D == 64 ? go(paged_summary_kernel<__half, true, 4>)
+             : p.g.D == 128 ? go(paged_summary_kernel<__half, true, 8>) : go(paged_summary_kernel<__half, true, 16>);
+  }
 }
 
 int check_new(const bd_tensor* t, const char* name, int64_t T, int64_t D, int dtype) {
@@ -279,8 +601,13 @@ int bd_paged_append(const bd_tensor* k, const bd_tensor* v, const bd_tensor* q, 
     p.interleaved = interleaved != 0;
     p.cu = cu_seqlens ? static_cast<const int*>(cu_seqlens->data) : nullptr;
     p.k_inv = 1.f / k_scale; p.v_inv = 1.f / v_scale;
-    paged_append_kernel<<<unsigned(T), 128, 0, stream>>>(p);
-    return cuda_check(cudaGetLastError(), "paged_append_kernel launch");
+    const int items = int(D / 16);
+    const bool vector = D % 16 == 0 && items <= 16 && !(items & (items - 1)) && p.half % 8 == 0 && by_eight(k) &&
+                        by_eight(v) && (!q || (by_eight(q) && by_eight(q_out))) && by_eight(k_cache) &&
+                        by_eight(v_cache) && (!cos || (by_eight(cos) && by_eight(sin)));
+    if (vector) return launch_append(p, stream);
+    paged_append_generic_kernel<<<unsigned(T), 128, 0, stream>>>(p);
+    return cuda_check(cudaGetLastError(), "paged_append_generic_kernel launch");
   });
 }
 
@@ -312,12 +639,10 @@ int bd_paged_block_summary(const bd_tensor* k_cache, const bd_tensor* block_tabl
     p.s_sb = summary_scale->stride[0]; p.s_sh = summary_scale->stride[1];
     p.k_scale = k_scale; p.T = new_tokens;
     p.cu = cu_seqlens ? static_cast<const int*>(cu_seqlens->data) : nullptr;
-    const int64_t items = new_tokens > 0 ? new_tokens : int64_t(p.g.B) * p.g.wide;
-    const int64_t ctas = (items * p.g.Hk + 3) / 4;
-    if (ctas == 0) return BD_OK;
-    if (ctas > 0x7fffffff) return fail(BD_ERR_SHAPE, "too many pages for one launch");
-    paged_summary_kernel<<<unsigned(ctas), 128, 0, stream>>>(p);
-    return cuda_check(cudaGetLastError(), "paged_summary_kernel launch");
+    const bool types = p.dtype == BD_BF16 || p.dtype == BD_F16 || p.dtype == BD_F8E4M3;
+    const bool vector = types && (p.g.D == 64 || p.g.D == 128 || p.g.D == 256) && !check_rows_aligned(k_cache, "k_cache") &&
+                        !((reinterpret_cast<uintptr_t>(p.code) | size_t(p.c_sb) | size_t(p.c_sh)) & 15);
+    return launch_summary(p, vector, stream);
   });
 }
 
