@@ -183,17 +183,41 @@ __device__ __forceinline__ int64_t total_units(const AttnParams& p, int lane) {
   return n * (p.g.Hk * p.chunks);
 }
 
-// First unit of warp w's share.
-__device__ __forceinline__ int64_t share(int64_t total, int w, int n) {
-  const int64_t each = total / n, rest = total % n;
-  return each * w + min(int64_t(w), rest);
-}
+// The list's shares: equal ones for the grid's CTAs (the first few get one unit more), and of a CTA's
+// share equal ones for its warps: warp w has units [begin(w), begin(w + 1)). A short list goes to as
+// many CTAs as it has kMinUnits: spread over the SMs it is there sooner, in fewer parts it is joined sooner.
+constexpr int kMinUnits = 4;
 
-// Warp whose share holds unit u.
-__device__ __forceinline__ int owner(int64_t total, int64_t u, int n) {
-  const int64_t each = total / n, rest = total % n;
-  const int64_t cut = (each + 1) * rest;
-  return u < cut ? int(u / (each + 1)) : int(rest + (u - cut) / each);
+template <int WARPS>
+struct Shares {
+  int64_t each; int rest;
+  __device__ __forceinline__ Shares(int64_t total, int warps) {
+    const int n = int(max(int64_t(1), min(int64_t(warps / WARPS), total / kMinUnits)));
+    each = total / n;
+    rest = int(total - each * n);
+    ctas = n;
+  }
+  int ctas;
+  __device__ __forceinline__ int64_t cta(int c) const { c = min(c, ctas); return each * c + min(c, rest); }
+  __device__ __forceinline__ int64_t begin(int w) const {
+    const int c = w / WARPS, i = w % WARPS;
+    const int64_t first = cta(c);
+    const int n = int(cta(c + 1) - first);
+    return first + n / WARPS * i + min(i, n % WARPS);
+  }
+  // Warp whose share holds unit u.
+  __device__ __forceinline__ int owner(int64_t u) const {
+    const int64_t cut = (each + 1) * rest;
+    const int c = u < cut ? int(u / (each + 1)) : int(rest + (u - cut) / each);
+    const int64_t first = cta(c);
+    const int r = int(u - first), n = int(cta(c + 1) - first);
+    const int k = n / WARPS, m = n % WARPS;
+    return c * WARPS + (r < (k + 1) * m ? r / (k + 1) : m + (r - (k + 1) * m) / max(k, 1));
+  }
+};
+
+__device__ __forceinline__ void prefetch_tensormap(const void* map) {
+  asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
 }
 
 // A place in the list of units.
@@ -247,23 +271,33 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
   constexpr int KSTEPS = D / 16, NH = 8 * NT;
   // weights are kept 2^kUp above 1 where they are rounded to f16, so that small ones stay normal
   constexpr float kUp = KIND == kBf16 ? 0.f : 14.f;
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(128) uint8_t smem_raw[];
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + uint32_t(warp) * T::STAGES * 2 * T::HALF;
   const uint32_t bars = ((smem_u32(smem_raw) + 1023u) & ~1023u) + uint32_t(T::WARPS) * T::STAGES * 2 * T::HALF +
                         uint32_t(warp) * T::STAGES * 8;
   const int w = blockIdx.x * T::WARPS + warp;
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+  }
   const int64_t total = total_units(p, lane);
-  const int64_t first = share(total, w, p.warps);
-  int left = int(share(total, w + 1, p.warps) - first);
-  if (left == 0) return;
+  const Shares<T::WARPS> sh(total, p.warps);
+  const int64_t first = sh.begin(w), cta_first = sh.begin(w - warp), cta_end = sh.begin(w - warp + T::WARPS);
+  int left = int(sh.begin(w + 1) - first);
+  if (cta_end == cta_first) return;
   if (lane < T::STAGES) mbar_init(bars + lane * 8, 1);
   if (lane == 0) mbar_fence_init();
   __syncwarp();
 
   Place in;  // the next unit to bring in
-  in.find(p, first, lane);
+  in.find(p, cta_first, lane);
+  // with all of the CTA's units in one row its warps' parts are added up here, and one goes out
+  const bool one_row = in.u + (cta_end - cta_first) <= in.units;
+  if (one_row) in.u += int(first - cta_first);
+  else if (left > 0) in.find(p, first, lane);
+  if (!one_row && left == 0) return;
   Place at = in;  // the unit at hand
   int to_issue = left;
   // list positions held by the lanes: entry_first + lane of the row in.b, in.hc
@@ -339,9 +373,9 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
   int stage = 0;
   unsigned phase = 0;
   bool lost = false;
-  const int64_t list_first = first;
   int64_t seg_first = first;
-  while (left > 0) {
+  float o[KSTEPS][NT][4], mrow[NT][2], lrow[NT][2];
+  while (left > 0 || one_row) {
     const int n = min(left, at.units - at.u);  // this warp's units of the row
     const int hk = at.hc / p.chunks, h0 = (at.hc % p.chunks) * NH;
     const int nheads = min(NH, p.G - h0);
@@ -386,7 +420,6 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
             qb[kk][nt][i] = KIND == kBf16 ? pack_bf16x2(qv[kk][nt][2 * i], qv[kk][nt][2 * i + 1])
                                           : pack_f16x2(qv[kk][nt][2 * i] * qscale, qv[kk][nt][2 * i + 1] * qscale);
     }
-    float o[KSTEPS][NT][4], mrow[NT][2], lrow[NT][2];
 #pragma unroll
     for (int mt = 0; mt < KSTEPS; ++mt)
 #pragma unroll
@@ -536,8 +569,6 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
     }
 
     // ---- the row's result, or this warp's part of it
-    const bool whole = n == at.units;
-    const int64_t slot = 2 * int64_t(w) + (seg_first != list_first);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -546,10 +577,20 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
         l += __shfl_xor_sync(0xffffffffu, l, 4);
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
-        if (lost) l = NAN;
+        lrow[nt][j] = lost ? NAN : l;
+        mrow[nt][j] = lost ? 0.f : mrow[nt][j] - kUp;  // of sums that are 2^kUp times as large
+      }
+    left -= n;
+    if (one_row) break;  // the warp's only segment: joined with the others' below
+    const bool whole = n == at.units;
+    const int64_t slot = 2 * int64_t(w) + (seg_first != first);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
         const int h = nt * 8 + 2 * tq + j;
         if (h >= nheads) continue;
-        const float m = lost ? 0.f : mrow[nt][j] - kUp;  // of sums that are 2^kUp times as large
+        const float m = mrow[nt][j], l = lrow[nt][j];
         if (whole) {
           const int hq = hk * p.G + h0 + h;
           const float f = m == -INFINITY ? 0.f : p.v_scale / l;
@@ -576,34 +617,92 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
           }
         }
       }
-    left -= n;
     seg_first += n;
     if (left > 0) at.next_row(p);
   }
   // a copy that was given up is still waited for (again with a limit) before the memory goes
   if (lost)
     for (int s = 0; s < T::STAGES; ++s) mbar_wait(bars + s * 8, s < stage ? phase ^ 1 : phase);
+  if (!one_row) return;
+  // ---- the CTA's warps each have a part of the same row: one sum of them goes out
+  __syncthreads();  // nothing is in flight: the rings' memory takes the parts
+  float* sm = reinterpret_cast<float*>(smem_raw);  // [warps][NH] maxima, sums, then [warps][NH][D]
+  float* sl = sm + T::WARPS * NH;
+  float* so = sl + T::WARPS * NH;
+  if (g == 0) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        sm[warp * NH + nt * 8 + 2 * tq + j] = mrow[nt][j];
+        sl[warp * NH + nt * 8 + 2 * tq + j] = lrow[nt][j];
+      }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int h = nt * 8 + 2 * tq + j;
+      float M = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < T::WARPS; ++i) M = fmaxf(M, sm[i * NH + h]);
+      const float f = mrow[nt][j] == -INFINITY ? 0.f : exp2f(mrow[nt][j] - M);
+      float* to = so + (warp * NH + h) * D;
+#pragma unroll
+      for (int mt = 0; mt < KSTEPS; ++mt) {
+        const int ca = FP8 ? mt * 16 + 2 * g : mt * 16 + g, cb = FP8 ? ca + 1 : ca + 8;
+        to[ca] = o[mt][nt][j] * f;
+        to[cb] = o[mt][nt][2 + j] * f;
+      }
+    }
+  __syncthreads();
+  const int64_t slot = 2 * int64_t(w - warp);
+  const int nheads = min(NH, p.G - (at.hc % p.chunks) * NH);
+  for (int e = threadIdx.x; e < nheads * (D / 4); e += T::WARPS * 32) {
+    const int h = e / (D / 4), c = e % (D / 4);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < T::WARPS; ++i) {
+      const float4 y = reinterpret_cast<const float4*>(so + (i * NH + h) * D)[c];
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    reinterpret_cast<float4*>(p.part_o + (slot * NH + h) * D)[c] = x;
+    if (c) continue;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < T::WARPS; ++i) M = fmaxf(M, sm[i * NH + h]);
+#pragma unroll
+    for (int i = 0; i < T::WARPS; ++i) L += sm[i * NH + h] == -INFINITY ? 0.f : sl[i * NH + h] * exp2f(sm[i * NH + h] - M);
+    p.part_m[slot * NH + h] = M;
+    p.part_l[slot * NH + h] = L;
+  }
 }
 
 // Joins the parts of the rows that more than one warp had, and writes the rows that have no token.
-// One CTA per (query head, sequence); a thread has 4 channels of every eighth (D = 64), fourth or
-// second (256) part.
-constexpr int kJoinThreads = 128;
-template <int D>
+// One CTA per HEADS query heads of a row. The parts of a row: one for every CTA of the tile kernel whose
+// units all lie in it, one for every warp of the CTAs at its ends otherwise; 32 of them at a time get
+// their weights in shared memory, then a thread adds 4 channels of one head up over every SLICES-th part.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinParts = 32;
+
+template <int D, int WARPS, int HEADS>
 __global__ void __launch_bounds__(kJoinThreads) paged_tile_join_kernel(const AttnParams p) {
-  constexpr int PER = D / 4, SLICES = kJoinThreads / PER;
-  __shared__ float4 red[SLICES][PER];
-  const int hq = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31;
-  const int hk = hq / p.G, hl = hq % p.G, hc = hk * p.chunks + hl / p.heads, h = hl % p.heads;
+  constexpr int PER = D / 4, SLICES = kJoinThreads / (PER * HEADS);
+  __shared__ float4 red[SLICES][HEADS][PER];
+  __shared__ float weight[HEADS][kJoinParts], row_m[HEADS], row_l[HEADS], back[HEADS];
+  __shared__ int64_t part_slot[kJoinParts];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int groups = (min(p.heads, p.G) + HEADS - 1) / HEADS;  // of a chunk's heads
+  const int hc = blockIdx.x / groups, h0 = (blockIdx.x % groups) * HEADS, b = blockIdx.y;
+  const int hq0 = (hc / p.chunks) * p.G + (hc % p.chunks) * p.heads + h0;
+  const int nheads = min(HEADS, min(p.heads, p.G - (hc % p.chunks) * p.heads) - h0);
+  const int part = threadIdx.x % PER, head = threadIdx.x / PER % HEADS, slice = threadIdx.x / (PER * HEADS);
   const int units = row_units(p, paged_len(p.g, b));
-  const int64_t out = b * p.o_sb + hq * p.o_sh;
-  const int part = threadIdx.x % PER, slice = threadIdx.x / PER;
-  if (units == 0) {
-    if (slice == 0)
-      for (int i = 0; i < 4; ++i) store_as(p.out, p.out_dtype, out + (4 * part + i) * p.o_sd, 0.f);
-    if (p.lse && threadIdx.x == 0) p.lse[b * p.e_sb + hq * p.e_sh] = -INFINITY;
-    griddep_wait();  // a kernel that waits for this one then finds the tile kernel done as well
-    return;
+  const int64_t out = b * p.o_sb + (hq0 + head) * p.o_sh;
+  if (units == 0 && slice == 0 && head < nheads) {
+    for (int i = 0; i < 4; ++i) store_as(p.out, p.out_dtype, out + (4 * part + i) * p.o_sd, 0.f);
+    if (p.lse && part == 0) p.lse[b * p.e_sb + (hq0 + head) * p.e_sh] = -INFINITY;
   }
   // units of all sequences, and of those before this one
   int64_t all = 0, before = 0;
@@ -619,40 +718,81 @@ __global__ void __launch_bounds__(kJoinThreads) paged_tile_join_kernel(const Att
   }
   const int per = p.g.Hk * p.chunks;
   all *= per;
-  const int64_t u0 = before * per + int64_t(hc) * units;
-  const int w0 = owner(all, u0, p.warps), w1 = owner(all, u0 + units - 1, p.warps);
-  griddep_wait();
-  if (w0 == w1) return;  // one warp had the whole row
-  auto slot = [&](int w) { return (2 * int64_t(w) + (share(all, w, p.warps) < u0)) * p.heads + h; };
-  float M = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, p.part_m[slot(w)]);
-  M = warp_max(M);
-  float L = 0.f;
+  const Shares<WARPS> sh(all, p.warps);
+  const int64_t u0 = before * per + int64_t(hc) * units, u1 = u0 + units;
+  int w0 = 0, w1 = 0, c0 = 0, c1 = 0, n0 = 0, n1 = 0, n = 0;
+  bool in0 = false, in1 = false;
+  if (units > 0 && nheads > 0) {
+    w0 = sh.owner(u0);
+    w1 = sh.owner(u1 - 1);
+    // the CTAs with units of the row, and whether those at its ends have units of it only
+    c0 = w0 / WARPS;
+    c1 = w1 / WARPS;
+    in0 = sh.cta(c0) >= u0 && sh.cta(c0 + 1) <= u1;
+    in1 = sh.cta(c1) >= u0 && sh.cta(c1 + 1) <= u1;
+    // parts of the first (a CTA with fewer units than warps leaves its last warps without one), of the
+    // last, and of all of them; none if one warp had the whole row and wrote it
+    n0 = in0 ? 1 : min(w1, sh.owner(sh.cta(c0 + 1) - 1)) - w0 + 1;
+    n1 = c1 == c0 ? 0 : in1 ? 1 : w1 - c1 * WARPS + 1;
+    n = w0 == w1 && !in0 ? 0 : n0 + max(0, c1 - c0 - 1) + n1;
+  }
+  griddep_wait();  // also for a kernel that waits for this one: it then finds the tile kernel done as well
+  if (n == 0) return;
+  if (threadIdx.x < HEADS) row_m[threadIdx.x] = -INFINITY, row_l[threadIdx.x] = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int w = w0 + slice; w <= w1; w += SLICES) {
-    const int64_t s = slot(w);
-    const float m = p.part_m[s], f = m == -INFINITY ? 0.f : exp2f(m - M);
-    const float4 x = reinterpret_cast<const float4*>(p.part_o + s * D)[part];
-    L = fmaf(p.part_l[s], f, L);
-    acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
-    acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+  for (int first = 0; first < n; first += kJoinParts) {
+    const int here = min(kJoinParts, n - first);
+    __syncthreads();
+    // ---- weights of up to 32 parts, relative to the largest maximum so far: a warp a head
+    for (int hh = warp; hh < nheads; hh += kJoinThreads / 32) {
+      float m = -INFINITY, l = 0.f;
+      if (lane < here) {
+        const int i = first + lane;
+        const int w = i < n0 ? (in0 ? c0 * WARPS : w0 + i)
+                      : i < n - n1 ? (c0 + 1 + i - n0) * WARPS : c1 * WARPS + (i - (n - n1));
+        const int64_t slot = (2 * int64_t(w) + (sh.begin(w) < u0)) * p.heads + h0;
+        if (hh == 0) part_slot[lane] = slot;
+        m = __ldcg(p.part_m + slot + hh);
+        l = __ldcg(p.part_l + slot + hh);
+      }
+      const float M = row_m[hh], Mn = fmaxf(M, warp_max(m));
+      const float f = m == -INFINITY ? 0.f : exp2f(m - Mn), r = M == -INFINITY ? 0.f : exp2f(M - Mn);
+      l = warp_sum(l * f);
+      __syncwarp();
+      weight[hh][lane] = f;
+      if (lane == 0) row_m[hh] = Mn, back[hh] = r, row_l[hh] = row_l[hh] * r + l;
+    }
+    __syncthreads();
+    if (head >= nheads) continue;
+    const float r = back[head];
+    acc.x *= r; acc.y *= r; acc.z *= r; acc.w *= r;
+#pragma unroll 8
+    for (int i = slice; i < here; i += SLICES) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + (part_slot[i] + head) * D) + part);
+      const float f = weight[head][i];
+      acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+    }
   }
-  __shared__ float sums[SLICES];
-  red[slice][part] = acc;
-  if (part == 0) sums[slice] = L;
-  __syncthreads();
-  if (slice) return;
-  for (int i = 1; i < SLICES; ++i) {
-    const float4 x = red[i][part];
-    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
-    L += sums[i];
+  if (SLICES > 1) {
+    red[slice][head][part] = acc;
+    __syncthreads();
+    if (slice) return;
+#pragma unroll
+    for (int i = 1; i < SLICES; ++i) {
+      const float4 x = red[i][head][part];
+      acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+    }
   }
+  if (head >= nheads) return;
+  const float M = row_m[head], L = row_l[head];
   const float f = M == -INFINITY ? 0.f : p.v_scale / L;
   store_as(p.out, p.out_dtype, out + 4 * part * p.o_sd, acc.x * f);
   store_as(p.out, p.out_dtype, out + (4 * part + 1) * p.o_sd, acc.y * f);
   store_as(p.out, p.out_dtype, out + (4 * part + 2) * p.o_sd, acc.z * f);
   store_as(p.out, p.out_dtype, out + (4 * part + 3) * p.o_sd, acc.w * f);
-  if (p.lse && part == 0) p.lse[b * p.e_sb + hq * p.e_sh] = M == -INFINITY ? -INFINITY : M * kLn2 + logf(L);
+  if (p.lse && part == 0)
+    p.lse[b * p.e_sb + (hq0 + head) * p.e_sh] = M == -INFINITY ? -INFINITY : M * kLn2 + logf(L);
 }
 
 // Whether the tiles can take a call: 16-bit queries and caches of one type, or 8-bit caches; pages of
@@ -725,8 +865,14 @@ int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor*
   }
   kern<<<p.warps / T::WARPS, T::WARPS * 32, T::SMEM, st>>>(p, km, vm);
   if ((rc = cuda_check(cudaGetLastError(), "paged_attn_tile_kernel launch"))) return rc;
-  return launch_programmatic(paged_tile_join_kernel<D>, dim3(p.Hq, p.g.B), dim3(kJoinThreads), 0, st, p,
-                             "paged_tile_join_kernel launch");
+  // few rows: a CTA a head, its threads over many parts at once; many rows, which have few parts each: a
+  // CTA the heads that its threads can hold
+  constexpr int MANY = D == 256 ? 4 : 8;
+  const bool many = int64_t(p.g.B) * p.Hq > 8 * num_sms();
+  const int heads = many ? MANY : 1;
+  return launch_programmatic(many ? paged_tile_join_kernel<D, T::WARPS, MANY> : paged_tile_join_kernel<D, T::WARPS, 1>,
+                             dim3(p.g.Hk * p.chunks * ((std::min(p.heads, p.G) + heads - 1) / heads), p.g.B), dim3(kJoinThreads), 0,
+                             st, p, "paged_tile_join_kernel launch");
 }
 
 template <int D, int KIND>
