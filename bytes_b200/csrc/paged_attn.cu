@@ -29,6 +29,7 @@ struct AttnParams {
   float* part_o; float* part_m; float* part_l;  // [B*Hq][n_splits]([D]); m in log2 units
   // tile form: warps of the grid, its partials [2 * warps][heads]([D])
   int warps, heads, block_shift;
+  int row_mode;  // a CTA has a row, and nothing is joined
   void* out; int out_dtype; int64_t o_sb, o_sh, o_sd;
   float* lse; int64_t e_sb, e_sh;
 };
@@ -136,32 +137,43 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const AttnParams p) {
 
 // ------------------------------------------------------------------ tensor-core tiles
 //
-// The work is one list of 16-token units: for every sequence, every KV head (and chunk of 8 or 16
-// of its query heads), the units of its tokens, or of its chosen pages. Warp w of the grid's n takes
-// units [w T / n, (w + 1) T / n): equal shares whatever the lengths, which only the device knows. A
-// warp works alone, with no barrier of the CTA: its lane 0 brings units ahead of use into the warp's
-// own ring of shared memory by TMA (one box of a page's 16 rows for keys and one for values, 128-byte
-// swizzle, so that ldmatrix reads without bank conflicts), and each unit is
+// The work is one list: for every sequence, every KV head (and chunk of 8 or 16 of its query heads),
+// the 16-token units of its tokens, or of its chosen pages, behind kRowCost slots that stand for what
+// a row costs before its first unit. The list is cut into equal shares for the grid's warps, whatever the
+// lengths, which only the device knows. A warp works alone, with no barrier of the CTA: its lane 0 brings
+// units ahead of use into the warp's own ring of shared memory by TMA (one box of a page's 16 rows for keys
+// and one for values, 128-byte swizzle, so that ldmatrix reads without bank conflicts), and each unit is
 //   S^T[16 x heads] = K Q^T, running maximum and sum, O^T[D x heads] += V^T P^T
 // in mma.sync m16n8k16 with 32-bit sums (the query heads of a KV head are the n of the product, so
 // every key and value is read once). Rows that a warp has whole are written at once; the others'
-// (maximum, sum, numerator) go to the workspace, two at most for a warp, and paged_join_kernel joins
+// (maximum, sum, numerator) go to the workspace, two at most for a warp, and paged_tile_join_kernel joins
 // them.
 
 constexpr int kUnit = 16;
 
 enum { kBf16 = 0, kF16 = 1, kFp8 = 2 };
 
-template <int D, int KIND>
+#ifndef P_WF
+#define P_WF 16
+#endif
+#ifndef P_WB
+#define P_WB 12
+#endif
+#ifndef P_W64
+#define P_W64 16
+#endif
+template <int D, int KIND, int NT>
 struct TileShape {
   static constexpr int ELT = KIND == kFp8 ? 1 : 2;
   static constexpr int ROWB = D * ELT;
   static constexpr int SW = ROWB < 128 ? ROWB : 128;  // bytes of a row in one slab (the swizzle's span)
   static constexpr int SLABS = ROWB / SW;
   static constexpr int HALF = kUnit * ROWB;           // keys (or values) of a unit
-  static constexpr int WARPS = HALF * 2 > 8192 ? 4 : 8;
-  static constexpr int STAGES = (200 * 1024 / (WARPS * HALF * 2)) < 8 ? (200 * 1024 / (WARPS * HALF * 2)) : 8;
-  static constexpr int SMEM = WARPS * STAGES * HALF * 2 + WARPS * STAGES * 8 + 1024;
+  static constexpr int WARPS = D == 256 ? (KIND == kFp8 ? 8 : 6) : NT == 2 ? 8 : D == 64 ? P_W64 : KIND == kFp8 ? P_WF : P_WB;
+  static constexpr int FIT = 200 * 1024 / (WARPS * HALF * 2);
+  static constexpr int STAGES = FIT < 8 ? FIT : 8;
+  static_assert(STAGES >= 2, "a unit in flight beside the one at hand");
+  static constexpr int SMEM = WARPS * STAGES * HALF * 2 + WARPS * STAGES * 12 + 1024;
 };
 
 // waits on tile copies that ran past their limit (a result is then NaN)
@@ -169,202 +181,344 @@ __device__ unsigned int g_paged_timeouts = 0;
 
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-// Units of a row (one sequence and KV head), and of all rows.
-__device__ __forceinline__ int row_units(const AttnParams& p, int len) {
-  if (p.n_sel >= 0) return len > 0 ? int((int64_t(p.n_sel) * p.g.block + kUnit - 1) / kUnit) : 0;
-  return (len + kUnit - 1) / kUnit;
+__device__ __forceinline__ void prefetch_tensormap(const void* map) {
+  asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
 }
 
-__device__ __forceinline__ int64_t total_units(const AttnParams& p, int lane) {
-  int64_t n = 0;
-  for (int b = lane; b < p.g.B; b += 32) n += row_units(p, paged_len(p.g, b));
+// A row's place in the list: its slots are kRowCost and its units; 0 without a token.
+#ifndef P_COST
+#define P_COST 1
+#endif
+constexpr int kRowCost = P_COST;
+
+__device__ __forceinline__ int row_slots(const AttnParams& p, int len) {
+  if (len <= 0) return 0;
+  const int tokens = p.n_sel >= 0 ? p.n_sel << p.block_shift : len;
+  return tokens > 0 ? (tokens - 1) / kUnit + 1 + kRowCost : 0;
+}
+
+// Inclusive sum over the lanes.
+__device__ __forceinline__ int warp_prefix(int x, int lane) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n * (p.g.Hk * p.chunks);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
 }
 
-// The list's shares: equal ones for the grid's CTAs (the first few get one unit more), and of a CTA's
-// share equal ones for its warps: warp w has units [begin(w), begin(w + 1)). A short list goes to as
-// many CTAs as it has kMinUnits: spread over the SMs it is there sooner, in fewer parts it is joined sooner.
-constexpr int kMinUnits = 4;
+// Running sums of the list's slots over the sequences. Up to 32 sequences are a warp's own: lane b has
+// sequence b's. More are summed by the CTA in shared memory, over up to kGroups groups of `size` neighbours.
+constexpr int kGroups = 1024;
+struct GroupSums {
+  int sum[kGroups];
+  int warp_sum[32];
+};
 
+struct ListSums {
+  int total, len, sum;  // (lane b's length and running sum, up to 32 sequences)
+  int groups, size;
+  template <int WARPS>
+  __device__ __forceinline__ void build(const AttnParams& p, GroupSums& g, int warp, int lane) {
+    const int per = p.g.Hk * p.chunks;
+    if (p.g.B <= 32) {
+      len = lane < p.g.B ? paged_len(p.g, lane) : 0;
+      sum = warp_prefix(row_slots(p, len) * per, lane);
+      total = __shfl_sync(0xffffffffu, sum, 31);
+      return;
+    }
+    size = (p.g.B + kGroups - 1) / kGroups;
+    groups = (p.g.B + size - 1) / size;
+    const int each = (groups + WARPS * 32 - 1) / (WARPS * 32) * 32, first = warp * each;
+    int carry = 0;
+    for (int i = first + lane; i - lane < min(groups, first + each); i += 32) {
+      int n = 0;
+      if (i < groups)
+        for (int b = i * size; b < min(p.g.B, (i + 1) * size); ++b) n += row_slots(p, paged_len(p.g, b));
+      n = warp_prefix(n * per, lane) + carry;
+      if (i < groups) g.sum[i] = n;
+      carry = __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) g.warp_sum[warp] = carry;
+    __syncthreads();
+    const int mine = lane < WARPS ? g.warp_sum[lane] : 0, before = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+    total = __reduce_add_sync(0xffffffffu, mine);
+    for (int i = first + lane; i < min(groups, first + each); i += 32) g.sum[i] += before;
+    __syncthreads();
+  }
+};
+
+// The list's shares: equal ones for the grid's CTAs (the first few get one slot more), and of a CTA's
+// share equal ones for its warps: warp w has slots [begin(w), begin(w + 1)). A short list goes to as
+// many CTAs as it has kMinSlots: spread over the SMs it is there sooner, in fewer parts it is joined sooner
+// (one sequence of 777 tokens, 28 heads over 4: 12.5, 9.5, 9.2, 9.8 us for 1, 2, 4, 8).
+constexpr int kMinSlots = 4;
+
+// A border inside a row of up to `whole` slots, two shares, moves to the nearer end of the row: so short a
+// row costs less unevenly shared than joined. What cuts a longer row stays where it is.
 template <int WARPS>
 struct Shares {
-  int64_t each; int rest;
-  __device__ __forceinline__ Shares(int64_t total, int warps) {
-    const int n = int(max(int64_t(1), min(int64_t(warps / WARPS), total / kMinUnits)));
-    each = total / n;
-    rest = int(total - each * n);
-    ctas = n;
+  int each, rest, ctas, whole;
+  __device__ __forceinline__ Shares(int total, int warps) {
+    ctas = max(1, min(warps / WARPS, total / kMinSlots));
+    each = total / ctas;
+    rest = total - each * ctas;
+    whole = 2 * each / WARPS;
   }
-  int ctas;
-  __device__ __forceinline__ int64_t cta(int c) const { c = min(c, ctas); return each * c + min(c, rest); }
-  __device__ __forceinline__ int64_t begin(int w) const {
-    const int c = w / WARPS, i = w % WARPS;
-    const int64_t first = cta(c);
-    const int n = int(cta(c + 1) - first);
+  __device__ __forceinline__ int cta(int c) const { c = min(c, ctas); return each * c + min(c, rest); }
+  __device__ __forceinline__ int begin(int w) const {
+    const int c = w / WARPS, i = w % WARPS, first = cta(c), n = cta(c + 1) - first;
     return first + n / WARPS * i + min(i, n % WARPS);
   }
-  // Warp whose share holds unit u.
-  __device__ __forceinline__ int owner(int64_t u) const {
-    const int64_t cut = (each + 1) * rest;
-    const int c = u < cut ? int(u / (each + 1)) : int(rest + (u - cut) / each);
-    const int64_t first = cta(c);
-    const int r = int(u - first), n = int(cta(c + 1) - first);
+  // Warp whose share holds slot s.
+  __device__ __forceinline__ int owner(int s) const {
+    const int cut = (each + 1) * rest;
+    const int c = s < cut ? s / (each + 1) : rest + (s - cut) / max(each, 1);
+    const int first = cta(c), r = s - first, n = cta(c + 1) - first;
     const int k = n / WARPS, m = n % WARPS;
     return c * WARPS + (r < (k + 1) * m ? r / (k + 1) : m + (r - (k + 1) * m) / max(k, 1));
   }
 };
 
-__device__ __forceinline__ void prefetch_tensormap(const void* map) {
-  asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
-}
-
-// A place in the list of units.
+// A place in the list: slot s of a row (its unit s - kRowCost).
 struct Place {
-  int b, hc, u, units, len;
-  // Goes to unit `at` of the list (a warp's lanes together).
-  __device__ __forceinline__ void find(const AttnParams& p, int64_t at, int lane) {
-    const int per = p.g.Hk * p.chunks;
-    for (int b0 = 0; b0 < p.g.B; b0 += 32) {
-      const int mine = b0 + lane < p.g.B ? paged_len(p.g, b0 + lane) : 0;
-      const int64_t n = int64_t(row_units(p, mine)) * per;
-      int64_t sum = n;  // inclusive prefix
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += x;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, sum > at);
-      if (past) {
-        const int l = __ffs(past) - 1;
-        b = b0 + l;
-        len = __shfl_sync(0xffffffffu, mine, l);
-        const int64_t in = at - __shfl_sync(0xffffffffu, sum - n, l);
-        units = row_units(p, len);
-        hc = int(in / units);
-        u = int(in % units);
-        return;
-      }
-      at -= __shfl_sync(0xffffffffu, sum, 31);
+  int b = 0, hk = 0, chunk = 0, s = 0, slots = 0, len = 0;
+  // Slot `in` of sequence b's rows.
+  __device__ __forceinline__ void within(const AttnParams& p, int sequence, int length, int in) {
+    b = sequence;
+    len = length;
+    slots = row_slots(p, len);
+    hk = in / slots;
+    s = in - hk * slots;
+    if (p.chunks > 1) {
+      const int hc = hk;
+      hk = hc / p.chunks;
+      chunk = hc - hk * p.chunks;
     }
   }
-  // Goes to the first unit of the next row that has any; there has to be one.
-  __device__ __forceinline__ void next_row(const AttnParams& p) {
-    u = 0;
-    if (++hc < p.g.Hk * p.chunks) return;
-    hc = 0;
+  // Goes to slot `at` of the list (a warp's lanes together).
+  __device__ __forceinline__ void find(const AttnParams& p, const ListSums& l, const GroupSums& g, int at, int lane) {
+    if (p.g.B <= 32) {
+      const int i = __ffs(__ballot_sync(0xffffffffu, l.sum > at)) - 1;
+      const int before = __shfl_sync(0xffffffffu, l.sum, i - 1);
+      within(p, i, __shfl_sync(0xffffffffu, l.len, i), i ? at - before : at);
+      return;
+    }
+    // the group: 32 of them apart, then one by one
+    const int step = (l.groups + 31) / 32;
+    const int k = __ffs(__ballot_sync(0xffffffffu, g.sum[min(l.groups, (lane + 1) * step) - 1] > at)) - 1;
+    const int j = k * step + lane;
+    const int i = k * step + __ffs(__ballot_sync(0xffffffffu, j >= l.groups || g.sum[j] > at)) - 1;
+    if (i) at -= g.sum[i - 1];
+    const int per = p.g.Hk * p.chunks;
+    int b0 = i * l.size;
+#pragma unroll 1
+    for (;;) {  // the group's sequences
+      const int length = paged_len(p.g, b0), n = row_slots(p, length) * per;
+      if (at < n) {
+        within(p, b0, length, at);
+        return;
+      }
+      at -= n;
+      ++b0;
+    }
+  }
+  // Moves a border that is here off a short row; how far. (Then s may be the row's end.)
+  __device__ __forceinline__ int snap(int whole) {
+    if (s == 0 || slots > whole) return 0;
+    const int to = 2 * s < slots ? 0 : slots, by = to - s;
+    s = to;
+    return by;
+  }
+  // Goes to the start of the next row that has any slots; there has to be one. True in another sequence.
+  __device__ __forceinline__ bool next_row(const AttnParams& p) {
+    s = 0;
+    if (++chunk < p.chunks) return false;
+    chunk = 0;
+    if (++hk < p.g.Hk) return false;
+    hk = 0;
     do {
       ++b;
       len = paged_len(p.g, b);
-      units = row_units(p, len);
-    } while (units == 0 && b + 1 < p.g.B);
+      slots = row_slots(p, len);
+    } while (slots == 0 && b + 1 < p.g.B);
+    return true;
+  }
+};
+
+__device__ __forceinline__ uint32_t pack_out(const AttnParams& p, float a, float b) {
+  return p.out_dtype == BD_BF16 ? pack_bf16x2(a, b) : pack_f16x2(a, b);
+}
+
+// Maximum (log2 units), sum and four channels of the numerator, relative to the maximum.
+struct Sum4 {
+  float m, l;
+  float4 o;
+  static __device__ __forceinline__ Sum4 none() { return Sum4{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)}; }
+  __device__ __forceinline__ void add(float m2, float l2, float4 o2) {
+    const float M = fmaxf(m, m2);
+    const float a = m == -INFINITY ? 0.f : exp2f(m - M), b = m2 == -INFINITY ? 0.f : exp2f(m2 - M);
+    m = M;
+    l = fmaf(l, a, l2 * b);
+    o.x = fmaf(o.x, a, o2.x * b); o.y = fmaf(o.y, a, o2.y * b);
+    o.z = fmaf(o.z, a, o2.z * b); o.w = fmaf(o.w, a, o2.w * b);
+  }
+  // Writes channels 4 * part.. of query head hq.
+  __device__ __forceinline__ void write(const AttnParams& p, int b, int hq, int part) const {
+    const float f = m == -INFINITY ? 0.f : p.v_scale / l;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + b * p.o_sb + int64_t(hq) * p.o_sh + 4 * part;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_out(p, o.x * f, o.y * f), pack_out(p, o.z * f, o.w * f));
+    if (p.lse && part == 0) p.lse[b * p.e_sb + hq * p.e_sh] = m == -INFINITY ? -INFINITY : m * kLn2 + logf(l);
   }
 };
 
 template <int D, int KIND, int NT>
-__global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
+__global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     paged_attn_tile_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
                            const __grid_constant__ CUtensorMap vmap) {
-  using T = TileShape<D, KIND>;
+  using T = TileShape<D, KIND, NT>;
   constexpr bool FP8 = KIND == kFp8;
   constexpr int KSTEPS = D / 16, NH = 8 * NT;
   // weights are kept 2^kUp above 1 where they are rounded to f16, so that small ones stay normal
   constexpr float kUp = KIND == kBf16 ? 0.f : 14.f;
   extern __shared__ __align__(128) uint8_t smem_raw[];
+  __shared__ GroupSums groups;
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-  const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + uint32_t(warp) * T::STAGES * 2 * T::HALF;
-  const uint32_t bars = ((smem_u32(smem_raw) + 1023u) & ~1023u) + uint32_t(T::WARPS) * T::STAGES * 2 * T::HALF +
-                        uint32_t(warp) * T::STAGES * 8;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t ring = base + uint32_t(warp) * T::STAGES * 2 * T::HALF;
+  const uint32_t bars = base + uint32_t(T::WARPS) * T::STAGES * 2 * T::HALF + uint32_t(warp) * T::STAGES * 8;
+  const uint32_t notes = base + uint32_t(T::WARPS) * T::STAGES * (2 * T::HALF + 8) + uint32_t(warp) * T::STAGES * 4;
   const int w = blockIdx.x * T::WARPS + warp;
   if (threadIdx.x == 0) {
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
-  const int64_t total = total_units(p, lane);
-  const Shares<T::WARPS> sh(total, p.warps);
-  const int64_t first = sh.begin(w), cta_first = sh.begin(w - warp), cta_end = sh.begin(w - warp + T::WARPS);
-  int left = int(sh.begin(w + 1) - first);
-  if (cta_end == cta_first) return;
   if (lane < T::STAGES) mbar_init(bars + lane * 8, 1);
   if (lane == 0) mbar_fence_init();
   __syncwarp();
 
-  Place in;  // the next unit to bring in
-  in.find(p, cta_first, lane);
-  // with all of the CTA's units in one row its warps' parts are added up here, and one goes out
-  const bool one_row = in.u + (cta_end - cta_first) <= in.units;
-  if (one_row) in.u += int(first - cta_first);
-  else if (left > 0) in.find(p, first, lane);
-  if (!one_row && left == 0) return;
-  Place at = in;  // the unit at hand
-  int to_issue = left;
-  // list positions held by the lanes: entry_first + lane of the row in.b, in.hc
-  int entry_first = -1, entry_page = -1, entry_logical = 0;
-  unsigned long long live = 0;  // a byte a stage: live rows of the unit's first and second eight
-  // rows of a box, and where in a unit's keys row r of slab c starts: (r / 8) * step8 + c * slab + (r % 8) * SW
+  Place in;           // the next unit to bring in
+  int left;           // slots of this warp's share that are not worked off
+  bool one_row, row_begins = true;
+  if (p.row_mode) {   // a CTA has a row
+    one_row = true;
+    const int per = p.g.Hk * p.chunks, b = blockIdx.x / per, len = paged_len(p.g, b), slots = row_slots(p, len);
+    if (slots == 0) {
+      const int hc = blockIdx.x - b * per, hk = hc / p.chunks, chunk = hc - hk * p.chunks;
+      const int nheads = min(NH, p.G - chunk * NH);
+      for (int e = threadIdx.x; e < nheads * (D / 4); e += T::WARPS * 32)
+        Sum4::none().write(p, b, hk * p.G + chunk * NH + e / (D / 4), e % (D / 4));
+      return;
+    }
+    in.within(p, b, len, (blockIdx.x - b * per) * slots);
+    const int units = slots - kRowCost, n = units / T::WARPS, m = units % T::WARPS;
+    in.s = kRowCost + n * warp + min(warp, m);
+    left = n + (warp < m);
+  } else {
+    ListSums list;
+    list.build<T::WARPS>(p, groups, warp, lane);
+    const Shares<T::WARPS> sh(list.total, p.warps);
+    int first = sh.begin(w), end = sh.begin(w + 1);
+    const int cta_first = sh.cta(blockIdx.x), cta_end = sh.cta(blockIdx.x + 1);
+    if (cta_end == cta_first) return;
+    in.find(p, list, groups, cta_first, lane);
+    // with all of the CTA's share in one row that is cut its warps' parts are added up here, and one goes out
+    one_row = in.s + (cta_end - cta_first) <= in.slots && in.slots > sh.whole;
+    row_begins = in.s == 0;
+    if (one_row) {
+      in.s += first - cta_first;
+    } else {
+      if (first == end) return;
+      if (end < list.total) {
+        Place to;
+        to.find(p, list, groups, end, lane);
+        end += to.snap(sh.whole);
+      }
+      if (warp) in.find(p, list, groups, first, lane);
+      first += in.snap(sh.whole);
+      if (first >= end) return;
+      if (in.s == in.slots) in.next_row(p);
+    }
+    left = end - first;
+  }
+  Place at = in;        // the row at hand, from its slot at.s on
+  int to_issue = left;  // slots from `in` on
+  // list entries held by the lanes, entry_first + lane of the row in.b, in.hk: the page, and the tokens of
+  // the sequence from its first on (0: none to be read)
+  int entry_first = -1, entry_page = 0, entry_left = 0;
+  unsigned full = 0;  // a bit a stage: all of its unit's rows count; else notes has how many do
+  // where in a unit's keys row r of slab c starts: (r / 8) * step8 + c * slab + (r % 8) * SW
   const bool small_page = p.block_shift == 3;
   const uint32_t step8 = (small_page ? T::SLABS : 1) * 8 * T::SW, slab = (small_page ? 8 : 16) * T::SW;
 
+  // skips the slots that bring nothing in, over rows of this warp's share
+  auto to_unit = [&]() {
+    while (in.s < kRowCost || in.s >= in.slots) {
+      if (in.s < kRowCost) {
+        const int skip = min(kRowCost - in.s, to_issue);
+        in.s += skip;
+        to_issue -= skip;
+      }
+      if (to_issue == 0) return;
+      if (in.s >= in.slots && (in.next_row(p) || p.n_sel >= 0)) entry_first = -1;
+    }
+  };
+  to_unit();
+
   auto issue = [&](int stage) {
     if (to_issue == 0) return;
-    const int idx = small_page ? in.u * 2 : in.u >> (p.block_shift - 4);
-    const int hk = in.hc / p.chunks;
-    if (entry_first < 0 || idx - entry_first >= 32) {
+    const int u = in.s - kRowCost, hk = in.hk;
+    const int idx = small_page ? u * 2 : u >> (p.block_shift - 4);
+    if (entry_first < 0 || unsigned(idx - entry_first) >= 32u) {
       entry_first = idx;
       int j = idx + lane;
-      if (p.n_sel >= 0)
-        j = j < p.n_sel ? p.selected[in.b * p.s_sb + hk * p.s_sh + j * p.s_si] : -1;
-      entry_logical = j;
-      entry_page = j >= 0 && j < p.g.wide && (int64_t(j) << p.block_shift) < in.len ? paged_block(p.g, in.b, j) : -1;
+      if (p.n_sel >= 0) j = j < p.n_sel ? p.selected[in.b * p.s_sb + hk * p.s_sh + j * p.s_si] : -1;
+      entry_left = 0;
+      if (j >= 0 && j < p.g.wide && (int64_t(j) << p.block_shift) < in.len) {
+        entry_page = paged_block(p.g, in.b, j);
+        if (entry_page >= 0) entry_left = in.len - (j << p.block_shift);
+      }
     }
     const uint32_t dst = ring + stage * 2 * T::HALF, bar = bars + stage * 8;
-    unsigned rows = 0;
+    const int e = idx - entry_first;
+    int page = __shfl_sync(0xffffffffu, entry_page, e);
+    int n = __shfl_sync(0xffffffffu, entry_left, e);
+    unsigned rows;
     if (!small_page) {
-      const int page = __shfl_sync(0xffffffffu, entry_page, idx - entry_first);
-      const int j = __shfl_sync(0xffffffffu, entry_logical, idx - entry_first);
-      const int off = (in.u & ((1 << (p.block_shift - 4)) - 1)) * kUnit;
-      const int64_t n = int64_t(in.len) - ((int64_t(j) << p.block_shift) + off);
-      if (page >= 0 && n > 0) {
-        rows = unsigned(n >= 8 ? 8 : n) | unsigned(n >= 16 ? 8 : n > 8 ? n - 8 : 0) << 4;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar, 2 * T::HALF);
+      const int off = (u & ((1 << (p.block_shift - 4)) - 1)) * kUnit;
+      n -= off;
+      rows = n >= 16 ? 0x88u : n <= 0 ? 0u : unsigned(min(n, 8)) | unsigned(max(n - 8, 0)) << 4;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, rows ? 2 * T::HALF : 0);  // nothing to bring: the phase ends at once
+        if (rows) {
           tma_load_5d(dst, &kmap, 0, off, 0, hk, page, bar);
           tma_load_5d(dst + T::HALF, &vmap, 0, off, 0, hk, page, bar);
         }
       }
     } else {
-      uint32_t bytes = 0;
-      int page[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        page[i] = __shfl_sync(0xffffffffu, entry_page, idx - entry_first + i);
-        const int j = __shfl_sync(0xffffffffu, entry_logical, idx - entry_first + i);
-        const int64_t n = int64_t(in.len) - (int64_t(j) << 3);
-        if (page[i] >= 0 && n > 0) {
-          rows |= unsigned(n >= 8 ? 8 : n) << (4 * i);
-          bytes += T::HALF;
-        } else {
-          page[i] = -1;
+      const int page1 = __shfl_sync(0xffffffffu, entry_page, e + 1);
+      const int n1 = __shfl_sync(0xffffffffu, entry_left, e + 1);
+      rows = unsigned(max(0, min(n, 8))) | unsigned(max(0, min(n1, 8))) << 4;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, (n > 0 ? T::HALF : 0) + (n1 > 0 ? T::HALF : 0));
+        if (n > 0) {
+          tma_load_5d(dst, &kmap, 0, 0, 0, hk, page, bar);
+          tma_load_5d(dst + T::HALF, &vmap, 0, 0, 0, hk, page, bar);
+        }
+        if (n1 > 0) {
+          tma_load_5d(dst + T::HALF / 2, &kmap, 0, 0, 0, hk, page1, bar);
+          tma_load_5d(dst + T::HALF + T::HALF / 2, &vmap, 0, 0, 0, hk, page1, bar);
         }
       }
-      if (rows && lane == 0) {
-        mbar_arrive_expect_tx(bar, bytes);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (page[i] >= 0) {
-            tma_load_5d(dst + i * T::HALF / 2, &kmap, 0, 0, 0, hk, page[i], bar);
-            tma_load_5d(dst + T::HALF + i * T::HALF / 2, &vmap, 0, 0, 0, hk, page[i], bar);
-          }
-      }
     }
-    if (!rows && lane == 0) mbar_arrive_expect_tx(bar, 0);  // nothing to bring: the phase ends at once
-    live = (live & ~(0xffull << (8 * stage))) | (static_cast<unsigned long long>(rows) << (8 * stage));
-    if (--to_issue && ++in.u == in.units) {
-      in.next_row(p);
-      entry_first = -1;
+    if (rows == 0x88u) full |= 1u << stage;
+    else {
+      full &= ~(1u << stage);
+      asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(notes + stage * 4), "r"(rows) : "memory");  // every lane the same
     }
+    ++in.s;
+    if (--to_issue) to_unit();
   };
 
 #pragma unroll 1
@@ -373,52 +527,56 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
   int stage = 0;
   unsigned phase = 0;
   bool lost = false;
-  int64_t seg_first = first;
   float o[KSTEPS][NT][4], mrow[NT][2], lrow[NT][2];
   while (left > 0 || one_row) {
-    const int n = min(left, at.units - at.u);  // this warp's units of the row
-    const int hk = at.hc / p.chunks, h0 = (at.hc % p.chunks) * NH;
-    const int nheads = min(NH, p.G - h0);
-    // ---- query fragments (B operand of K Q^T)
+    const int here = min(left, at.slots - at.s);  // this warp's slots of the row, and units:
+    const int n = max(0, here - max(0, kRowCost - at.s));
+    const bool whole = n == at.slots - kRowCost;
+    left -= here;
+    if (n == 0 && !one_row) break;  // the row's cost alone, at the end of the share
+    const int hk = at.hk, h0 = at.chunk * NH, nheads = min(NH, p.G - h0);
+    // ---- query fragments (B operand of K Q^T): 16-bit tiles take channels 2tq, 2tq+1, 2tq+8, 2tq+9 of a
+    // step, 8-bit ones 4tq..4tq+3
     uint32_t qb[KSTEPS][NT][2];
     float mul = p.scale_log2;
-    {
-      float qv[KSTEPS][NT][4], amax = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < KSTEPS; ++kk)
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool ok = nt * 8 + g < nheads;
+      const uint16_t* row = static_cast<const uint16_t*>(p.q) + at.b * p.q_sb +
+                            int64_t(hk * p.G + h0 + (ok ? nt * 8 + g : 0)) * p.q_sh + (FP8 ? 4 : 2) * tq;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int hl = nt * 8 + g;
-          const bool ok = hl < nheads;
-          const int64_t off = at.b * p.q_sb + int64_t(hk * p.G + h0 + (ok ? hl : 0)) * p.q_sh;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // 16-bit tiles: channels 2tq, 2tq+1, 2tq+8, 2tq+9 of a step; 8-bit: 4tq..4tq+3
-            const int c = FP8 ? kk * 16 + 4 * tq + e : kk * 16 + 2 * tq + (e & 1) + (e >> 1) * 8;
-            float x = 0.f;
-            if (ok) x = KIND == kBf16 ? to_f32(reinterpret_cast<const __nv_bfloat16*>(p.q)[off + c * p.q_sd])
-                                      : load_as(p.q, p.q_dtype, off + c * p.q_sd);
-            qv[kk][nt][e] = x;
-            amax = fmaxf(amax, fabsf(x));
-          }
-        }
-      float qscale = 1.f;
-      if (FP8) {  // a power of two that keeps |q| within f16 (exact)
-        amax = warp_max(amax);
-        int ex = 0;
-        frexpf(amax, &ex);
-        const int shift = ex > 15 && amax <= FLT_MAX ? ex - 15 : 0;
-        qscale = ldexpf(1.f, -shift);
-        mul = ldexpf(p.scale_log2, shift);
+      for (int kk = 0; kk < KSTEPS; ++kk) {
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(row + kk * 16);
+        const uint32_t y = *reinterpret_cast<const uint32_t*>(row + kk * 16 + (FP8 ? 2 : 8));
+        qb[kk][nt][0] = ok ? x : 0u;
+        qb[kk][nt][1] = ok ? y : 0u;
       }
+    }
+    if (FP8 && p.q_dtype == BD_BF16) {
+      // as f16 times a power of two that puts the largest at 2^14..2^15 (exact down to 2^-31 of it)
+      float amax = 0.f;
 #pragma unroll
       for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            qb[kk][nt][i] = KIND == kBf16 ? pack_bf16x2(qv[kk][nt][2 * i], qv[kk][nt][2 * i + 1])
-                                          : pack_f16x2(qv[kk][nt][2 * i] * qscale, qv[kk][nt][2 * i + 1] * qscale);
+            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(qb[kk][nt][i] << 16)),
+                                     fabsf(__uint_as_float(qb[kk][nt][i] & 0xffff0000u))));
+      amax = warp_max(amax);
+      int ex = 0;
+      frexpf(amax, &ex);
+      const int shift = amax > 0.f && amax <= FLT_MAX ? max(ex - 15, -100) : 0;
+      const float f = ldexpf(1.f, -shift);
+      mul = ldexpf(p.scale_log2, shift);
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            qb[kk][nt][i] = pack_f16x2(__uint_as_float(qb[kk][nt][i] << 16) * f,
+                                       __uint_as_float(qb[kk][nt][i] & 0xffff0000u) * f);
     }
 #pragma unroll
     for (int mt = 0; mt < KSTEPS; ++mt)
@@ -433,24 +591,26 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
     for (int i = 0; i < n; ++i) {
       if (!lost && !mbar_wait(bars + stage * 8, phase)) {
         lost = true;
-        to_issue = 0;
         if (lane == 0) atomicAdd(&g_paged_timeouts, 1u);
       }
       lost = __any_sync(0xffffffffu, lost);
       if (lost) break;
-      const unsigned rows = unsigned(live >> (8 * stage)) & 0xffu;
+      unsigned rows = 0x88u;
+      if (!(full >> stage & 1)) asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(rows) : "r"(notes + stage * 4) : "memory");
       const int nv0 = rows & 15, nv1 = rows >> 4;
       if (rows) {
         const uint32_t ks = ring + stage * 2 * T::HALF, vs = ks + T::HALF;
         if (rows != 0x88u) {
           // rows past the sequence's end hold whatever was there: their weights are zero, and so must
           // their values be (zero times infinity is not zero)
-          for (int e = lane; e < kUnit * T::ROWB / 16; e += 32) {
-            const int r = e / (T::ROWB / 16), c = e % (T::ROWB / 16);
-            const uint32_t a = vs + (r >> 3) * step8 + (c * 16 / T::SW) * slab + (r & 7) * T::SW + c * 16 % T::SW;
-            if ((r & 7) >= (r < 8 ? nv0 : nv1))  // whole rows: the swizzle moves chunks within a row only
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(a), "r"(0) : "memory");
-          }
+          constexpr int CH = T::ROWB / 16;  // whole rows: the swizzle moves a row's chunks within it only
+          const int c = lane % CH;
+#pragma unroll 1
+          for (int r = lane / CH; r < kUnit; r += 32 / CH)
+            if ((r & 7) >= (r < 8 ? nv0 : nv1)) {
+              const uint32_t to = vs + (r >> 3) * step8 + (c * 16 / T::SW) * slab + (r & 7) * T::SW + c * 16 % T::SW;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(to), "r"(0) : "memory");
+            }
           fence_proxy_async();
           __syncwarp();
         }
@@ -462,11 +622,11 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
         // chunk ^ (row / 2 % 4) (64-byte rows)
         const uint32_t x = (T::SW == 128 ? lane & 7 : (lane >> 1) & 3) * 16;
         {
-          const uint32_t base = ks + ((lane >> 3) & 1) * step8 + (lane & 7) * T::SW, hi = uint32_t(lane >> 4) * 16;
+          const uint32_t from = ks + ((lane >> 3) & 1) * step8 + (lane & 7) * T::SW, hi = uint32_t(lane >> 4) * 16;
 #pragma unroll
           for (int c = 0; c < T::ROWB / 32; ++c) {
             uint32_t r0, r1, r2, r3;
-            ldmatrix_x4(r0, r1, r2, r3, base + (c * 32 / T::SW) * slab + ((c * 32 % T::SW) ^ (hi ^ x)));
+            ldmatrix_x4(r0, r1, r2, r3, from + (c * 32 / T::SW) * slab + ((c * 32 % T::SW) ^ (hi ^ x)));
             if (!FP8) {
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
@@ -533,22 +693,22 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
         }
         // ---- O^T += V^T P^T
         if (!FP8) {
-          const uint32_t base = vs + (lane >> 4) * step8 + (lane & 7) * T::SW, hi = uint32_t((lane >> 3) & 1) * 16;
+          const uint32_t from = vs + (lane >> 4) * step8 + (lane & 7) * T::SW, hi = uint32_t((lane >> 3) & 1) * 16;
 #pragma unroll
           for (int mt = 0; mt < KSTEPS; ++mt) {
             uint32_t a0, a1, a2, a3;
-            ldmatrix_x4_trans(a0, a1, a2, a3, base + (mt * 32 / T::SW) * slab + ((mt * 32 % T::SW) ^ (hi ^ x)));
+            ldmatrix_x4_trans(a0, a1, a2, a3, from + (mt * 32 / T::SW) * slab + ((mt * 32 % T::SW) ^ (hi ^ x)));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               if (KIND == kBf16) mma_bf16(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
               else mma_f16(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
           }
         } else {
-          const uint32_t base = vs + ((lane >> 3) & 1) * step8 + (lane & 7) * T::SW, hi = uint32_t(lane >> 4) * 16;
+          const uint32_t from = vs + ((lane >> 3) & 1) * step8 + (lane & 7) * T::SW, hi = uint32_t(lane >> 4) * 16;
 #pragma unroll
           for (int m2 = 0; m2 < KSTEPS / 2; ++m2) {
             uint32_t r0, r1, r2, r3;
-            ldmatrix_x4_trans(r0, r1, r2, r3, base + (m2 * 32 / T::SW) * slab + ((m2 * 32 % T::SW) ^ (hi ^ x)));
+            ldmatrix_x4_trans(r0, r1, r2, r3, from + (m2 * 32 / T::SW) * slab + ((m2 * 32 % T::SW) ^ (hi ^ x)));
             // r0, r1: tokens 0-7, 8-15 of channels [32 m2, +16); r2, r3: of the next 16; each holds
             // (token 2tq: channels 2g, 2g+1 | token 2tq+1: the same)
             const uint32_t a0 = e4m3x2_to_f16x2(prmt(r0, 0, 0x0020)), a1 = e4m3x2_to_f16x2(prmt(r0, 0, 0x0031));
@@ -580,44 +740,60 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
         lrow[nt][j] = lost ? NAN : l;
         mrow[nt][j] = lost ? 0.f : mrow[nt][j] - kUp;  // of sums that are 2^kUp times as large
       }
-    left -= n;
-    if (one_row) break;  // the warp's only segment: joined with the others' below
-    const bool whole = n == at.units;
-    const int64_t slot = 2 * int64_t(w) + (seg_first != first);
+    if (one_row) break;  // the warp's only row: joined with the others' parts below
+    if (whole) {
+      // 8x8 transposes give a thread neighbouring channels of head g
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float inv[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int h = nt * 8 + 2 * tq + j;
-        if (h >= nheads) continue;
-        const float m = mrow[nt][j], l = lrow[nt][j];
-        if (whole) {
-          const int hq = hk * p.G + h0 + h;
-          const float f = m == -INFINITY ? 0.f : p.v_scale / l;
-          const int64_t off = at.b * p.o_sb + int64_t(hq) * p.o_sh;
+        for (int j = 0; j < 2; ++j) {
+          const float m = mrow[nt][j], l = lrow[nt][j];
+          inv[j] = m == -INFINITY ? 0.f : p.v_scale / l;
+          const int h = nt * 8 + 2 * tq + j;
+          if (p.lse && g == 0 && h < nheads)
+            p.lse[at.b * p.e_sb + (hk * p.G + h0 + h) * p.e_sh] = m == -INFINITY ? -INFINITY : m * kLn2 + logf(l);
+        }
+        uint16_t* to = static_cast<uint16_t*>(p.out) + at.b * p.o_sb + int64_t(hk * p.G + h0 + nt * 8 + g) * p.o_sh +
+                       (FP8 ? 4 : 2) * tq;
+        const bool ok = nt * 8 + g < nheads;
 #pragma unroll
-          for (int mt = 0; mt < KSTEPS; ++mt) {
-            const int ca = FP8 ? mt * 16 + 2 * g : mt * 16 + g, cb = FP8 ? ca + 1 : ca + 8;
-            store_as(p.out, p.out_dtype, off + ca * p.o_sd, o[mt][nt][j] * f);
-            store_as(p.out, p.out_dtype, off + cb * p.o_sd, o[mt][nt][2 + j] * f);
-          }
-          if (p.lse && g == 0)
-            p.lse[at.b * p.e_sb + hq * p.e_sh] = m == -INFINITY ? -INFINITY : m * kLn2 + logf(l);
-        } else {
-          float* po = p.part_o + (slot * NH + h) * D;
-#pragma unroll
-          for (int mt = 0; mt < KSTEPS; ++mt) {
-            const int ca = FP8 ? mt * 16 + 2 * g : mt * 16 + g, cb = FP8 ? ca + 1 : ca + 8;
-            po[ca] = o[mt][nt][j];
-            po[cb] = o[mt][nt][2 + j];
-          }
-          if (g == 0) {
-            p.part_m[slot * NH + h] = m;
-            p.part_l[slot * NH + h] = l;
+        for (int mt = 0; mt < KSTEPS; ++mt) {
+          const uint32_t x = movmatrix_trans(pack_out(p, o[mt][nt][0] * inv[0], o[mt][nt][1] * inv[1]));
+          const uint32_t y = movmatrix_trans(pack_out(p, o[mt][nt][2] * inv[0], o[mt][nt][3] * inv[1]));
+          if (!ok) continue;
+          if (FP8) {  // x: channels 4tq, 4tq + 2 of the step, y: 4tq + 1, 4tq + 3
+            *reinterpret_cast<uint2*>(to + mt * 16) = make_uint2(prmt(x, y, 0x5410), prmt(x, y, 0x7632));
+          } else {
+            *reinterpret_cast<uint32_t*>(to + mt * 16) = x;
+            *reinterpret_cast<uint32_t*>(to + mt * 16 + 8) = y;
           }
         }
       }
-    seg_first += n;
+    } else {
+      const int64_t slot = 2 * int64_t(w) + (at.s == 0);  // 0: the row began before this share
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int h = nt * 8 + 2 * tq + j;
+          if (h >= nheads) continue;
+          float* po = p.part_o + (slot * NH + h) * D + (FP8 ? 2 * g : g);
+#pragma unroll
+          for (int mt = 0; mt < KSTEPS; ++mt) {
+            if (FP8) {
+              *reinterpret_cast<float2*>(po + mt * 16) = make_float2(o[mt][nt][j], o[mt][nt][2 + j]);
+            } else {
+              po[mt * 16] = o[mt][nt][j];
+              po[mt * 16 + 8] = o[mt][nt][2 + j];
+            }
+          }
+          if (g == 0) {
+            p.part_m[slot * NH + h] = mrow[nt][j];
+            p.part_l[slot * NH + h] = lrow[nt][j];
+          }
+        }
+    }
     if (left > 0) at.next_row(p);
   }
   // a copy that was given up is still waited for (again with a limit) before the memory goes
@@ -648,151 +824,175 @@ __global__ void __launch_bounds__(TileShape<D, KIND>::WARPS * 32, 1)
 #pragma unroll
       for (int i = 0; i < T::WARPS; ++i) M = fmaxf(M, sm[i * NH + h]);
       const float f = mrow[nt][j] == -INFINITY ? 0.f : exp2f(mrow[nt][j] - M);
-      float* to = so + (warp * NH + h) * D;
+      float* to = so + (warp * NH + h) * D + (FP8 ? 2 * g : g);
 #pragma unroll
       for (int mt = 0; mt < KSTEPS; ++mt) {
-        const int ca = FP8 ? mt * 16 + 2 * g : mt * 16 + g, cb = FP8 ? ca + 1 : ca + 8;
-        to[ca] = o[mt][nt][j] * f;
-        to[cb] = o[mt][nt][2 + j] * f;
+        to[mt * 16] = o[mt][nt][j] * f;
+        to[mt * 16 + (FP8 ? 1 : 8)] = o[mt][nt][2 + j] * f;
       }
     }
   __syncthreads();
-  const int64_t slot = 2 * int64_t(w - warp);
-  const int nheads = min(NH, p.G - (at.hc % p.chunks) * NH);
+  const int64_t slot = 2 * int64_t(w - warp) + row_begins;
+  const int nheads = min(NH, p.G - at.chunk * NH);
   for (int e = threadIdx.x; e < nheads * (D / 4); e += T::WARPS * 32) {
     const int h = e / (D / 4), c = e % (D / 4);
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    Sum4 x = Sum4::none();
 #pragma unroll
     for (int i = 0; i < T::WARPS; ++i) {
       const float4 y = reinterpret_cast<const float4*>(so + (i * NH + h) * D)[c];
-      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      x.o.x += y.x; x.o.y += y.y; x.o.z += y.z; x.o.w += y.w;
+      x.m = fmaxf(x.m, sm[i * NH + h]);
     }
-    reinterpret_cast<float4*>(p.part_o + (slot * NH + h) * D)[c] = x;
-    if (c) continue;
-    float M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int i = 0; i < T::WARPS; ++i) M = fmaxf(M, sm[i * NH + h]);
-#pragma unroll
-    for (int i = 0; i < T::WARPS; ++i) L += sm[i * NH + h] == -INFINITY ? 0.f : sl[i * NH + h] * exp2f(sm[i * NH + h] - M);
-    p.part_m[slot * NH + h] = M;
-    p.part_l[slot * NH + h] = L;
+    for (int i = 0; i < T::WARPS; ++i)
+      x.l += sm[i * NH + h] == -INFINITY ? 0.f : sl[i * NH + h] * exp2f(sm[i * NH + h] - x.m);
+    if (p.row_mode) {
+      x.write(p, at.b, at.hk * p.G + at.chunk * NH + h, c);
+      continue;
+    }
+    reinterpret_cast<float4*>(p.part_o + (slot * NH + h) * D)[c] = x.o;
+    if (c == 0) {
+      p.part_m[slot * NH + h] = x.m;
+      p.part_l[slot * NH + h] = x.l;
+    }
   }
 }
 
-// Joins the parts of the rows that more than one warp had, and writes the rows that have no token.
-// One CTA per HEADS query heads of a row. The parts of a row: one for every CTA of the tile kernel whose
-// units all lie in it, one for every warp of the CTAs at its ends otherwise; 32 of them at a time get
-// their weights in shared memory, then a thread adds 4 channels of one head up over every SLICES-th part.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinParts = 32;
-
-template <int D, int WARPS, int HEADS>
-__global__ void __launch_bounds__(kJoinThreads) paged_tile_join_kernel(const AttnParams p) {
-  constexpr int PER = D / 4, SLICES = kJoinThreads / (PER * HEADS);
-  __shared__ float4 red[SLICES][HEADS][PER];
-  __shared__ float weight[HEADS][kJoinParts], row_m[HEADS], row_l[HEADS], back[HEADS];
-  __shared__ int64_t part_slot[kJoinParts];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int groups = (min(p.heads, p.G) + HEADS - 1) / HEADS;  // of a chunk's heads
-  const int hc = blockIdx.x / groups, h0 = (blockIdx.x % groups) * HEADS, b = blockIdx.y;
-  const int hq0 = (hc / p.chunks) * p.G + (hc % p.chunks) * p.heads + h0;
-  const int nheads = min(HEADS, min(p.heads, p.G - (hc % p.chunks) * p.heads) - h0);
-  const int part = threadIdx.x % PER, head = threadIdx.x / PER % HEADS, slice = threadIdx.x / (PER * HEADS);
-  const int units = row_units(p, paged_len(p.g, b));
-  const int64_t out = b * p.o_sb + (hq0 + head) * p.o_sh;
-  if (units == 0 && slice == 0 && head < nheads) {
-    for (int i = 0; i < 4; ++i) store_as(p.out, p.out_dtype, out + (4 * part + i) * p.o_sd, 0.f);
-    if (p.lse && part == 0) p.lse[b * p.e_sb + (hq0 + head) * p.e_sh] = -INFINITY;
-  }
-  // units of all sequences, and of those before this one
-  int64_t all = 0, before = 0;
-  for (int i = lane; i < p.g.B; i += 32) {
-    const int n = row_units(p, paged_len(p.g, i));
-    all += n;
-    if (i < b) before += n;
-  }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, s);
-    before += __shfl_xor_sync(0xffffffffu, before, s);
-  }
-  const int per = p.g.Hk * p.chunks;
-  all *= per;
-  const Shares<WARPS> sh(all, p.warps);
-  const int64_t u0 = before * per + int64_t(hc) * units, u1 = u0 + units;
-  int w0 = 0, w1 = 0, c0 = 0, c1 = 0, n0 = 0, n1 = 0, n = 0;
-  bool in0 = false, in1 = false;
-  if (units > 0 && nheads > 0) {
-    w0 = sh.owner(u0);
-    w1 = sh.owner(u1 - 1);
-    // the CTAs with units of the row, and whether those at its ends have units of it only
+// The parts of a row: one for every CTA of the tile kernel whose share lies in it, one for every warp of the
+// CTAs at its ends otherwise; none if one warp had all of its units and wrote it.
+template <int WARPS>
+struct Parts {
+  int w0, c0, c1, n0, n1, n, s0;
+  bool in0;
+  __device__ __forceinline__ Parts(const Shares<WARPS>& sh, int first, int end) : s0(first) {
+    w0 = sh.owner(first + kRowCost);  // of the first unit, and of the last
+    const int w1 = sh.owner(end - 1);
     c0 = w0 / WARPS;
     c1 = w1 / WARPS;
-    in0 = sh.cta(c0) >= u0 && sh.cta(c0 + 1) <= u1;
-    in1 = sh.cta(c1) >= u0 && sh.cta(c1 + 1) <= u1;
-    // parts of the first (a CTA with fewer units than warps leaves its last warps without one), of the
-    // last, and of all of them; none if one warp had the whole row and wrote it
+    // whether their CTAs have slots of this row only
+    in0 = sh.cta(c0) >= first && sh.cta(c0 + 1) <= end;
+    const bool in1 = sh.cta(c1) >= first && sh.cta(c1 + 1) <= end;
+    // (a CTA with fewer slots than warps leaves its last warps without a part)
     n0 = in0 ? 1 : min(w1, sh.owner(sh.cta(c0 + 1) - 1)) - w0 + 1;
     n1 = c1 == c0 ? 0 : in1 ? 1 : w1 - c1 * WARPS + 1;
     n = w0 == w1 && !in0 ? 0 : n0 + max(0, c1 - c0 - 1) + n1;
   }
-  griddep_wait();  // also for a kernel that waits for this one: it then finds the tile kernel done as well
-  if (n == 0) return;
-  if (threadIdx.x < HEADS) row_m[threadIdx.x] = -INFINITY, row_l[threadIdx.x] = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int first = 0; first < n; first += kJoinParts) {
-    const int here = min(kJoinParts, n - first);
-    __syncthreads();
-    // ---- weights of up to 32 parts, relative to the largest maximum so far: a warp a head
-    for (int hh = warp; hh < nheads; hh += kJoinThreads / 32) {
-      float m = -INFINITY, l = 0.f;
-      if (lane < here) {
-        const int i = first + lane;
-        const int w = i < n0 ? (in0 ? c0 * WARPS : w0 + i)
-                      : i < n - n1 ? (c0 + 1 + i - n0) * WARPS : c1 * WARPS + (i - (n - n1));
-        const int64_t slot = (2 * int64_t(w) + (sh.begin(w) < u0)) * p.heads + h0;
-        if (hh == 0) part_slot[lane] = slot;
-        m = __ldcg(p.part_m + slot + hh);
-        l = __ldcg(p.part_l + slot + hh);
-      }
-      const float M = row_m[hh], Mn = fmaxf(M, warp_max(m));
-      const float f = m == -INFINITY ? 0.f : exp2f(m - Mn), r = M == -INFINITY ? 0.f : exp2f(M - Mn);
-      l = warp_sum(l * f);
-      __syncwarp();
-      weight[hh][lane] = f;
-      if (lane == 0) row_m[hh] = Mn, back[hh] = r, row_l[hh] = row_l[hh] * r + l;
-    }
-    __syncthreads();
-    if (head >= nheads) continue;
-    const float r = back[head];
-    acc.x *= r; acc.y *= r; acc.z *= r; acc.w *= r;
-#pragma unroll 8
-    for (int i = slice; i < here; i += SLICES) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + (part_slot[i] + head) * D) + part);
-      const float f = weight[head][i];
-      acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
-      acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
-    }
+  // Where part i is.
+  __device__ __forceinline__ int64_t slot(const Shares<WARPS>& sh, int i) const {
+    const int w = i < n0 ? (in0 ? c0 * WARPS : w0 + i) : i < n - n1 ? (c0 + 1 + i - n0) * WARPS : c1 * WARPS + (i - (n - n1));
+    return 2 * int64_t(w) + (sh.begin(w) <= s0);
   }
+};
+
+// Adds parts i, i + step, ... of head h, channels 4 * part..; four of them in flight.
+template <int D, int WARPS>
+__device__ __forceinline__ void add_parts(Sum4& sum, const AttnParams& p, const Parts<WARPS>& parts,
+                                          const Shares<WARPS>& sh, int h, int part, int i, int step) {
+  for (; i < parts.n; i += 4 * step) {
+    float m[4], l[4];
+    float4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t at = parts.slot(sh, min(i + k * step, parts.n - 1)) * p.heads + h;
+      m[k] = __ldcg(p.part_m + at);
+      l[k] = __ldcg(p.part_l + at);
+      x[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + part);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k * step < parts.n) sum.add(m[k], l[k], x[k]);
+  }
+}
+
+// Joins the parts of the rows that more than one warp had, and writes the rows that have no token. One CTA
+// per HEADS query heads of a row, its threads 4 channels of a head and every SLICES-th part. What depends on
+// the lengths alone is done before the wait for the tile kernel.
+constexpr int kJoinThreads = 256;
+
+template <int D, int WARPS, int HEADS>
+__global__ void __launch_bounds__(kJoinThreads) paged_tile_join_kernel(const AttnParams p) {
+  constexpr int PER = D / 4, SLICES = kJoinThreads / (PER * HEADS);
+  __shared__ Sum4 red[SLICES][HEADS][PER];
+  const int groups = (min(p.heads, p.G) + HEADS - 1) / HEADS;  // of a chunk's heads
+  const int hc = blockIdx.x / groups, hk = hc / p.chunks, chunk = hc - hk * p.chunks, b = blockIdx.y;
+  const int part = threadIdx.x % PER, slice = threadIdx.x / (PER * HEADS), lane = threadIdx.x & 31;
+  const int hl = threadIdx.x / PER % HEADS, h = (blockIdx.x - hc * groups) * HEADS + hl;
+  const bool some = h < p.heads && chunk * p.heads + h < p.G;  // a head of this row
+  int all = 0, before = 0;  // slots of all sequences, and of those before this one
+  for (int i = lane; i < p.g.B; i += 32) {
+    const int n = row_slots(p, paged_len(p.g, i));
+    all += n;
+    if (i < b) before += n;
+  }
+  const int per = p.g.Hk * p.chunks, slots = row_slots(p, paged_len(p.g, b));
+  const Shares<WARPS> sh(__reduce_add_sync(0xffffffffu, all) * per, p.warps);
+  const int s0 = __reduce_add_sync(0xffffffffu, before) * per + hc * slots;
+  const Parts<WARPS> parts(sh, s0, s0 + max(slots, kRowCost + 1));
+  griddep_wait();  // also for a kernel that waits for this one: it then finds the tile kernel done as well
+  if (slots > 0 && (slots <= sh.whole || parts.n == 0)) return;  // one warp had all of it, and wrote it
+  Sum4 sum = Sum4::none();
+  if (slots > 0 && some) add_parts<D>(sum, p, parts, sh, h, part, slice, SLICES);
   if (SLICES > 1) {
-    red[slice][head][part] = acc;
+    red[slice][hl][part] = sum;
     __syncthreads();
     if (slice) return;
-#pragma unroll
-    for (int i = 1; i < SLICES; ++i) {
-      const float4 x = red[i][head][part];
-      acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+#pragma unroll 1
+    for (int i = 1; i < SLICES; ++i) sum.add(red[i][hl][part].m, red[i][hl][part].l, red[i][hl][part].o);
+  }
+  if (some) sum.write(p, b, hk * p.G + chunk * p.heads + h, part);
+}
+
+// The same for many rows, of which few are cut: CTA 2c joins the row that the border before share c of the
+// tile kernel is the first to cut, its warps every eighth part; CTA 2c + 1 those within share c, a warp each
+// (warp w's is the one whose first cut is the beginning of w's share). All heads of a row, PER lanes
+// a head.
+template <int D, int WARPS>
+__global__ void __launch_bounds__(kJoinThreads) paged_tile_join_cuts_kernel(const AttnParams p) {
+  constexpr int PER = D / 4, JW = kJoinThreads / 32, LANES = PER < 32 ? PER : 32, HEADS = 32 / LANES, TURNS = PER / LANES;
+  __shared__ Sum4 red[JW][32];
+  __shared__ GroupSums groups;
+  const int c = blockIdx.x >> 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool within = blockIdx.x & 1;
+  ListSums list;
+  list.build<JW>(p, groups, warp, lane);
+  const Shares<WARPS> sh(list.total, p.warps);
+  // sequences without a token
+  for (int b = blockIdx.x; b < p.g.B; b += gridDim.x)
+    if (row_slots(p, paged_len(p.g, b)) == 0)
+      for (int i = threadIdx.x; i < p.Hq * PER; i += kJoinThreads) Sum4::none().write(p, b, i / PER, i % PER);
+  const int first_cta = sh.cta(c), end_cta = sh.cta(c + 1);
+#pragma unroll 1
+  for (int i = within ? 1 + warp : 0; i < (within ? WARPS : 1); i += JW) {
+    const int w = c * WARPS + i, at_slot = sh.begin(w);
+    Place at;
+    if (at_slot < end_cta) at.find(p, list, groups, at_slot, lane);
+    griddep_wait();
+    if (at_slot >= end_cta) continue;
+    const int s0 = at_slot - at.s, s1 = s0 + at.slots;
+    if (at.slots <= sh.whole) continue;  // not cut at all
+    if (within ? at.s == 0 || s0 < first_cta || s1 > end_cta || sh.begin(w - 1) > s0 || (s0 == first_cta && s1 == end_cta)
+               : at.s == 0 ? s1 != end_cta : sh.cta(c - 1) > s0)
+      continue;
+    const Parts<WARPS> parts(sh, s0, s1);
+    if (parts.n == 0) continue;
+    const int nheads = min(p.heads, p.G - at.chunk * p.heads), hq = at.hk * p.G + at.chunk * p.heads;
+#pragma unroll 1
+    for (int k = 0; k < nheads * TURNS; k += HEADS) {
+      const int h = TURNS > 1 ? k / TURNS : k + lane / LANES, part = lane % LANES + (TURNS > 1 ? k % TURNS * LANES : 0);
+      Sum4 sum = Sum4::none();
+      if (h < nheads) add_parts<D>(sum, p, parts, sh, h, part, within ? 0 : warp, within ? 1 : JW);
+      if (!within) {
+        red[warp][lane] = sum;
+        __syncthreads();
+        sum = red[0][lane];
+#pragma unroll 1
+        for (int j = 1; j < JW; ++j) sum.add(red[j][lane].m, red[j][lane].l, red[j][lane].o);
+        __syncthreads();
+      }
+      if (h < nheads && (within || warp == 0)) sum.write(p, at.b, hq + h, part);
     }
   }
-  if (head >= nheads) return;
-  const float M = row_m[head], L = row_l[head];
-  const float f = M == -INFINITY ? 0.f : p.v_scale / L;
-  store_as(p.out, p.out_dtype, out + 4 * part * p.o_sd, acc.x * f);
-  store_as(p.out, p.out_dtype, out + (4 * part + 1) * p.o_sd, acc.y * f);
-  store_as(p.out, p.out_dtype, out + (4 * part + 2) * p.o_sd, acc.z * f);
-  store_as(p.out, p.out_dtype, out + (4 * part + 3) * p.o_sd, acc.w * f);
-  if (p.lse && part == 0)
-    p.lse[b * p.e_sb + (hq0 + head) * p.e_sh] = M == -INFINITY ? -INFINITY : M * kLn2 + logf(L);
+  griddep_wait();
 }
 
 // Whether the tiles can take a call: 16-bit queries and caches of one type, or 8-bit caches; pages of
@@ -807,27 +1007,64 @@ bool tile_layout(const bd_tensor* t) {
   return true;
 }
 
+int64_t most_slots(const AttnParams& p, int chunks) {
+  const int64_t tokens = int64_t(p.n_sel >= 0 ? p.n_sel : p.g.wide) * p.g.block;
+  return ((tokens + kUnit - 1) / kUnit + kRowCost) * p.g.Hk * chunks * p.g.B;
+}
+
+// 16-bit rows of contiguous channels on `align` bytes.
+bool rows_on(const void* data, int dtype, int64_t sb, int64_t sh, int64_t sd, size_t align) {
+  return dtype != BD_F32 && sd == 1 && !((reinterpret_cast<uintptr_t>(data) | size_t(sb) * 2 | size_t(sh) * 2) & (align - 1));
+}
+
 bool use_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v_cache) {
   const int D = p.g.D;
   if (D != 64 && D != 128 && D != 256) return false;
   const bool types = (p.kv_dtype == BD_BF16 && p.q_dtype == BD_BF16) || (p.kv_dtype == BD_F16 && p.q_dtype == BD_F16) ||
                      (p.kv_dtype == BD_F8E4M3 && p.q_dtype != BD_F32);
   if (!types || p.g.block < 8 || p.g.block > 65536 || (p.g.block & (p.g.block - 1))) return false;
-  return p.g.num_blocks > 0 && tile_layout(k_cache) && tile_layout(v_cache);
+  // the list's slots are counted in 32 bits: about 2^34 tokens times KV heads that the tables can name
+  if (most_slots(p, (p.G + 7) / 8) >= int64_t(1) << 31 || int64_t(p.n_sel) * p.g.block >= int64_t(1) << 31) return false;
+  return p.g.num_blocks > 0 && rows_on(p.q, p.q_dtype, p.q_sb, p.q_sh, p.q_sd, 4) && tile_layout(k_cache) && tile_layout(v_cache);
 }
 
 // Warps of the grid: the CTAs fill the GPU once, if the block table has work for them.
-void plan_tiles(AttnParams* p, int warps_per_cta) {
+#ifndef ROW_UNITS
+#define ROW_UNITS 6
+#endif
+template <typename F>
+auto with_shape(const AttnParams& p, F&& f) {
+  auto kind = [&](auto d, auto nt) {
+    constexpr int D = decltype(d)::value;
+    switch (p.kv_dtype) {
+      case BD_BF16: return f(std::integral_constant<int, D>(), std::integral_constant<int, kBf16>(), nt);
+      case BD_F16: return f(std::integral_constant<int, D>(), std::integral_constant<int, kF16>(), nt);
+      default: return f(std::integral_constant<int, D>(), std::integral_constant<int, kFp8>(), nt);
+    }
+  };
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  if (p.g.D == 64) return p.heads == 16 ? kind(std::integral_constant<int, 64>(), two) : kind(std::integral_constant<int, 64>(), one);
+  if (p.g.D == 128) return p.heads == 16 ? kind(std::integral_constant<int, 128>(), two) : kind(std::integral_constant<int, 128>(), one);
+  return kind(std::integral_constant<int, 256>(), one);
+}
+
+void plan_tiles(AttnParams* p) {
   p->heads = p->G > 8 && p->g.D <= 128 ? 16 : 8;
   p->chunks = (p->G + p->heads - 1) / p->heads;
-  const int64_t tokens = int64_t(p->n_sel >= 0 ? p->n_sel : p->g.wide) * p->g.block;
-  const int64_t units = (tokens + kUnit - 1) / kUnit * p->g.B * p->g.Hk * p->chunks;
-  const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(num_sms(), units));
-  p->warps = int(ctas) * warps_per_cta;
+  const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(num_sms(), most_slots(*p, p->chunks) / kMinSlots));
+  const int warps = with_shape(*p, [](auto d, auto kind, auto nt) {
+    return TileShape<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>::WARPS;
+  });
+  // few rows of few tokens (as far as the block table goes): a CTA a row, no join
+  const int64_t rows = int64_t(p->g.B) * p->g.Hk * p->chunks;
+  p->row_mode = rows <= num_sms() && most_slots(*p, p->chunks) <= rows * (ROW_UNITS * warps + kRowCost);
+  p->warps = int(p->row_mode ? rows : ctas) * warps;
   p->block_shift = 31 - __builtin_clz(unsigned(p->g.block));
 }
 
 size_t tile_bytes(const AttnParams& p) {
+  if (p.row_mode) return 0;
   return size_t(2) * p.warps * p.heads * (size_t(p.g.D) + 2) * sizeof(float) + 256;
 }
 
@@ -847,9 +1084,12 @@ bool tile_map(CUtensorMap* m, const bd_tensor* t, int sw) {
                     sw == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
+#ifndef JOIN_ROWS
+#define JOIN_ROWS 4
+#endif
 template <int D, int KIND, int NT>
 int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v_cache, cudaStream_t st) {
-  using T = TileShape<D, KIND>;
+  using T = TileShape<D, KIND, NT>;
   CUtensorMap km, vm;
   if (!tile_map(&km, k_cache, T::SW) || !tile_map(&vm, v_cache, T::SW))
     return fail(BD_ERR_CUDA, "cuTensorMapEncodeTiled refused the cache's layout");
@@ -865,39 +1105,19 @@ int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor*
   }
   kern<<<p.warps / T::WARPS, T::WARPS * 32, T::SMEM, st>>>(p, km, vm);
   if ((rc = cuda_check(cudaGetLastError(), "paged_attn_tile_kernel launch"))) return rc;
-  // few rows: a CTA a head, its threads over many parts at once; many rows, which have few parts each: a
-  // CTA the heads that its threads can hold
-  constexpr int MANY = D == 256 ? 4 : 8;
-  const bool many = int64_t(p.g.B) * p.Hq > 8 * num_sms();
-  const int heads = many ? MANY : 1;
-  return launch_programmatic(many ? paged_tile_join_kernel<D, T::WARPS, MANY> : paged_tile_join_kernel<D, T::WARPS, 1>,
-                             dim3(p.g.Hk * p.chunks * ((std::min(p.heads, p.G) + heads - 1) / heads), p.g.B), dim3(kJoinThreads), 0,
-                             st, p, "paged_tile_join_kernel launch");
-}
-
-template <int D, int KIND>
-int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v_cache, cudaStream_t st) {
-  if constexpr (D <= 128)
-    if (p.heads == 16) return launch_tiles<D, KIND, 2>(p, k_cache, v_cache, st);
-  return launch_tiles<D, KIND, 1>(p, k_cache, v_cache, st);
-}
-
-template <int D>
-int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v_cache, cudaStream_t st) {
-  switch (p.kv_dtype) {
-    case BD_BF16: return launch_tiles<D, kBf16>(p, k_cache, v_cache, st);
-    case BD_F16: return launch_tiles<D, kF16>(p, k_cache, v_cache, st);
-    default: return launch_tiles<D, kFp8>(p, k_cache, v_cache, st);
-  }
-}
-
-int tile_warps(int D, int kv_dtype) {
-  auto of = [&](auto d) {
-    constexpr int N = decltype(d)::value;
-    return kv_dtype == BD_F8E4M3 ? TileShape<N, kFp8>::WARPS : TileShape<N, kBf16>::WARPS;
-  };
-  return D == 64 ? of(std::integral_constant<int, 64>()) : D == 128 ? of(std::integral_constant<int, 128>())
-                                                                   : of(std::integral_constant<int, 256>());
+  if (p.row_mode) return BD_OK;
+  const int ctas = p.warps / T::WARPS;
+  constexpr int MANY = D == 256 ? 4 : 8;  // heads that 256 threads hold at 4 channels each, 8 at most
+  const int64_t rows = int64_t(p.g.B) * p.g.Hk * p.chunks;
+  const int heads = std::min(p.heads, p.G), groups = (heads + MANY - 1) / MANY;
+  if (rows * heads <= 4 * num_sms())
+    return launch_programmatic(paged_tile_join_kernel<D, T::WARPS, 1>, dim3(p.g.Hk * p.chunks * heads, p.g.B),
+                               dim3(kJoinThreads), 0, st, p, "paged_tile_join_kernel launch");
+  if (rows * groups <= JOIN_ROWS * num_sms())
+    return launch_programmatic(paged_tile_join_kernel<D, T::WARPS, MANY>, dim3(p.g.Hk * p.chunks * groups, p.g.B),
+                               dim3(kJoinThreads), 0, st, p, "paged_tile_join_kernel launch");
+  return launch_programmatic(paged_tile_join_cuts_kernel<D, T::WARPS>, dim3(2 * ctas), dim3(kJoinThreads), 0, st, p,
+                             "paged_tile_join_cuts_kernel launch");
 }
 
 // Splits of the generic form: about four CTAs an SM, of 64 tokens at least.
@@ -963,13 +1183,12 @@ size_t bd_paged_decode_attn_workspace(const bd_tensor* q, const bd_tensor* k_cac
     AttnParams p{};
     const int rc = check_attn(q, k_cache, v_cache, block_table, context_lens, selected, &p);
     if (rc) return rc;
-    if (use_tiles(p, k_cache, v_cache)) {
-      plan_tiles(&p, tile_warps(p.g.D, p.kv_dtype));
+    if (use_tiles(p, k_cache, v_cache)) {  // unless the output's rows are not aligned
+      plan_tiles(&p);
       n = tile_bytes(p);
-      return BD_OK;
     }
     plan_generic(&p);
-    n = join_bytes(p);
+    n = std::max(n, join_bytes(p));
     return BD_OK;
   });
   return n;
@@ -1002,19 +1221,19 @@ int bd_paged_decode_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_
     p.scale_log2 = scaling * k_scale * kLog2e;
     p.v_scale = v_scale;
     if (p.g.B == 0) return BD_OK;
-    const bool tiles = use_tiles(p, k_cache, v_cache);
-    if (tiles) plan_tiles(&p, tile_warps(p.g.D, p.kv_dtype));
+    const bool tiles = use_tiles(p, k_cache, v_cache) && rows_on(p.out, p.out_dtype, p.o_sb, p.o_sh, p.o_sd, 8);
+    if (tiles) plan_tiles(&p);
     else plan_generic(&p);
     const size_t need = tiles ? tile_bytes(p) : join_bytes(p);
-    if (!workspace || workspace_bytes < need)
+    if (need && (!workspace || workspace_bytes < need))
       return fail(BD_ERR_WORKSPACE, "need " + std::to_string(need) + " workspace bytes");
     const Partials part = tiles ? carve_partials(workspace, size_t(2) * p.warps * p.heads, 1, p.g.D)
                                 : carve_partials(workspace, size_t(p.g.B) * p.Hq, p.n_splits, p.g.D);
     p.part_o = part.o; p.part_m = part.m; p.part_l = part.l;
     if (tiles)
-      return p.g.D == 64    ? launch_tiles<64>(p, k_cache, v_cache, stream)
-             : p.g.D == 128 ? launch_tiles<128>(p, k_cache, v_cache, stream)
-                            : launch_tiles<256>(p, k_cache, v_cache, stream);
+      return with_shape(p, [&](auto d, auto kind, auto nt) {
+        return launch_tiles<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>(p, k_cache, v_cache, stream);
+      });
     if (int64_t(p.g.Hk) * p.chunks > 65535) return fail(BD_ERR_SHAPE, "more than 65535 head chunks");
     paged_attn_generic_kernel<<<dim3(p.n_splits, p.g.Hk * p.chunks, p.g.B), kGenWarps * 32, 0, stream>>>(p);
     if ((rc = cuda_check(cudaGetLastError(), "paged_attn_generic_kernel launch"))) return rc;
