@@ -18,6 +18,11 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// Where a warp's share of the tile kernel's list begins (slots 0: it has none), and the list's length.
+struct __align__(16) ShareStart {
+  int b, hk, chunk, s, slots, total, unused[2];
+};
+
 struct AttnParams {
   PagedGeometry g;
   const void* q; int64_t q_sb, q_sh, q_sd; int q_dtype;
@@ -30,6 +35,7 @@ struct AttnParams {
   // tile form: warps of the grid, its partials [2 * warps][heads]([D])
   int warps, heads, block_shift;
   int row_mode;  // a CTA has a row, and nothing is joined
+  ShareStart* starts;  // one a warp, where paged_tile_join_cuts_kernel follows
   void* out; int out_dtype; int64_t o_sb, o_sh, o_sd;
   float* lse; int64_t e_sb, e_sh;
 };
@@ -153,15 +159,6 @@ constexpr int kUnit = 16;
 
 enum { kBf16 = 0, kF16 = 1, kFp8 = 2 };
 
-#ifndef P_WF
-#define P_WF 16
-#endif
-#ifndef P_WB
-#define P_WB 12
-#endif
-#ifndef P_W64
-#define P_W64 16
-#endif
 template <int D, int KIND, int NT>
 struct TileShape {
   static constexpr int ELT = KIND == kFp8 ? 1 : 2;
@@ -169,7 +166,7 @@ struct TileShape {
   static constexpr int SW = ROWB < 128 ? ROWB : 128;  // bytes of a row in one slab (the swizzle's span)
   static constexpr int SLABS = ROWB / SW;
   static constexpr int HALF = kUnit * ROWB;           // keys (or values) of a unit
-  static constexpr int WARPS = D == 256 ? (KIND == kFp8 ? 8 : 6) : NT == 2 ? 8 : D == 64 ? P_W64 : KIND == kFp8 ? P_WF : P_WB;
+  static constexpr int WARPS = D == 256 ? (KIND == kFp8 ? 8 : 6) : NT == 2 ? 8 : D == 64 || KIND == kFp8 ? 16 : 12;
   static constexpr int FIT = 200 * 1024 / (WARPS * HALF * 2);
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   static_assert(STAGES >= 2, "a unit in flight beside the one at hand");
@@ -186,10 +183,7 @@ __device__ __forceinline__ void prefetch_tensormap(const void* map) {
 }
 
 // A row's place in the list: its slots are kRowCost and its units; 0 without a token.
-#ifndef P_COST
-#define P_COST 1
-#endif
-constexpr int kRowCost = P_COST;
+constexpr int kRowCost = 1;
 
 __device__ __forceinline__ int row_slots(const AttnParams& p, int len) {
   if (len <= 0) return 0;
@@ -254,8 +248,10 @@ struct ListSums {
 // (one sequence of 777 tokens, 28 heads over 4: 12.5, 9.5, 9.2, 9.8 us for 1, 2, 4, 8).
 constexpr int kMinSlots = 4;
 
-// A border inside a row of up to `whole` slots, two shares, moves to the nearer end of the row: so short a
-// row costs less unevenly shared than joined. What cuts a longer row stays where it is.
+// A border inside a row of up to `whole` slots, half a share or 8, moves to the nearer end of the row: so
+// short a row costs less unevenly shared than joined. What cuts a longer row stays where it is (64 sequences
+// of 33 to 8192 tokens: 73.8, 74.7, 82 us for 8, half a share, a share and a half; 148 sequences of 100
+// tokens: 14.9 us against 27 with 4).
 template <int WARPS>
 struct Shares {
   int each, rest, ctas, whole;
@@ -263,7 +259,7 @@ struct Shares {
     ctas = max(1, min(warps / WARPS, total / kMinSlots));
     each = total / ctas;
     rest = total - each * ctas;
-    whole = 2 * each / WARPS;
+    whole = max(8, each / (2 * WARPS));
   }
   __device__ __forceinline__ int cta(int c) const { c = min(c, ctas); return each * c + min(c, rest); }
   __device__ __forceinline__ int begin(int w) const {
@@ -421,11 +417,13 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     const Shares<T::WARPS> sh(list.total, p.warps);
     int first = sh.begin(w), end = sh.begin(w + 1);
     const int cta_first = sh.cta(blockIdx.x), cta_end = sh.cta(blockIdx.x + 1);
+    if (p.starts && first == end && lane == 0) p.starts[w] = ShareStart{0, 0, 0, 0, 0, list.total, {0, 0}};
     if (cta_end == cta_first) return;
     in.find(p, list, groups, cta_first, lane);
     // with all of the CTA's share in one row that is cut its warps' parts are added up here, and one goes out
     one_row = in.s + (cta_end - cta_first) <= in.slots && in.slots > sh.whole;
     row_begins = in.s == 0;
+    int snapped = end;
     if (one_row) {
       in.s += first - cta_first;
     } else {
@@ -433,10 +431,15 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
       if (end < list.total) {
         Place to;
         to.find(p, list, groups, end, lane);
-        end += to.snap(sh.whole);
+        snapped += to.snap(sh.whole);
       }
       if (warp) in.find(p, list, groups, first, lane);
+    }
+    if (p.starts && first < end && lane == 0)
+      p.starts[w] = ShareStart{in.b, in.hk, in.chunk, in.s, in.slots, list.total, {0, 0}};
+    if (!one_row) {
       first += in.snap(sh.whole);
+      end = snapped;
       if (first >= end) return;
       if (in.s == in.slots) in.next_row(p);
     }
@@ -942,57 +945,82 @@ __global__ void __launch_bounds__(kJoinThreads) paged_tile_join_kernel(const Att
   if (some) sum.write(p, b, hk * p.G + chunk * p.heads + h, part);
 }
 
-// The same for many rows, of which few are cut: CTA 2c joins the row that the border before share c of the
-// tile kernel is the first to cut, its warps every eighth part; CTA 2c + 1 those within share c, a warp each
-// (warp w's is the one whose first cut is the beginning of w's share). All heads of a row, PER lanes
-// a head.
+// The same for many rows, of which few are cut: CTA c looks at the borders of share c. The row that the border
+// before it is the first to cut is joined by all warps, a warp a head and every so manieth part; the
+// rows within the share by a warp each (warp w's is the one whose first cut is the beginning of w's
+// share), four heads in flight.
+constexpr int kCutsThreads = 512;
+
 template <int D, int WARPS>
-__global__ void __launch_bounds__(kJoinThreads) paged_tile_join_cuts_kernel(const AttnParams p) {
-  constexpr int PER = D / 4, JW = kJoinThreads / 32, LANES = PER < 32 ? PER : 32, HEADS = 32 / LANES, TURNS = PER / LANES;
+__global__ void __launch_bounds__(kCutsThreads) paged_tile_join_cuts_kernel(const AttnParams p) {
+  constexpr int PER = D / 4, JW = kCutsThreads / 32, TURNS = PER > 32 ? PER / 32 : 1;
+  static_assert(WARPS <= JW, "a warp for every border");
   __shared__ Sum4 red[JW][32];
-  __shared__ GroupSums groups;
-  const int c = blockIdx.x >> 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool within = blockIdx.x & 1;
-  ListSums list;
-  list.build<JW>(p, groups, warp, lane);
-  const Shares<WARPS> sh(list.total, p.warps);
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // sequences without a token
-  for (int b = blockIdx.x; b < p.g.B; b += gridDim.x)
+  for (int b = c * JW + warp; b < p.g.B; b += gridDim.x * JW)
     if (row_slots(p, paged_len(p.g, b)) == 0)
-      for (int i = threadIdx.x; i < p.Hq * PER; i += kJoinThreads) Sum4::none().write(p, b, i / PER, i % PER);
-  const int first_cta = sh.cta(c), end_cta = sh.cta(c + 1);
+      for (int i = lane; i < p.Hq * PER; i += 32) Sum4::none().write(p, b, i / PER, i % PER);
+  griddep_wait();  // also for a kernel that waits for this one: it then finds the tile kernel done as well
+  // warps 1.. the borders within the share, then all of them the one before it
 #pragma unroll 1
-  for (int i = within ? 1 + warp : 0; i < (within ? WARPS : 1); i += JW) {
-    const int w = c * WARPS + i, at_slot = sh.begin(w);
-    Place at;
-    if (at_slot < end_cta) at.find(p, list, groups, at_slot, lane);
-    griddep_wait();
-    if (at_slot >= end_cta) continue;
-    const int s0 = at_slot - at.s, s1 = s0 + at.slots;
-    if (at.slots <= sh.whole) continue;  // not cut at all
-    if (within ? at.s == 0 || s0 < first_cta || s1 > end_cta || sh.begin(w - 1) > s0 || (s0 == first_cta && s1 == end_cta)
-               : at.s == 0 ? s1 != end_cta : sh.cta(c - 1) > s0)
+  for (int border = 0; border < 2; ++border) {
+    const int w = c * WARPS + (border ? 0 : warp);
+    if (!border && (warp == 0 || warp >= WARPS)) continue;
+    const ShareStart at = p.starts[w];
+    if (at.slots == 0) continue;
+    const Shares<WARPS> sh(at.total, p.warps);
+    const int s0 = sh.begin(w) - at.s, s1 = s0 + at.slots, first_cta = sh.cta(c), end_cta = sh.cta(c + 1);
+    if (at.slots <= sh.whole) continue;
+    if (border ? (at.s ? sh.cta(c - 1) > s0 : s1 != end_cta)
+               : at.s == 0 || s0 < first_cta || s1 > end_cta || sh.begin(w - 1) > s0 || s1 - s0 == end_cta - first_cta)
       continue;
     const Parts<WARPS> parts(sh, s0, s1);
     if (parts.n == 0) continue;
     const int nheads = min(p.heads, p.G - at.chunk * p.heads), hq = at.hk * p.G + at.chunk * p.heads;
+    if (!border) {
 #pragma unroll 1
-    for (int k = 0; k < nheads * TURNS; k += HEADS) {
-      const int h = TURNS > 1 ? k / TURNS : k + lane / LANES, part = lane % LANES + (TURNS > 1 ? k % TURNS * LANES : 0);
-      Sum4 sum = Sum4::none();
-      if (h < nheads) add_parts<D>(sum, p, parts, sh, h, part, within ? 0 : warp, within ? 1 : JW);
-      if (!within) {
-        red[warp][lane] = sum;
-        __syncthreads();
-        sum = red[0][lane];
-#pragma unroll 1
-        for (int j = 1; j < JW; ++j) sum.add(red[j][lane].m, red[j][lane].l, red[j][lane].o);
-        __syncthreads();
+      for (int k0 = 0; k0 < nheads * TURNS; k0 += 4) {
+        Sum4 sum[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum[u] = Sum4::none();
+#pragma unroll 4
+        for (int i = 0; i < parts.n; ++i) {
+          const int64_t slot = parts.slot(sh, i) * p.heads;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int k = min(k0 + u, nheads * TURNS - 1);
+            const int64_t from = slot + k / TURNS;
+            sum[u].add(__ldcg(p.part_m + from), __ldcg(p.part_l + from),
+                       __ldcg(reinterpret_cast<const float4*>(p.part_o + from * D) + (k % TURNS * 32 + lane) % PER));
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (k0 + u < nheads * TURNS && lane < PER)
+            sum[u].write(p, at.b, hq + (k0 + u) / TURNS, (k0 + u) % TURNS * 32 + lane);
       }
-      if (h < nheads && (within || warp == 0)) sum.write(p, at.b, hq + h, part);
+      continue;
+    }
+    const int wide = 1 << (32 - __clz(nheads - 1)), slices = JW / wide;  // (nheads 1: __clz(0) is 32)
+    const int h = warp % wide, slice = warp / wide;
+#pragma unroll 1
+    for (int turn = 0; turn < TURNS; ++turn) {
+      Sum4 sum = Sum4::none();
+      if (h < nheads) add_parts<D>(sum, p, parts, sh, h, (turn * 32 + lane) % PER, slice, slices);
+      red[warp][lane] = sum;
+      __syncthreads();
+      if (slice == 0 && h < nheads) {
+#pragma unroll 1
+        for (int j = 1; j < slices; ++j) {
+          const Sum4 x = red[j * wide + h][lane];
+          sum.add(x.m, x.l, x.o);
+        }
+        if (lane < PER) sum.write(p, at.b, hq + h, turn * 32 + lane);
+      }
+      __syncthreads();
     }
   }
-  griddep_wait();
 }
 
 // Whether the tiles can take a call: 16-bit queries and caches of one type, or 8-bit caches; pages of
@@ -1029,9 +1057,6 @@ bool use_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v
 }
 
 // Warps of the grid: the CTAs fill the GPU once, if the block table has work for them.
-#ifndef ROW_UNITS
-#define ROW_UNITS 6
-#endif
 template <typename F>
 auto with_shape(const AttnParams& p, F&& f) {
   auto kind = [&](auto d, auto nt) {
@@ -1056,16 +1081,23 @@ void plan_tiles(AttnParams* p) {
   const int warps = with_shape(*p, [](auto d, auto kind, auto nt) {
     return TileShape<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>::WARPS;
   });
-  // few rows of few tokens (as far as the block table goes): a CTA a row, no join
+  // rows of few tokens (as far as the block table goes), no more of them than SMs: a CTA a row, and no join
   const int64_t rows = int64_t(p->g.B) * p->g.Hk * p->chunks;
-  p->row_mode = rows <= num_sms() && most_slots(*p, p->chunks) <= rows * (ROW_UNITS * warps + kRowCost);
+  const int units = 2 * rows >= num_sms() ? 10 : 2;  // of a warp at most
+  p->row_mode = rows <= num_sms() && most_slots(*p, p->chunks) <= rows * (units * warps + kRowCost);
   p->warps = int(p->row_mode ? rows : ctas) * warps;
   p->block_shift = 31 - __builtin_clz(unsigned(p->g.block));
 }
 
+// Many rows are joined by what cuts them (one CTA a share of the list), few by themselves.
+bool join_by_cuts(const AttnParams& p) {
+  const int most = p.g.D == 256 ? 4 : 8, groups = (std::min(p.heads, p.G) + most - 1) / most;
+  return int64_t(p.g.B) * p.g.Hk * p.chunks * groups > 4 * num_sms();
+}
+
 size_t tile_bytes(const AttnParams& p) {
   if (p.row_mode) return 0;
-  return size_t(2) * p.warps * p.heads * (size_t(p.g.D) + 2) * sizeof(float) + 256;
+  return size_t(2) * p.warps * p.heads * (size_t(p.g.D) + 2) * sizeof(float) + p.warps * sizeof(ShareStart) + 256 + 16;
 }
 
 bool tile_map(CUtensorMap* m, const bd_tensor* t, int sw) {
@@ -1084,9 +1116,6 @@ bool tile_map(CUtensorMap* m, const bd_tensor* t, int sw) {
                     sw == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-#ifndef JOIN_ROWS
-#define JOIN_ROWS 4
-#endif
 template <int D, int KIND, int NT>
 int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v_cache, cudaStream_t st) {
   using T = TileShape<D, KIND, NT>;
@@ -1110,14 +1139,14 @@ int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor*
   constexpr int MANY = D == 256 ? 4 : 8;  // heads that 256 threads hold at 4 channels each, 8 at most
   const int64_t rows = int64_t(p.g.B) * p.g.Hk * p.chunks;
   const int heads = std::min(p.heads, p.G), groups = (heads + MANY - 1) / MANY;
+  if (p.starts)
+    return launch_programmatic(paged_tile_join_cuts_kernel<D, T::WARPS>, dim3(ctas), dim3(kCutsThreads), 0, st, p,
+                               "paged_tile_join_cuts_kernel launch");
   if (rows * heads <= 4 * num_sms())
     return launch_programmatic(paged_tile_join_kernel<D, T::WARPS, 1>, dim3(p.g.Hk * p.chunks * heads, p.g.B),
                                dim3(kJoinThreads), 0, st, p, "paged_tile_join_kernel launch");
-  if (rows * groups <= JOIN_ROWS * num_sms())
-    return launch_programmatic(paged_tile_join_kernel<D, T::WARPS, MANY>, dim3(p.g.Hk * p.chunks * groups, p.g.B),
-                               dim3(kJoinThreads), 0, st, p, "paged_tile_join_kernel launch");
-  return launch_programmatic(paged_tile_join_cuts_kernel<D, T::WARPS>, dim3(2 * ctas), dim3(kJoinThreads), 0, st, p,
-                             "paged_tile_join_cuts_kernel launch");
+  return launch_programmatic(paged_tile_join_kernel<D, T::WARPS, MANY>, dim3(p.g.Hk * p.chunks * groups, p.g.B),
+                             dim3(kJoinThreads), 0, st, p, "paged_tile_join_kernel launch");
 }
 
 // Splits of the generic form: about four CTAs an SM, of 64 tokens at least.
@@ -1230,6 +1259,9 @@ int bd_paged_decode_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_
     const Partials part = tiles ? carve_partials(workspace, size_t(2) * p.warps * p.heads, 1, p.g.D)
                                 : carve_partials(workspace, size_t(p.g.B) * p.Hq, p.n_splits, p.g.D);
     p.part_o = part.o; p.part_m = part.m; p.part_l = part.l;
+    if (tiles && !p.row_mode && join_by_cuts(p))
+      p.starts = reinterpret_cast<ShareStart*>((reinterpret_cast<uintptr_t>(part.l + size_t(2) * p.warps * p.heads) + 15) &
+                                               ~uintptr_t(15));
     if (tiles)
       return with_shape(p, [&](auto d, auto kind, auto nt) {
         return launch_tiles<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>(p, k_cache, v_cache, stream);
