@@ -35,6 +35,7 @@ struct AttnParams {
   // tile form: warps of the grid, its partials [2 * warps][heads]([D])
   int warps, heads, block_shift;
   int row_mode;  // a CTA has a row, and nothing is joined
+  int after_select;  // launched as a programmatic dependent of the choice of pages, which it waits for
   ShareStart* starts;  // one a warp, where paged_tile_join_cuts_kernel follows
   void* out; int out_dtype; int64_t o_sb, o_sh, o_sd;
   float* lse; int64_t e_sb, e_sh;
@@ -468,6 +469,7 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     }
   };
   to_unit();
+  if (p.after_select) griddep_wait();
 
   auto issue = [&](int stage) {
     if (to_issue == 0) return;
@@ -1132,8 +1134,13 @@ int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor*
       return rc;
     set[dev & 63] = true;
   }
-  kern<<<p.warps / T::WARPS, T::WARPS * 32, T::SMEM, st>>>(p, km, vm);
-  if ((rc = cuda_check(cudaGetLastError(), "paged_attn_tile_kernel launch"))) return rc;
+  const dim3 grid(p.warps / T::WARPS), block(T::WARPS * 32);
+  if (p.after_select) {
+    if ((rc = launch_pdl(kern, grid, block, T::SMEM, st, "paged_attn_tile_kernel launch", p, km, vm))) return rc;
+  } else {
+    kern<<<grid, block, T::SMEM, st>>>(p, km, vm);
+    if ((rc = cuda_check(cudaGetLastError(), "paged_attn_tile_kernel launch"))) return rc;
+  }
   if (p.row_mode) return BD_OK;
   const int ctas = p.warps / T::WARPS;
   constexpr int MANY = D == 256 ? 4 : 8;  // heads that 256 threads hold at 4 channels each, 8 at most
@@ -1191,6 +1198,78 @@ int check_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_
   return BD_OK;
 }
 
+int check_out(const bd_tensor* q, const bd_tensor* k_cache, float k_scale, float v_scale, const bd_tensor* out,
+              const bd_tensor* lse, AttnParams* pp) {
+  AttnParams& p = *pp;
+  int rc;
+  if ((rc = check_tensor(out, "out", 3))) return rc;
+  if (!is_float16_32(out->dtype)) return fail(BD_ERR_DTYPE, "out must be bf16, f16 or f32");
+  for (int i = 0; i < 3; ++i)
+    if (out->shape[i] != q->shape[i]) return fail(BD_ERR_SHAPE, "out shape must equal q shape");
+  if (lse) {
+    if ((rc = check_tensor(lse, "lse", 2, BD_F32))) return rc;
+    if (lse->shape[0] != q->shape[0] || lse->shape[1] != q->shape[1])
+      return fail(BD_ERR_SHAPE, "lse must be [B, Hq]");
+    p.lse = static_cast<float*>(lse->data); p.e_sb = lse->stride[0]; p.e_sh = lse->stride[1];
+  }
+  if (!(k_scale > 0.f) || !(v_scale > 0.f)) return fail(BD_ERR_VALUE, "k_scale and v_scale must be positive");
+  if (k_cache->dtype != BD_F8E4M3 && (k_scale != 1.f || v_scale != 1.f))
+    return fail(BD_ERR_VALUE, "k_scale and v_scale belong to an fp8 cache");
+  p.out = out->data; p.out_dtype = out->dtype;
+  p.o_sb = out->stride[0]; p.o_sh = out->stride[1]; p.o_sd = out->stride[2];
+  return BD_OK;
+}
+
+// The whole call; after_select: `selected` is written by the kernel launched just before, which was itself
+// launched in stream order (so all that came before it is done).
+int run_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_cache, const bd_tensor* block_table,
+             const bd_tensor* context_lens, const bd_tensor* selected, bool after_select, float scaling, float k_scale,
+             float v_scale, const bd_tensor* out, const bd_tensor* lse, void* workspace, size_t workspace_bytes,
+             cudaStream_t stream) {
+  int rc;
+  AttnParams p{};
+  if ((rc = check_attn(q, k_cache, v_cache, block_table, context_lens, selected, &p))) return rc;
+  p.after_select = after_select;
+  if ((rc = check_out(q, k_cache, k_scale, v_scale, out, lse, &p))) return rc;
+  p.scale_log2 = scaling * k_scale * kLog2e;
+  p.v_scale = v_scale;
+  if (p.g.B == 0) return BD_OK;
+  const bool tiles = use_tiles(p, k_cache, v_cache) && rows_on(p.out, p.out_dtype, p.o_sb, p.o_sh, p.o_sd, 8);
+  if (tiles) plan_tiles(&p);
+  else plan_generic(&p);
+  const size_t need = tiles ? tile_bytes(p) : join_bytes(p);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(BD_ERR_WORKSPACE, "need " + std::to_string(need) + " workspace bytes");
+  const Partials part = tiles ? carve_partials(workspace, size_t(2) * p.warps * p.heads, 1, p.g.D)
+                              : carve_partials(workspace, size_t(p.g.B) * p.Hq, p.n_splits, p.g.D);
+  p.part_o = part.o; p.part_m = part.m; p.part_l = part.l;
+  if (tiles && !p.row_mode && join_by_cuts(p))
+    p.starts = reinterpret_cast<ShareStart*>((reinterpret_cast<uintptr_t>(part.l + size_t(2) * p.warps * p.heads) + 15) &
+                                             ~uintptr_t(15));
+  if (tiles)
+    return with_shape(p, [&](auto d, auto kind, auto nt) {
+      return launch_tiles<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>(p, k_cache, v_cache, stream);
+    });
+  if (int64_t(p.g.Hk) * p.chunks > 65535) return fail(BD_ERR_SHAPE, "more than 65535 head chunks");
+  paged_attn_generic_kernel<<<dim3(p.n_splits, p.g.Hk * p.chunks, p.g.B), kGenWarps * 32, 0, stream>>>(p);
+  if ((rc = cuda_check(cudaGetLastError(), "paged_attn_generic_kernel launch"))) return rc;
+  paged_join_kernel<<<dim3(p.Hq, p.g.B), 128, 0, stream>>>(p);
+  return cuda_check(cudaGetLastError(), "paged_join_kernel launch");
+}
+
+size_t attn_bytes(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_cache, const bd_tensor* block_table,
+                  const bd_tensor* context_lens, const bd_tensor* selected) {
+  AttnParams p{};
+  if (check_attn(q, k_cache, v_cache, block_table, context_lens, selected, &p)) return 0;
+  size_t n = 0;
+  if (use_tiles(p, k_cache, v_cache)) {  // unless the output's rows are not aligned
+    plan_tiles(&p);
+    n = tile_bytes(p);
+  }
+  plan_generic(&p);
+  return std::max(n, join_bytes(p));
+}
+
 }  // namespace
 
 // host read of this file's wait-timeout counter (-1 on failure)
@@ -1209,15 +1288,7 @@ size_t bd_paged_decode_attn_workspace(const bd_tensor* q, const bd_tensor* k_cac
   using namespace bd;
   size_t n = 0;
   guarded([&]() -> int {
-    AttnParams p{};
-    const int rc = check_attn(q, k_cache, v_cache, block_table, context_lens, selected, &p);
-    if (rc) return rc;
-    if (use_tiles(p, k_cache, v_cache)) {  // unless the output's rows are not aligned
-      plan_tiles(&p);
-      n = tile_bytes(p);
-    }
-    plan_generic(&p);
-    n = std::max(n, join_bytes(p));
+    n = attn_bytes(q, k_cache, v_cache, block_table, context_lens, selected);
     return BD_OK;
   });
   return n;
@@ -1229,48 +1300,45 @@ int bd_paged_decode_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_
                          void* workspace, size_t workspace_bytes, bd_stream_t stream) {
   using namespace bd;
   return guarded([&]() -> int {
+    return run_attn(q, k_cache, v_cache, block_table, context_lens, selected, false, scaling, k_scale, v_scale, out, lse,
+                    workspace, workspace_bytes, stream);
+  });
+}
+
+size_t bd_paged_sparse_decode_attn_workspace(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_cache,
+                                             const bd_tensor* summary, const bd_tensor* block_table,
+                                             const bd_tensor* context_lens, const bd_tensor* selected) {
+  using namespace bd;
+  size_t n = 0;
+  guarded([&]() -> int {
+    n = bd_paged_select_workspace(q, summary, block_table) +
+        attn_bytes(q, k_cache, v_cache, block_table, context_lens, selected);
+    return BD_OK;
+  });
+  return n;
+}
+
+int bd_paged_sparse_decode_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_cache,
+                                const bd_tensor* summary, const bd_tensor* summary_scale, const bd_tensor* block_table,
+                                const bd_tensor* context_lens, int sink, int recent, float scaling, float k_scale,
+                                float v_scale, const bd_tensor* selected, const bd_tensor* out, const bd_tensor* lse,
+                                void* workspace, size_t workspace_bytes, bd_stream_t stream) {
+  using namespace bd;
+  return guarded([&]() -> int {
     int rc;
-    AttnParams p{};
-    if ((rc = check_attn(q, k_cache, v_cache, block_table, context_lens, selected, &p))) return rc;
-    if ((rc = check_tensor(out, "out", 3))) return rc;
-    if (!is_float16_32(out->dtype)) return fail(BD_ERR_DTYPE, "out must be bf16, f16 or f32");
-    for (int i = 0; i < 3; ++i)
-      if (out->shape[i] != q->shape[i]) return fail(BD_ERR_SHAPE, "out shape must equal q shape");
-    if (lse) {
-      if ((rc = check_tensor(lse, "lse", 2, BD_F32))) return rc;
-      if (lse->shape[0] != q->shape[0] || lse->shape[1] != q->shape[1])
-        return fail(BD_ERR_SHAPE, "lse must be [B, Hq]");
-      p.lse = static_cast<float*>(lse->data); p.e_sb = lse->stride[0]; p.e_sh = lse->stride[1];
-    }
-    if (!(k_scale > 0.f) || !(v_scale > 0.f)) return fail(BD_ERR_VALUE, "k_scale and v_scale must be positive");
-    if (k_cache->dtype != BD_F8E4M3 && (k_scale != 1.f || v_scale != 1.f))
-      return fail(BD_ERR_VALUE, "k_scale and v_scale belong to an fp8 cache");
-    p.out = out->data; p.out_dtype = out->dtype;
-    p.o_sb = out->stride[0]; p.o_sh = out->stride[1]; p.o_sd = out->stride[2];
-    p.scale_log2 = scaling * k_scale * kLog2e;
-    p.v_scale = v_scale;
-    if (p.g.B == 0) return BD_OK;
-    const bool tiles = use_tiles(p, k_cache, v_cache) && rows_on(p.out, p.out_dtype, p.o_sb, p.o_sh, p.o_sd, 8);
-    if (tiles) plan_tiles(&p);
-    else plan_generic(&p);
-    const size_t need = tiles ? tile_bytes(p) : join_bytes(p);
-    if (need && (!workspace || workspace_bytes < need))
-      return fail(BD_ERR_WORKSPACE, "need " + std::to_string(need) + " workspace bytes");
-    const Partials part = tiles ? carve_partials(workspace, size_t(2) * p.warps * p.heads, 1, p.g.D)
-                                : carve_partials(workspace, size_t(p.g.B) * p.Hq, p.n_splits, p.g.D);
-    p.part_o = part.o; p.part_m = part.m; p.part_l = part.l;
-    if (tiles && !p.row_mode && join_by_cuts(p))
-      p.starts = reinterpret_cast<ShareStart*>((reinterpret_cast<uintptr_t>(part.l + size_t(2) * p.warps * p.heads) + 15) &
-                                               ~uintptr_t(15));
-    if (tiles)
-      return with_shape(p, [&](auto d, auto kind, auto nt) {
-        return launch_tiles<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>(p, k_cache, v_cache, stream);
-      });
-    if (int64_t(p.g.Hk) * p.chunks > 65535) return fail(BD_ERR_SHAPE, "more than 65535 head chunks");
-    paged_attn_generic_kernel<<<dim3(p.n_splits, p.g.Hk * p.chunks, p.g.B), kGenWarps * 32, 0, stream>>>(p);
-    if ((rc = cuda_check(cudaGetLastError(), "paged_attn_generic_kernel launch"))) return rc;
-    paged_join_kernel<<<dim3(p.Hq, p.g.B), 128, 0, stream>>>(p);
-    return cuda_check(cudaGetLastError(), "paged_join_kernel launch");
+    AttnParams p{};  // what the second half refuses is refused before the first is launched
+    if (!selected) return fail(BD_ERR_NULL, "selected descriptor is NULL");
+    if ((rc = check_attn(q, k_cache, v_cache, block_table, context_lens, selected, &p)) ||
+        (rc = check_out(q, k_cache, k_scale, v_scale, out, lse, &p)))
+      return rc;
+    const size_t first = bd_paged_select_workspace(q, summary, block_table);
+    if (!workspace || workspace_bytes < first + attn_bytes(q, k_cache, v_cache, block_table, context_lens, selected))
+      return fail(BD_ERR_WORKSPACE, "workspace is smaller than bd_paged_sparse_decode_attn_workspace");
+    if ((rc = bd_paged_select(q, summary, summary_scale, block_table, context_lens, p.g.block, sink, recent, selected,
+                              workspace, first, stream)))
+      return rc;
+    return run_attn(q, k_cache, v_cache, block_table, context_lens, selected, p.g.B > 0 && p.n_sel > 0, scaling, k_scale,
+                    v_scale, out, lse, static_cast<uint8_t*>(workspace) + first, workspace_bytes - first, stream);
   });
 }
 

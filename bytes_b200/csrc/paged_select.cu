@@ -34,37 +34,30 @@ __device__ __forceinline__ unsigned score_key(float x) {
   return max(2u, min(0xfffffffeu, u & 0x80000000u ? ~u : u | 0x80000000u));
 }
 
-// Rows with no more pages than the budget take them all: their scores are not needed.
-__device__ __forceinline__ int row_pages(const SelectParams& p, int b) {
-  return int((int64_t(paged_len(p.g, b)) + p.g.block - 1) / p.g.block);
-}
-
 // One query row's 8-bit numbers (a warp together): n of them as [negative part | positive part] at
 // q8, s_q returned.
 __device__ __forceinline__ float quantize_query(const SelectParams& p, int b, int hq, int8_t* q8, int lane) {
   const int64_t base = b * p.q_sb + hq * p.q_sh;
-  float top = 0.f;
-  for (int d = lane; d < p.g.D; d += 32) top = fmaxf(top, fabsf(load_as(p.q, p.q_dtype, base + d * p.q_sd)));
+  float x[8], top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = lane + 32 * i;
+    x[i] = d < p.g.D ? load_as(p.q, p.q_dtype, base + d * p.q_sd) : 0.f;
+    top = fmaxf(top, fabsf(x[i]));
+  }
   top = warp_max(top);
   const float mul = __fdiv_rn(127.f, top);
-  for (int d = lane; d < p.g.D; d += 32) {
-    int x = top > 0.f ? __float2int_rn(__fmul_rn(load_as(p.q, p.q_dtype, base + d * p.q_sd), mul)) : 0;
-    x = max(-127, min(127, x));
-    q8[d] = int8_t(min(x, 0));
-    q8[p.g.D + d] = int8_t(max(x, 0));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = lane + 32 * i;
+    if (d >= p.g.D) continue;
+    int y = top > 0.f ? __float2int_rn(__fmul_rn(x[i], mul)) : 0;
+    y = max(-127, min(127, y));
+    q8[d] = int8_t(min(y, 0));
+    q8[p.g.D + d] = int8_t(max(y, 0));
   }
   return __fdiv_rn(top, 127.f);
 }
-
-// ---------------------------------------------------------------------------------- scores
-// On the integer tensor cores: a page's summary is one row [min8 | max8] of 2D numbers, a head's query
-// one column [q8 below 0 | q8 above 0], and I their product (mma.sync m16n8k32, 16 pages by 8 heads).
-// The order of the 2D numbers is free, so that a thread's operand registers are 16 contiguous bytes
-// of a row, loaded from global memory as such: no shared memory but for the queries.
-constexpr int kScoreWarps = 8;
-constexpr int kScoreTiles = 2;                                 // 16-page tiles a warp has in flight
-constexpr int kScorePages = kScoreWarps * kScoreTiles * 16;    // pages of a CTA's step
-constexpr int kScoreSteps = 2;
 
 __device__ __forceinline__ void mma_s8(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
@@ -74,140 +67,125 @@ __device__ __forceinline__ void mma_s8(int* d, uint32_t a0, uint32_t a1, uint32_
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// One kernel for scores and choice: a cluster of CTAs has a row (one KV head of a sequence). Its warps score
+// the row's pages, 16 at a time, into `keys` (global memory, which L2 holds); then the cluster's first CTA
+// finds the threshold and writes the pages above it in order.
+//
+// Scores are taken on the integer tensor cores: a page's summary is one row [min8 | max8] of 2D numbers, a
+// head's query one column [q8 below 0 | q8 above 0], and I their product (mma.sync m16n8k32, 16 pages by 8
+// heads). The order of the 2D numbers is free, so that a thread's operand registers are 16 contiguous
+// bytes of a row, loaded from global memory as such: no shared memory but for the queries.
+//
+// D = 0: any head dim, any alignment of the summaries, a lane a page.
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+
 template <int D>
-__global__ void __launch_bounds__(kScoreWarps * 32) paged_score_kernel(const SelectParams p) {
-  extern __shared__ __align__(16) int8_t q8[];  // [heads, a multiple of 8][2D], then their scales
-  griddep_launch_dependents();
-  const int hk = blockIdx.x, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, tq = lane & 3;
-  const int n = row_pages(p, b);
-  const int j_first = blockIdx.y * kScorePages * kScoreSteps;
-  if (n <= p.budget || j_first >= n) return;
+__device__ __forceinline__ void score_pages(const SelectParams& p, int b, int hk, int n, unsigned* keys, int8_t* q8,
+                                            int rank, int ctas, int warp, int lane) {
   const int heads = (p.G + 7) & ~7;
   float* q_scale = reinterpret_cast<float*>(q8 + heads * 2 * D);
-  for (int h = warp; h < heads; h += kScoreWarps) {
+  const int g = lane >> 2, tq = lane & 3, step = ctas * kSelWarps * 16;
+  int j0 = (rank * kSelWarps + warp) * 16;
+  // rows g and g + 8 of the tile; the first tile's loads are under way while the queries are made
+  int page[2];
+  uint4 a[2][D / 32];
+  float scale[2];
+  auto load_page = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) page[i] = at + i * 8 + g < n ? paged_block(p.g, b, at + i * 8 + g) : -1;
+  };
+  auto load_rows = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t at = max(page[i], 0);
+      const uint4* row = reinterpret_cast<const uint4*>(p.code + at * p.c_sb + hk * p.c_sh) + tq;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) a[i][c] = page[i] >= 0 ? __ldg(row + c * 4) : make_uint4(0, 0, 0, 0);
+      scale[i] = page[i] >= 0 ? __ldg(p.scale + at * p.s_sb + hk * p.s_sh) : 0.f;
+    }
+  };
+  load_page(j0);
+  load_rows();
+  for (int h = warp; h < heads; h += kSelWarps) {
     if (h < p.G) {
       const float s = quantize_query(p, b, hk * p.G + h, q8 + h * 2 * D, lane);
       if (lane == 0) q_scale[h] = s;
-    } else {  // heads that fill the last eight up: their score is below every other
+    } else {  // columns that fill the last eight up are not looked at
       for (int d = lane; d < 2 * D; d += 32) q8[h * 2 * D + d] = 0;
-      if (lane == 0) q_scale[h] = 0.f;
     }
   }
   __syncthreads();
-  unsigned* keys = p.keys + (int64_t(b) * p.g.Hk + hk) * p.pitch;
-  for (int step = 0; step < kScoreSteps; ++step) {
-    const int j0 = j_first + step * kScorePages + warp * kScoreTiles * 16;
-    if (j0 >= n) return;
-    // rows g and g + 8 of each tile
-    int page[kScoreTiles][2];
-    uint4 a[kScoreTiles][2][D / 32];
-#pragma unroll
-    for (int t = 0; t < kScoreTiles; ++t)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int j = j0 + t * 16 + i * 8 + g;
-        page[t][i] = j < n ? paged_block(p.g, b, j) : -1;
-      }
-    float scale[kScoreTiles][2];
-#pragma unroll
-    for (int t = 0; t < kScoreTiles; ++t)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int64_t at = max(page[t][i], 0);
-        const uint4* row = reinterpret_cast<const uint4*>(p.code + at * p.c_sb + hk * p.c_sh);
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c)
-          a[t][i][c] = page[t][i] >= 0 ? __ldg(row + c * 4 + tq) : make_uint4(0, 0, 0, 0);
-        scale[t][i] = page[t][i] >= 0 ? __ldg(p.scale + at * p.s_sb + hk * p.s_sh) : 0.f;
-      }
-    float best[kScoreTiles][2];
-#pragma unroll
-    for (int t = 0; t < kScoreTiles; ++t) best[t][0] = best[t][1] = -INFINITY;
+#pragma unroll 1
+  for (; j0 < n; j0 += step) {
+    float best[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
     for (int h0 = 0; h0 < p.G; h0 += 8) {
-      int acc[kScoreTiles][4];
-#pragma unroll
-      for (int t = 0; t < kScoreTiles; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0;
+      int acc[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         const uint4 w = *reinterpret_cast<const uint4*>(q8 + (h0 + g) * 2 * D + c * 64 + tq * 16);
-#pragma unroll
-        for (int t = 0; t < kScoreTiles; ++t) {
-          mma_s8(acc[t], a[t][0][c].x, a[t][1][c].x, a[t][0][c].y, a[t][1][c].y, w.x, w.y);
-          mma_s8(acc[t], a[t][0][c].z, a[t][1][c].z, a[t][0][c].w, a[t][1][c].w, w.z, w.w);
-        }
+        mma_s8(acc, a[0][c].x, a[1][c].x, a[0][c].y, a[1][c].y, w.x, w.y);
+        mma_s8(acc, a[0][c].z, a[1][c].z, a[0][c].w, a[1][c].w, w.z, w.w);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {  // heads 2tq, 2tq + 1
         const int h = h0 + 2 * tq + i;
         if (h >= p.G) continue;
-        const float s = q_scale[h];
-#pragma unroll
-        for (int t = 0; t < kScoreTiles; ++t) {
-          best[t][0] = fmaxf(best[t][0], __fmul_rn(float(acc[t][i]), s));
-          best[t][1] = fmaxf(best[t][1], __fmul_rn(float(acc[t][2 + i]), s));
-        }
+        best[0] = fmaxf(best[0], __fmul_rn(float(acc[i]), q_scale[h]));
+        best[1] = fmaxf(best[1], __fmul_rn(float(acc[2 + i]), q_scale[h]));
       }
     }
+    unsigned key[2];
 #pragma unroll
-    for (int t = 0; t < kScoreTiles; ++t)
+    for (int i = 0; i < 2; ++i) {
+      float x = best[i];
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      const int j = j0 + i * 8 + g;
+      key[i] = j < p.sink || j >= n - p.recent ? 0xffffffffu : page[i] < 0 ? 1u : score_key(__fmul_rn(x, scale[i]));
+    }
+    if (j0 + step < n) {
+      load_page(j0 + step);
+      load_rows();
+    }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float x = best[t][i];
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        const int j = j0 + t * 16 + i * 8 + g;
-        if (tq == 0 && j < n)
-          keys[j] = j < p.sink || j >= n - p.recent ? 0xffffffffu
-                    : page[t][i] < 0                ? 1u
-                                                    : score_key(__fmul_rn(x, scale[t][i]));
-      }
+    for (int i = 0; i < 2; ++i)
+      if (tq == 0 && j0 + i * 8 + g < n) __stcg(keys + j0 + i * 8 + g, key[i]);
   }
 }
 
-// Head dims that are no multiple of 32, and summaries whose rows are not 16-byte aligned: a thread a page.
-__global__ void __launch_bounds__(256) paged_score_generic_kernel(const SelectParams p) {
-  extern __shared__ __align__(16) int8_t q8[];
-  griddep_launch_dependents();
-  const int hk = blockIdx.x, b = blockIdx.z, D = p.g.D, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = row_pages(p, b);
-  const int j = blockIdx.y * 256 + threadIdx.x;
-  if (n <= p.budget || j - int(threadIdx.x) >= n) return;
+template <>
+__device__ __forceinline__ void score_pages<0>(const SelectParams& p, int b, int hk, int n, unsigned* keys, int8_t* q8,
+                                               int rank, int ctas, int warp, int lane) {
+  const int D = p.g.D;
   float* q_scale = reinterpret_cast<float*>(q8 + ((p.G + 7) & ~7) * 2 * D);
-  for (int h = warp; h < p.G; h += 8) {
+  for (int h = warp; h < p.G; h += kSelWarps) {
     const float s = quantize_query(p, b, hk * p.G + h, q8 + h * 2 * D, lane);
     if (lane == 0) q_scale[h] = s;
   }
   __syncthreads();
-  if (j >= n) return;
-  unsigned key = 0xffffffffu;
-  if (j >= p.sink && j < n - p.recent) {
-    const int page = paged_block(p.g, b, j);
-    key = 1;
-    if (page >= 0) {
-      const int8_t* row = p.code + page * p.c_sb + hk * p.c_sh;
-      float best = -INFINITY;
-      for (int h = 0; h < p.G; ++h) {
-        int sum = 0;
-        for (int d = 0; d < 2 * D; ++d) sum += int(q8[h * 2 * D + d]) * row[d];
-        best = fmaxf(best, __fmul_rn(float(sum), q_scale[h]));
+  for (int j = rank * kSelThreads + warp * 32 + lane; j < n; j += ctas * kSelThreads) {
+    unsigned key = 0xffffffffu;
+    if (j >= p.sink && j < n - p.recent) {
+      const int page = paged_block(p.g, b, j);
+      key = 1;
+      if (page >= 0) {
+        const int8_t* row = p.code + page * p.c_sb + hk * p.c_sh;
+        float best = -INFINITY;
+        for (int h = 0; h < p.G; ++h) {
+          int sum = 0;
+          for (int d = 0; d < 2 * D; ++d) sum += int(q8[h * 2 * D + d]) * row[d];
+          best = fmaxf(best, __fmul_rn(float(sum), q_scale[h]));
+        }
+        key = score_key(__fmul_rn(best, p.scale[page * p.s_sb + hk * p.s_sh]));
       }
-      key = score_key(__fmul_rn(best, p.scale[page * p.s_sb + hk * p.s_sh]));
     }
+    __stcg(keys + j, key);
   }
-  p.keys[(int64_t(b) * p.g.Hk + hk) * p.pitch + j] = key;
 }
 
-// ---------------------------------------------------------------------------------- choice
-// One CTA a row. Thread t holds keys [t KPT, (t + 1) KPT) in registers (pages past 512 KPT are read
-// again from L2 each time); the threshold, the largest that `want` keys reach, is found two bits at
-// a time by counting the keys that reach each of three candidates (no histogram: scores share their
-// leading bits, and its counters would all be the same few); then a scan gives every taken page
-// its place, in order.
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
-
-// Sums over the CTA of three counts, each below 2^20 for the block.
+// Sums over the CTA of three counts.
 struct Count3 { int a, b, c; };
 __device__ __forceinline__ Count3 block_sum3(Count3 x, Count3* buf) {
   x.a = __reduce_add_sync(0xffffffffu, x.a);
@@ -216,49 +194,73 @@ __device__ __forceinline__ Count3 block_sum3(Count3 x, Count3* buf) {
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = x;
   __syncthreads();
   const int lane = threadIdx.x & 31;
-  Count3 y = lane < kSelWarps ? buf[lane] : Count3{0, 0, 0};
-  y.a = __reduce_add_sync(0xffffffffu, y.a);
-  y.b = __reduce_add_sync(0xffffffffu, y.b);
-  y.c = __reduce_add_sync(0xffffffffu, y.c);
-  return y;
+  const Count3 y = lane < kSelWarps ? buf[lane] : Count3{0, 0, 0};
+  return Count3{int(__reduce_add_sync(0xffffffffu, y.a)), int(__reduce_add_sync(0xffffffffu, y.b)),
+                int(__reduce_add_sync(0xffffffffu, y.c))};
 }
 
-template <int KPT>
-__global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(const SelectParams p) {
+// The largest threshold that `want` of a row's n keys reach, then the pages: those above it, and the lowest of
+// those at it. Thread t holds keys 4 (i 512 + t) .. + 3, i < 4, in registers (pages past 8192 are read again
+// from L2 each time). The threshold is found two bits at a time, from the first bit in which the keys differ,
+// by counting the keys that reach each of three candidates (no histogram: scores share their leading bits,
+// and its counters would all be the same few); once at most 512 keys are left between the bounds, each
+// thread goes on with one of them.
+__device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int want, int* out, int64_t o_si) {
+  constexpr int GROUPS = 4, kHeld = GROUPS * 4 * kSelThreads;
   __shared__ Count3 buf[2][kSelWarps];
-  const int hk = blockIdx.x, b = blockIdx.y, t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int n = row_pages(p, b), want = min(n, p.budget);
-  int* out = p.selected + b * p.o_sb + hk * p.o_sh;
-  for (int i = want + t; i < p.budget; i += kSelThreads) out[i * p.o_si] = -1;
-  if (n <= p.budget) {
-    for (int i = t; i < n; i += kSelThreads) out[i * p.o_si] = i;
-    griddep_wait();
-    return;
-  }
-  griddep_wait();
-  const unsigned* keys = p.keys + (int64_t(b) * p.g.Hk + hk) * p.pitch;
-  unsigned key[KPT];
+  __shared__ unsigned left[kSelThreads];
+  __shared__ int n_left;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int groups = min(GROUPS, (n + 4 * kSelThreads - 1) / (4 * kSelThreads));
+  unsigned key[GROUPS][4];
+  unsigned lo = 0xffffffffu, hi = 0;
 #pragma unroll
-  for (int i = 0; i < KPT; i += 4) {
-    const int j = t * KPT + i;
+  for (int i = 0; i < GROUPS; ++i) {
+    const int j = 4 * (i * kSelThreads + t);
     // rows are padded to four keys; what lies past n is not a key
     const uint4 x = j < n ? __ldcg(reinterpret_cast<const uint4*>(keys + j)) : make_uint4(0, 0, 0, 0);
-    key[i] = x.x;
-    key[i + 1] = j + 1 < n ? x.y : 0;
-    key[i + 2] = j + 2 < n ? x.z : 0;
-    key[i + 3] = j + 3 < n ? x.w : 0;
+    key[i][0] = x.x;
+    key[i][1] = j + 1 < n ? x.y : 0;
+    key[i][2] = j + 2 < n ? x.z : 0;
+    key[i][3] = j + 3 < n ? x.w : 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      hi = max(hi, key[i][e]);
+      if (key[i][e]) lo = min(lo, key[i][e]);
+    }
   }
-  constexpr int kHeld = kSelThreads * KPT;
-  unsigned thr = 0;
-  for (int bit = 30; bit >= 0; bit -= 2) {
+  for (int j = kHeld + t; j < n; j += kSelThreads) {
+    const unsigned k = __ldcg(keys + j);
+    hi = max(hi, k);
+    lo = min(lo, k);
+  }
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  if (lane == 0) buf[1][warp] = Count3{int(hi), int(lo), 0};
+  if (t == 0) n_left = 0;
+  __syncthreads();
+  {
+    const Count3 y = buf[1][lane % kSelWarps];
+    hi = __reduce_max_sync(0xffffffffu, unsigned(y.a));
+    lo = __reduce_min_sync(0xffffffffu, unsigned(y.b));
+  }
+  __syncthreads();
+  // all keys share the bits above `bit`
+  int bit = hi == lo ? -2 : (31 - __clz(hi ^ lo)) & ~1;
+  unsigned thr = hi == lo ? hi : bit >= 30 ? 0u : hi & ~((4u << bit) - 1u);
+  int reach = n, above = 0;  // keys that reach thr, and that are above what thr may still become
+  for (; bit >= 0 && reach - above > kSelThreads; bit -= 2) {
     const unsigned c1 = thr | (1u << bit), c2 = thr | (2u << bit), c3 = thr | (3u << bit);
     Count3 c{0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-      c.a += key[i] >= c1;
-      c.b += key[i] >= c2;
-      c.c += key[i] >= c3;
-    }
+    for (int i = 0; i < GROUPS; ++i)
+      if (i < groups)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          c.a += key[i][e] >= c1;
+          c.b += key[i][e] >= c2;
+          c.c += key[i][e] >= c3;
+        }
     for (int j = kHeld + t; j < n; j += kSelThreads) {
       const unsigned k = __ldcg(keys + j);
       c.a += k >= c1;
@@ -266,59 +268,110 @@ __global__ void __launch_bounds__(kSelThreads) paged_choose_kernel(const SelectP
       c.c += k >= c3;
     }
     c = block_sum3(c, buf[(bit >> 1) & 1]);
-    if (c.c >= want) thr = c3;
-    else if (c.b >= want) thr = c2;
-    else if (c.a >= want) thr = c1;
+    if (c.c >= want) thr = c3, reach = c.c;
+    else if (c.b >= want) thr = c2, reach = c.b, above = c.c;
+    else if (c.a >= want) thr = c1, reach = c.a, above = c.b;
+    else above = c.a;
   }
-  // above the threshold, and at it, before this thread's keys and in all
-  Count3 mine{0, 0, 0};
+  if (bit >= 0) {
+    // the keys between thr and the next value that it cannot be
+    const unsigned span = bit >= 30 ? 0xffffffffu : (4u << bit) - 1u;
+    auto keep = [&](unsigned k) {
+      if (k >= thr && k - thr <= span) left[atomicAdd(&n_left, 1)] = k;
+    };
 #pragma unroll
-  for (int i = 0; i < KPT; ++i) {
-    mine.a += key[i] > thr;
-    mine.b += key[i] == thr;
-  }
-  Count3 sum = mine;  // inclusive over the warp
+    for (int i = 0; i < GROUPS; ++i)
+      if (i < groups)
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, sum.a, o), y = __shfl_up_sync(0xffffffffu, sum.b, o);
-    if (lane >= o) sum.a += x, sum.b += y;
-  }
-  // keys past the held ones, for the number above the threshold in all
-  int above = mine.a;
-  for (int j = kHeld + t; j < n; j += kSelThreads) above += __ldcg(keys + j) > thr;
-  __syncthreads();
-  if (lane == 31) buf[0][warp] = Count3{sum.a, sum.b, 0};
-  const int all_above = block_sum3(Count3{above, 0, 0}, buf[1]).a;
-  int gt = sum.a - mine.a, eq = sum.b - mine.b;
-  for (int w = 0; w < warp; ++w) gt += buf[0][w].a, eq += buf[0][w].b;
-  const int ties = want - all_above;  // of the pages at the threshold the lowest are taken
-#pragma unroll
-  for (int i = 0; i < KPT; ++i) {
-    const bool above_it = key[i] > thr, at_it = key[i] == thr;
-    if (above_it || (at_it && eq < ties)) out[(gt + min(eq, ties)) * p.o_si] = t * KPT + i;
-    gt += above_it;
-    eq += at_it;
-  }
-  if (n <= kHeld) return;
-  // the pages that are not held, 512 at a time
-  int gt0 = 0, eq0 = 0;
-  for (int w = 0; w < kSelWarps; ++w) gt0 += buf[0][w].a, eq0 += buf[0][w].b;
-  for (int j0 = kHeld; j0 < n; j0 += kSelThreads) {
-    const unsigned k = j0 + t < n ? __ldcg(keys + j0 + t) : 0;
-    const bool above_it = k > thr, at_it = k == thr;
-    const unsigned ga = __ballot_sync(0xffffffffu, above_it), ea = __ballot_sync(0xffffffffu, at_it);
+        for (int e = 0; e < 4; ++e)
+          if (key[i][e]) keep(key[i][e]);
+    for (int j = kHeld + t; j < n; j += kSelThreads) keep(__ldcg(keys + j));
     __syncthreads();
-    if (lane == 0) buf[0][warp] = Count3{__popc(ga), __popc(ea), 0};
-    __syncthreads();
-    gt = gt0 + __popc(ga & ((1u << lane) - 1));
-    eq = eq0 + __popc(ea & ((1u << lane) - 1));
-    for (int w = 0; w < kSelWarps; ++w) {
-      if (w < warp) gt += buf[0][w].a, eq += buf[0][w].b;
-      gt0 += buf[0][w].a;
-      eq0 += buf[0][w].b;
+    const unsigned mine = t < n_left ? left[t] : 0;
+    const int need = want - above;
+    for (; bit >= 0; bit -= 2) {
+      const unsigned c1 = thr | (1u << bit), c2 = thr | (2u << bit), c3 = thr | (3u << bit);
+      const Count3 c = block_sum3(Count3{mine >= c1, mine >= c2, mine >= c3}, buf[(bit >> 1) & 1]);
+      thr = c.c >= need ? c3 : c.b >= need ? c2 : c.a >= need ? c1 : thr;
     }
-    if (above_it || (at_it && eq < ties)) out[(gt + min(eq, ties)) * p.o_si] = j0 + t;
   }
+  // the number above the threshold; of the pages at it the lowest are taken
+  int gt = 0;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) gt += key[i][e] > thr;
+  for (int j = kHeld + t; j < n; j += kSelThreads) gt += __ldcg(keys + j) > thr;
+  __syncthreads();
+  const int ties = want - block_sum3(Count3{gt, 0, 0}, buf[0]).a;
+  int gt0 = 0, eq0 = 0;  // before the keys at hand
+#pragma unroll 1
+  for (int i = 0; i < groups || i * 4 * kSelThreads < n; ++i) {
+    unsigned k[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = 4 * (i * kSelThreads + t) + e;
+      k[e] = 0;
+      if (i < GROUPS) {
+#pragma unroll
+        for (int u = 0; u < GROUPS; ++u)
+          if (u == i) k[e] = key[u][e];
+      } else if (j < n) {
+        k[e] = __ldcg(keys + j);
+      }
+    }
+    // both counts in one number: 2048 keys of a step at most
+    int mine = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mine += (k[e] > thr) + ((k[e] == thr) << 16);
+    int sum = mine;  // inclusive over the warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    __syncthreads();
+    if (lane == 31) buf[0][warp].a = sum;
+    __syncthreads();
+    const int y = lane < kSelWarps ? buf[0][lane].a : 0;
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0), all = __reduce_add_sync(0xffffffffu, y);
+    int g = gt0 + ((before + sum - mine) & 0xffff), q = eq0 + ((before + sum - mine) >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool up = k[e] > thr, at = k[e] == thr;
+      if (up || (at && q < ties)) out[(g + min(q, ties)) * o_si] = 4 * (i * kSelThreads + t) + e;
+      g += up;
+      q += at;
+    }
+    gt0 += all & 0xffff;
+    eq0 += all >> 16;
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kSelThreads, D == 256 ? 1 : 2) paged_select_kernel(const SelectParams p) {
+  extern __shared__ __align__(16) int8_t q8[];  // [heads, a multiple of 8][2D], then their scales
+  griddep_launch_dependents();
+  const int rank = blockIdx.x, ctas = gridDim.x, hk = blockIdx.y, b = blockIdx.z;
+  const int t = threadIdx.x;
+  const int n = int((int64_t(paged_len(p.g, b)) + p.g.block - 1) / p.g.block), want = min(n, p.budget);
+  int* out = p.selected + b * p.o_sb + hk * p.o_sh;
+  if (rank == 0)
+    for (int i = want + t; i < p.budget; i += kSelThreads) out[i * p.o_si] = -1;
+  if (n <= p.budget) {  // all of them
+    if (rank == 0)
+      for (int i = t; i < n; i += kSelThreads) out[i * p.o_si] = i;
+    return;
+  }
+  unsigned* keys = p.keys + (int64_t(b) * p.g.Hk + hk) * p.pitch;
+  score_pages<D>(p, b, hk, n, keys, q8, rank, ctas, t >> 5, t & 31);
+  if (ctas > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (rank) return;
+  } else {
+    __syncthreads();
+  }
+  choose_pages(keys, n, want, out, p.o_si);
 }
 
 int check_select(const bd_tensor* q, const bd_tensor* summary, const bd_tensor* summary_scale,
@@ -364,23 +417,34 @@ size_t select_bytes(const SelectParams& p) {
   return size_t(p.g.B) * p.g.Hk * ((size_t(p.g.wide) + 3) & ~size_t(3)) * sizeof(unsigned) + 256;
 }
 
-int launch_scores(const SelectParams& p, cudaStream_t st) {
+// CTAs of a row: as many as fill the GPU twice, up to the eight of a portable cluster.
+int launch_select(const SelectParams& p, cudaStream_t st) {
   const int D = p.g.D;
   const size_t smem = size_t((p.G + 7) & ~7) * (2 * D + sizeof(float));
-  const size_t sb = size_t(p.c_sb), sh = size_t(p.c_sh);
-  const bool tiles = (D == 64 || D == 128 || D == 256) && !((reinterpret_cast<uintptr_t>(p.code) | sb | sh) & 15);
-  auto kern = !tiles ? paged_score_generic_kernel : D == 64 ? paged_score_kernel<64>
-              : D == 128 ? paged_score_kernel<128> : paged_score_kernel<256>;
-  if (smem > 48 * 1024) {
-    const int rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
-                              "cudaFuncSetAttribute(paged_score)");
-    if (rc) return rc;
-  }
-  const int64_t per = tiles ? kScorePages * kScoreSteps : 256;
-  const int64_t steps = (p.g.wide + per - 1) / per;
-  if (steps > 65535) return fail(BD_ERR_SHAPE, "block_table is too wide to score: " + std::to_string(p.g.wide));
-  kern<<<dim3(p.g.Hk, unsigned(steps), p.g.B), 256, smem, st>>>(p);
-  return cuda_check(cudaGetLastError(), "paged_score_kernel launch");
+  const bool tiles = (D == 64 || D == 128 || D == 256) &&
+                     !((reinterpret_cast<uintptr_t>(p.code) | size_t(p.c_sb) | size_t(p.c_sh)) & 15);
+  auto kern = !tiles ? paged_select_kernel<0> : D == 64 ? paged_select_kernel<64>
+              : D == 128 ? paged_select_kernel<128> : paged_select_kernel<256>;
+  int rc;
+  if (smem > 40 * 1024 && (rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
+                                           "cudaFuncSetAttribute(paged_select_kernel)")))
+    return rc;
+  const int64_t rows = int64_t(p.g.B) * p.g.Hk;
+  unsigned ctas = 1;
+  while (ctas < 8 && rows * ctas * 2 <= 2 * num_sms() && int64_t(ctas) * kSelWarps * 16 < p.g.wide) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, p.g.Hk, p.g.B);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kern, p), "paged_select_kernel launch");
 }
 
 }  // namespace
@@ -420,15 +484,7 @@ int bd_paged_select(const bd_tensor* q, const bd_tensor* summary, const bd_tenso
       return fail(BD_ERR_WORKSPACE, "need " + std::to_string(need) + " workspace bytes");
     p.keys = reinterpret_cast<unsigned*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
     p.pitch = (int64_t(p.g.wide) + 3) & ~int64_t(3);
-    const bool scores = p.g.wide > p.budget;
-    if (scores && (rc = launch_scores(p, stream))) return rc;
-    auto kern = p.g.wide <= kSelThreads * 4 ? paged_choose_kernel<4> : paged_choose_kernel<16>;
-    const dim3 grid(p.g.Hk, p.g.B);
-    // what the choice reads and writes before it waits is safe behind the score kernel alone, which is
-    // launched in stream order
-    if (scores) return launch_programmatic(kern, grid, dim3(kSelThreads), 0, stream, p, "paged_choose_kernel launch");
-    kern<<<grid, kSelThreads, 0, stream>>>(p);
-    return cuda_check(cudaGetLastError(), "paged_choose_kernel launch");
+    return launch_select(p, stream);
   });
 }
 

@@ -221,6 +221,27 @@ std::tuple<int64_t, at::Tensor, Opt> paged_decode_attn(const at::Tensor& q, cons
   return {rc, out, lse};
 }
 
+// -> (status, out like q, selected int32 [B, Hk, budget])
+std::tuple<int64_t, at::Tensor, at::Tensor> paged_sparse_decode_attn(
+    const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& summary,
+    const at::Tensor& summary_scale, const at::Tensor& table, const at::Tensor& lens, int64_t budget, int64_t sink,
+    int64_t recent, double scaling, double k_scale, double v_scale) {
+  const int dev = q.get_device();
+  const bd_tensor dq = desc_row(q, dev), dk = desc(k_cache, dev), dv = desc(v_cache, dev), ds = desc(summary, dev),
+                  dss = desc(summary_scale, dev), dt = desc(table, dev), dl = desc(lens, dev);
+  if (summary.dim() != 4) return {BD_ERR_SHAPE, at::Tensor(), at::Tensor()};
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor sel = at::empty({q.size(0), summary.size(1), budget}, q.options().dtype(at::kInt));
+  const bd_tensor dout = desc_row(out, dev), dsel = desc(sel, dev);
+  const size_t nws = bd_paged_sparse_decode_attn_workspace(&dq, &dk, &dv, &ds, &dt, &dl, &dsel);
+  const at::Tensor ws = workspace(nws, q);
+  const int rc = bd_paged_sparse_decode_attn(&dq, &dk, &dv, &ds, &dss, &dt, &dl, int(sink), int(recent),
+                                             float(scaling), float(k_scale), float(v_scale), &dsel, &dout, nullptr,
+                                             ws.data_ptr(), nws, at::cuda::getCurrentCUDAStream(dev).stream());
+  return {rc, out, sel};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -233,4 +254,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_block_summary", &paged_block_summary, "bd_paged_block_summary of every page");
   m.def("paged_select", &paged_select, "bd_paged_select: (status, selected)");
   m.def("paged_decode_attn", &paged_decode_attn, "bd_paged_decode_attn: (status, out, lse)");
+  m.def("paged_sparse_decode_attn", &paged_sparse_decode_attn, "bd_paged_sparse_decode_attn: (status, out, selected)");
 }

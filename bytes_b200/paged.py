@@ -134,11 +134,12 @@ def paged_sparse_decode_attn(q, k_cache, v_cache, summary, summary_scale, block_
     """``paged_decode_attn`` over the ``budget_blocks`` pages that ``paged_select_blocks`` chooses for each
     KV head; with ``return_selected`` (out, selected)."""
     N.require_cuda(q, k_cache, v_cache, summary, summary_scale, block_table, context_lens)
-    block_table, context_lens = _int32(block_table, "block_table"), _int32(context_lens, "context_lens")
-    if k_cache.dim() != 4:
-        raise ValueError("k_cache must be [num_blocks, H_k, block, D]")
-    selected = paged_select_blocks(q, summary, summary_scale, block_table, context_lens, budget_blocks,
-                                   k_cache.shape[2], sink_blocks=sink_blocks, recent_blocks=recent_blocks)
-    out = paged_decode_attn(q, k_cache, v_cache, block_table, context_lens, scaling, k_scale=k_scale, v_scale=v_scale,
-                            selected=selected)
+    _check_row(q)
+    if budget_blocks < 1:
+        raise ValueError("budget_blocks must be at least one page")
+    rc, out, selected = N.glue().paged_sparse_decode_attn(
+        q, k_cache, v_cache, summary, summary_scale, _int32(block_table, "block_table"),
+        _int32(context_lens, "context_lens"), budget_blocks, sink_blocks, recent_blocks, scaling, k_scale, v_scale)
+    if rc:
+        N.check(rc, "bd_paged_sparse_decode_attn")
     return (out, selected) if return_selected else out

@@ -366,6 +366,8 @@ int bd_asym_fakequant(const bd_tensor* x, int levels, const bd_tensor* y, bd_str
  * [B,Hk,pages], NULL: all; entries that hold no token do not count, duplicates count once per
  * occurrence). lse f32 [B,Hq] (may be NULL) = natural log of the softmax denominator. A row
  * without a token gives zeros and lse = -inf. q [B,Hq,D] bf16/f16/f32.
+ *
+ * bd_paged_sparse_decode_attn: bd_paged_select into `selected`, then bd_paged_decode_attn over it.
  * ref: none -- the reference pages its PQ caches only (paged_attn_pq_lut_kv,
  *      src/attention_kernels.py:588); Quest's pages (benchmarks/sparse_attention.py:328-364) are
  *      ranges of a contiguous cache, with a choice per query head. */
@@ -387,6 +389,14 @@ int bd_paged_decode_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_
                          const bd_tensor* block_table, const bd_tensor* context_lens, const bd_tensor* selected,
                          float scaling, float k_scale, float v_scale, const bd_tensor* out, const bd_tensor* lse,
                          void* workspace, size_t workspace_bytes, bd_stream_t stream);
+size_t bd_paged_sparse_decode_attn_workspace(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_cache,
+                                             const bd_tensor* summary, const bd_tensor* block_table,
+                                             const bd_tensor* context_lens, const bd_tensor* selected);
+int bd_paged_sparse_decode_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_cache,
+                                const bd_tensor* summary, const bd_tensor* summary_scale, const bd_tensor* block_table,
+                                const bd_tensor* context_lens, int sink, int recent, float scaling, float k_scale,
+                                float v_scale, const bd_tensor* selected, const bd_tensor* out, const bd_tensor* lse,
+                                void* workspace, size_t workspace_bytes, bd_stream_t stream);
 
 #ifdef __cplusplus
 }
