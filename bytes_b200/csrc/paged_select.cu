@@ -12,6 +12,7 @@
 #include "decode_shared.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace bd {
 
@@ -88,16 +89,18 @@ __device__ __forceinline__ void score_pages(const SelectParams& p, int b, int hk
   const int g = lane >> 2, tq = lane & 3, step = ctas * kSelWarps * 16;
   int j0 = (rank * kSelWarps + warp) * 16;
   // rows g and g + 8 of the tile; the first tile's loads are under way while the queries are made
-  int page[2];
+  // (and a tile's page numbers while the one before it is)
+  int page[2], next[2];
   uint4 a[2][D / 32];
   float scale[2];
-  auto load_page = [&](int at) {
+  auto load_next = [&](int at) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) page[i] = at + i * 8 + g < n ? paged_block(p.g, b, at + i * 8 + g) : -1;
+    for (int i = 0; i < 2; ++i) next[i] = at + i * 8 + g < n ? paged_block(p.g, b, at + i * 8 + g) : -1;
   };
   auto load_rows = [&]() {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      page[i] = next[i];
       const int64_t at = max(page[i], 0);
       const uint4* row = reinterpret_cast<const uint4*>(p.code + at * p.c_sb + hk * p.c_sh) + tq;
 #pragma unroll
@@ -105,8 +108,9 @@ __device__ __forceinline__ void score_pages(const SelectParams& p, int b, int hk
       scale[i] = page[i] >= 0 ? __ldg(p.scale + at * p.s_sb + hk * p.s_sh) : 0.f;
     }
   };
-  load_page(j0);
+  load_next(j0);
   load_rows();
+  load_next(j0 + step);
   for (int h = warp; h < heads; h += kSelWarps) {
     if (h < p.G) {
       const float s = quantize_query(p, b, hk * p.G + h, q8 + h * 2 * D, lane);
@@ -146,8 +150,8 @@ __device__ __forceinline__ void score_pages(const SelectParams& p, int b, int hk
       key[i] = j < p.sink || j >= n - p.recent ? 0xffffffffu : page[i] < 0 ? 1u : score_key(__fmul_rn(x, scale[i]));
     }
     if (j0 + step < n) {
-      load_page(j0 + step);
       load_rows();
+      load_next(j0 + 2 * step);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -185,170 +189,181 @@ __device__ __forceinline__ void score_pages<0>(const SelectParams& p, int b, int
   }
 }
 
-// Sums over the CTA of three counts.
-struct Count3 { int a, b, c; };
-__device__ __forceinline__ Count3 block_sum3(Count3 x, Count3* buf) {
-  x.a = __reduce_add_sync(0xffffffffu, x.a);
-  x.b = __reduce_add_sync(0xffffffffu, x.b);
-  x.c = __reduce_add_sync(0xffffffffu, x.c);
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = x;
-  __syncthreads();
-  const int lane = threadIdx.x & 31;
-  const Count3 y = lane < kSelWarps ? buf[lane] : Count3{0, 0, 0};
-  return Count3{int(__reduce_add_sync(0xffffffffu, y.a)), int(__reduce_add_sync(0xffffffffu, y.b)),
-                int(__reduce_add_sync(0xffffffffu, y.c))};
-}
-
 // The largest threshold that `want` of a row's n keys reach, then the pages: those above it, and the lowest of
-// those at it. Thread t holds keys 4 (i 512 + t) .. + 3, i < 4, in registers (pages past 8192 are read again
-// from L2 each time). The threshold is found two bits at a time, from the first bit in which the keys differ,
-// by counting the keys that reach each of three candidates (no histogram: scores share their leading bits,
-// and its counters would all be the same few); once at most 512 keys are left between the bounds, each
-// thread goes on with one of them.
-__device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int want, int* out, int64_t o_si) {
-  constexpr int GROUPS = 4, kHeld = GROUPS * 4 * kSelThreads;
-  __shared__ Count3 buf[2][kSelWarps];
-  __shared__ unsigned left[kSelThreads];
+// those at it. Thread t holds keys [t each, (t + 1) each), each <= kHold, in registers (pages past 512
+// kHold are read again from L2 each time). The threshold is found eight bits at a time by a histogram, which starts at the
+// first bit in which the keys differ (scores share their leading bits, and its counters would all be the
+// same few; the `forced` pages' keys, which differ from all in all bits, are left out). Of up to 512 keys that are left each thread goes on with one; up to 32 are ranked by a warp.
+template <int kHold>
+__device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int want, int forced, int* out, int64_t o_si) {
+  __shared__ unsigned left[kSelThreads], bound[2][kSelWarps];
+  __shared__ int hist[256], sums[kSelWarps];
   __shared__ int n_left;
+  __shared__ unsigned found[3];  // bin or threshold, keys above, keys left
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int groups = min(GROUPS, (n + 4 * kSelThreads - 1) / (4 * kSelThreads));
-  unsigned key[GROUPS][4];
-  unsigned lo = 0xffffffffu, hi = 0;
+  const int each = min(kHold, ((n + kSelThreads - 1) / kSelThreads + 3) & ~3), held = each * kSelThreads;
+  unsigned key[kHold], lo = 0xffffffffu, hi = 0;
+  auto scored = [](unsigned k) { return k - 1u < 0xfffffffeu; };  // neither 0 nor forced
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    const int j = 4 * (i * kSelThreads + t);
+  for (int i = 0; i < kHold; i += 4) {
+    const int j = t * each + i;
     // rows are padded to four keys; what lies past n is not a key
-    const uint4 x = j < n ? __ldcg(reinterpret_cast<const uint4*>(keys + j)) : make_uint4(0, 0, 0, 0);
-    key[i][0] = x.x;
-    key[i][1] = j + 1 < n ? x.y : 0;
-    key[i][2] = j + 2 < n ? x.z : 0;
-    key[i][3] = j + 3 < n ? x.w : 0;
+    const uint4 x = i < each && j < n ? __ldcg(reinterpret_cast<const uint4*>(keys + j)) : make_uint4(0, 0, 0, 0);
+    key[i] = x.x;
+    key[i + 1] = j + 1 < n ? x.y : 0;
+    key[i + 2] = j + 2 < n ? x.z : 0;
+    key[i + 3] = j + 3 < n ? x.w : 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      hi = max(hi, key[i][e]);
-      if (key[i][e]) lo = min(lo, key[i][e]);
-    }
+    for (int e = 0; e < 4; ++e)
+      if (scored(key[i + e])) hi = max(hi, key[i + e]), lo = min(lo, key[i + e]);
   }
-  for (int j = kHeld + t; j < n; j += kSelThreads) {
+  for (int j = held + t; j < n; j += kSelThreads) {
     const unsigned k = __ldcg(keys + j);
-    hi = max(hi, k);
-    lo = min(lo, k);
+    if (scored(k)) hi = max(hi, k), lo = min(lo, k);
   }
   hi = __reduce_max_sync(0xffffffffu, hi);
   lo = __reduce_min_sync(0xffffffffu, lo);
-  if (lane == 0) buf[1][warp] = Count3{int(hi), int(lo), 0};
+  if (lane == 0) bound[0][warp] = hi, bound[1][warp] = lo;
+  if (t < 256) hist[t] = 0;
   if (t == 0) n_left = 0;
   __syncthreads();
-  {
-    const Count3 y = buf[1][lane % kSelWarps];
-    hi = __reduce_max_sync(0xffffffffu, unsigned(y.a));
-    lo = __reduce_min_sync(0xffffffffu, unsigned(y.b));
-  }
-  __syncthreads();
-  // all keys share the bits above `bit`
-  int bit = hi == lo ? -2 : (31 - __clz(hi ^ lo)) & ~1;
-  unsigned thr = hi == lo ? hi : bit >= 30 ? 0u : hi & ~((4u << bit) - 1u);
-  int reach = n, above = 0;  // keys that reach thr, and that are above what thr may still become
-  for (; bit >= 0 && reach - above > kSelThreads; bit -= 2) {
-    const unsigned c1 = thr | (1u << bit), c2 = thr | (2u << bit), c3 = thr | (3u << bit);
-    Count3 c{0, 0, 0};
+  hi = __reduce_max_sync(0xffffffffu, bound[0][lane % kSelWarps]);
+  lo = __reduce_min_sync(0xffffffffu, bound[1][lane % kSelWarps]);
+  // the threshold's known leading bits, how many are not known, the keys that share them, those above
+  int low = hi == lo ? 0 : 32 - __clz(hi ^ lo);
+  unsigned thr = low == 32 ? 0u : hi >> low << low;
+  int rest = n - forced, above = forced;
+  if (want <= forced) thr = 0xffffffffu, above = 0, low = 0;
+  unsigned mine = 0;
+  bool one = false;  // each thread has one key
+  auto among = [&](unsigned k) { return scored(k) && (low == 32 || k >> low == thr >> low); };
+  // calls f for the keys that are left
+  auto each_key = [&](auto&& f) {
+    if (one) {
+      if (among(mine)) f(mine);
+      return;
+    }
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i)
-      if (i < groups)
+    for (int i = 0; i < kHold; i += 4) {
+      if (i >= each) break;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          c.a += key[i][e] >= c1;
-          c.b += key[i][e] >= c2;
-          c.c += key[i][e] >= c3;
-        }
-    for (int j = kHeld + t; j < n; j += kSelThreads) {
+      for (int e = 0; e < 4; ++e)
+        if (among(key[i + e])) f(key[i + e]);
+    }
+    for (int j = held + t; j < n; j += kSelThreads) {
       const unsigned k = __ldcg(keys + j);
-      c.a += k >= c1;
-      c.b += k >= c2;
-      c.c += k >= c3;
+      if (among(k)) f(k);
     }
-    c = block_sum3(c, buf[(bit >> 1) & 1]);
-    if (c.c >= want) thr = c3, reach = c.c;
-    else if (c.b >= want) thr = c2, reach = c.b, above = c.c;
-    else if (c.a >= want) thr = c1, reach = c.a, above = c.b;
-    else above = c.a;
-  }
-  if (bit >= 0) {
-    // the keys between thr and the next value that it cannot be
-    const unsigned span = bit >= 30 ? 0xffffffffu : (4u << bit) - 1u;
-    auto keep = [&](unsigned k) {
-      if (k >= thr && k - thr <= span) left[atomicAdd(&n_left, 1)] = k;
-    };
-#pragma unroll
-    for (int i = 0; i < GROUPS; ++i)
-      if (i < groups)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key[i][e]) keep(key[i][e]);
-    for (int j = kHeld + t; j < n; j += kSelThreads) keep(__ldcg(keys + j));
-    __syncthreads();
-    const unsigned mine = t < n_left ? left[t] : 0;
-    const int need = want - above;
-    for (; bit >= 0; bit -= 2) {
-      const unsigned c1 = thr | (1u << bit), c2 = thr | (2u << bit), c3 = thr | (3u << bit);
-      const Count3 c = block_sum3(Count3{mine >= c1, mine >= c2, mine >= c3}, buf[(bit >> 1) & 1]);
-      thr = c.c >= need ? c3 : c.b >= need ? c2 : c.a >= need ? c1 : thr;
-    }
-  }
-  // the number above the threshold; of the pages at it the lowest are taken
-  int gt = 0;
-#pragma unroll
-  for (int i = 0; i < GROUPS; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) gt += key[i][e] > thr;
-  for (int j = kHeld + t; j < n; j += kSelThreads) gt += __ldcg(keys + j) > thr;
-  __syncthreads();
-  const int ties = want - block_sum3(Count3{gt, 0, 0}, buf[0]).a;
-  int gt0 = 0, eq0 = 0;  // before the keys at hand
+  };
 #pragma unroll 1
-  for (int i = 0; i < groups || i * 4 * kSelThreads < n; ++i) {
-    unsigned k[4];
+  while (low > 0) {
+    if (rest <= 32 || (!one && rest <= kSelThreads)) {
+      each_key([&](unsigned k) { left[atomicAdd(&n_left, 1)] = k; });
+      __syncthreads();
+      if (rest <= 32) {  // their rank: need of them reach the threshold
+        if (warp == 0) {
+          const unsigned k = lane < rest ? left[lane] : 0;
+          int up = 0, at = 0;
+#pragma unroll 8
+          for (int i = 0; i < 32; ++i) {
+            const unsigned x = __shfl_sync(0xffffffffu, k, i);
+            up += x > k;
+            at += x == k;
+          }
+          const int need = want - above;
+          const int who = __ffs(__ballot_sync(0xffffffffu, k && up < need && need <= up + at)) - 1;
+          if (lane == who) found[0] = k, found[1] = above + up;
+        }
+        __syncthreads();
+        thr = found[0];
+        above = int(found[1]);
+        break;
+      }
+      mine = t < rest ? left[t] : 0;
+      one = true;
+      __syncthreads();
+      if (t == 0) n_left = 0;
+    }
+    const int shift = max(low - 8, 0);
+    const unsigned mask = (1u << (low - shift)) - 1u;
+    each_key([&](unsigned k) { atomicAdd(&hist[k >> shift & mask], 1); });
+    __syncthreads();
+    if (warp == 0) {
+      int bin[8], sum = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int j = 4 * (i * kSelThreads + t) + e;
-      k[e] = 0;
-      if (i < GROUPS) {
+      for (int i = 0; i < 8; ++i) sum += bin[i] = hist[lane * 8 + i];
+      int up = sum;  // keys in this lane's bins and the higher ones
 #pragma unroll
-        for (int u = 0; u < GROUPS; ++u)
-          if (u == i) k[e] = key[u][e];
-      } else if (j < n) {
-        k[e] = __ldcg(keys + j);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_down_sync(0xffffffffu, up, o);
+        if (lane + o < 32) up += x;
+      }
+      int over = above + up - sum;
+      if (over < want && want <= over + sum) {
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+          if (over < want && want <= over + bin[i]) found[0] = lane * 8 + i, found[1] = over, found[2] = bin[i];
+          over += bin[i];
+        }
       }
     }
-    // both counts in one number: 2048 keys of a step at most
-    int mine = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) mine += (k[e] > thr) + ((k[e] == thr) << 16);
-    int sum = mine;  // inclusive over the warp
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
-    }
     __syncthreads();
-    if (lane == 31) buf[0][warp].a = sum;
+    thr |= found[0] << shift;
+    above = int(found[1]);
+    rest = int(found[2]);
+    low = shift;
+    if (t < 256) hist[t] = 0;
     __syncthreads();
-    const int y = lane < kSelWarps ? buf[0][lane].a : 0;
-    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0), all = __reduce_add_sync(0xffffffffu, y);
-    int g = gt0 + ((before + sum - mine) & 0xffff), q = eq0 + ((before + sum - mine) >> 16);
+  }
+  const int ties = want - above;  // of the pages at the threshold the lowest are taken
+  // where this thread's pages go: the numbers above and at the threshold before them, in one (8192 at most)
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) count += (key[i] > thr) + ((key[i] == thr) << 16);
+  int sum = count;  // inclusive over the warp
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += x;
+  }
+  if (lane == 31) sums[warp] = sum;
+  __syncthreads();
+  const int y = lane < kSelWarps ? sums[lane] : 0;
+  const int before = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0) + sum - count;
+  int up = before & 0xffff, at = before >> 16;
+#pragma unroll
+  for (int i = 0; i < kHold; i += 4) {
+    if (i >= each) break;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const bool up = k[e] > thr, at = k[e] == thr;
-      if (up || (at && q < ties)) out[(g + min(q, ties)) * o_si] = 4 * (i * kSelThreads + t) + e;
-      g += up;
-      q += at;
+      const bool is_up = key[i + e] > thr, is_at = key[i + e] == thr;
+      if (is_up || (is_at && at < ties)) out[(up + min(at, ties)) * o_si] = t * each + i + e;
+      up += is_up;
+      at += is_at;
     }
-    gt0 += all & 0xffff;
-    eq0 += all >> 16;
+  }
+  if (n <= held) return;
+  // the pages that are not held, 512 at a time
+  const int all = __reduce_add_sync(0xffffffffu, y);
+  int up0 = all & 0xffff, at0 = all >> 16;
+#pragma unroll 1
+  for (int j0 = held; j0 < n; j0 += kSelThreads) {
+    const unsigned k = j0 + t < n ? __ldcg(keys + j0 + t) : 0;
+    const unsigned ups = __ballot_sync(0xffffffffu, k > thr), ats = __ballot_sync(0xffffffffu, k == thr);
+    __syncthreads();
+    if (lane == 0) sums[warp] = __popc(ups) + (__popc(ats) << 16);
+    __syncthreads();
+    const int z = lane < kSelWarps ? sums[lane] : 0;
+    const int b4 = __reduce_add_sync(0xffffffffu, lane < warp ? z : 0), sum_all = __reduce_add_sync(0xffffffffu, z);
+    const unsigned below = (1u << lane) - 1u;
+    const int u = up0 + (b4 & 0xffff) + __popc(ups & below), q = at0 + (b4 >> 16) + __popc(ats & below);
+    if (k > thr || (k == thr && q < ties)) out[(u + min(q, ties)) * o_si] = j0 + t;
+    up0 += sum_all & 0xffff;
+    at0 += sum_all >> 16;
   }
 }
 
-template <int D>
+template <int D, int HOLD>
 __global__ void __launch_bounds__(kSelThreads, D == 256 ? 1 : 2) paged_select_kernel(const SelectParams p) {
   extern __shared__ __align__(16) int8_t q8[];  // [heads, a multiple of 8][2D], then their scales
   griddep_launch_dependents();
@@ -371,7 +386,7 @@ __global__ void __launch_bounds__(kSelThreads, D == 256 ? 1 : 2) paged_select_ke
   } else {
     __syncthreads();
   }
-  choose_pages(keys, n, want, out, p.o_si);
+  choose_pages<HOLD>(keys, n, want, p.sink + p.recent, out, p.o_si);
 }
 
 int check_select(const bd_tensor* q, const bd_tensor* summary, const bd_tensor* summary_scale,
@@ -423,8 +438,12 @@ int launch_select(const SelectParams& p, cudaStream_t st) {
   const size_t smem = size_t((p.G + 7) & ~7) * (2 * D + sizeof(float));
   const bool tiles = (D == 64 || D == 128 || D == 256) &&
                      !((reinterpret_cast<uintptr_t>(p.code) | size_t(p.c_sb) | size_t(p.c_sh)) & 15);
-  auto kern = !tiles ? paged_select_kernel<0> : D == 64 ? paged_select_kernel<64>
-              : D == 128 ? paged_select_kernel<128> : paged_select_kernel<256>;
+  auto of = [&](auto hold) {
+    constexpr int H = decltype(hold)::value;
+    return !tiles ? paged_select_kernel<0, H> : D == 64 ? paged_select_kernel<64, H>
+           : D == 128 ? paged_select_kernel<128, H> : paged_select_kernel<256, H>;
+  };
+  auto kern = p.g.wide <= 4 * kSelThreads ? of(std::integral_constant<int, 4>()) : of(std::integral_constant<int, 16>());
   int rc;
   if (smem > 40 * 1024 && (rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
                                            "cudaFuncSetAttribute(paged_select_kernel)")))
