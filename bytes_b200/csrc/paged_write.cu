@@ -409,113 +409,184 @@ template <> struct Pair<__half> {
   static __device__ __forceinline__ float2 wide(V x) { return __half22float2(x); }
 };
 
-// 16- and 8-bit caches with 16-byte aligned rows: one warp per (page, KV head). A row is LPR lanes of 16
-// bytes, so a load instruction takes 32 / LPR rows; eight are in flight at a time. The row groups
-// then meet by shuffles; the first of them writes the minima, the second the maxima.
+// 16- and 8-bit caches with 16-byte aligned rows: a warp goes over pages for one KV head, every `stride`-th. A
+// row is LPR lanes of 16 bytes, so a load instruction takes 32 / LPR rows; eight are a step, the next step's
+// (of this page, or the next one's first) in flight while one is worked off, and the page number after that
+// as well. At a page's end the row groups meet by shuffles; the first of them writes the minima, the
+// second the maxima.
 template <typename T, bool FP8, int LPR>
-__global__ void __launch_bounds__(256) paged_summary_kernel(const SummaryParams p) {
+__global__ void __launch_bounds__(256, 2) paged_summary_kernel(const SummaryParams p, int64_t pages) {
   using P = Pair<T>;
   using V = typename P::V;
-  constexpr int NP = FP8 ? 8 : 4, GROUPS = 32 / LPR, D = LPR * NP * 2;
+  constexpr int NP = FP8 ? 8 : 4, GROUPS = 32 / LPR, D = LPR * NP * 2, ES = FP8 ? 1 : 2, STEP = 8 * GROUPS;
   const int lane = threadIdx.x & 31, part = lane % LPR, group = lane / LPR;
-  const int64_t w = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int h = int(w % p.g.Hk);
-  int b, j;
-  if (!page_of_item(p, w / p.g.Hk, b, j)) return;
-  const int n = int(min(int64_t(p.g.block), paged_len(p.g, b) - int64_t(j) * p.g.block));
-  if (n <= 0) return;
-  const int page = paged_block(p.g, b, j);
-  if (page < 0) return;
-  constexpr int ES = FP8 ? 1 : 2;
-  const uint8_t* base = static_cast<const uint8_t*>(p.k_cache) + (page * p.g.k_sb + h * p.g.k_sh) * ES + part * 16;
-  V lo[NP], hi[NP];
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    lo[i] = P::bits(std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u);
-    hi[i] = P::bits(std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
-  }
-  for (int r0 = 0; r0 < n; r0 += 8 * GROUPS) {
-    uint4 x[8];
+  const int w = blockIdx.x * 8 + (threadIdx.x >> 5), stride = int(gridDim.x) * 8 / p.g.Hk, h = w % p.g.Hk;
+  int64_t i = w / p.g.Hk;
+  if (i >= stride || i >= pages) return;
+  struct Item {
+    int page, n;  // n: its tokens, 0 if there is nothing to do
+  };
+  // of all pages: sequence and column of the next one, without a division each
+  int nb = 0, nj = 0;
+  const int wide = max(p.g.wide, 1), db = stride / wide, dj = stride - db * wide;
+  if (p.T == 0) nb = int(i / wide), nj = int(i - int64_t(nb) * wide);
+  auto next_item = [&](int64_t at) {
+    Item it{0, 0};
+    int b = nb, j = nj;
+    if (p.T == 0) {
+      nb += db;
+      nj += dj;
+      if (nj >= wide) nj -= wide, ++nb;
+    }
+    if (at >= pages || (p.T > 0 && !page_of_item(p, at, b, j))) return it;
+    it.page = paged_block(p.g, b, j);
+    // (a length past the table's end does not make a page longer: j is within it)
+    const int len = p.g.lens[int64_t(b) * p.g.l_s];
+    it.n = it.page < 0 ? 0 : int(max(int64_t(0), min(int64_t(p.g.block), len - int64_t(j) * p.g.block)));
+    return it;
+  };
+  auto load = [&](uint4 (&x)[8], const Item& it, int r0) {
+    const uint8_t* base = static_cast<const uint8_t*>(p.k_cache) + (it.page * p.g.k_sb + h * p.g.k_sh) * ES + part * 16;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       // rows past the last are read as the last one again
-      const int r = min(r0 + i * GROUPS + group, n - 1);
-      x[i] = *reinterpret_cast<const uint4*>(base + int64_t(r) * p.g.k_st * ES);
+      const int r = min(r0 + i * GROUPS + group, it.n - 1);
+      if (it.n > 0) x[i] = *reinterpret_cast<const uint4*>(base + int64_t(r) * p.g.k_st * ES);
     }
+  };
+  V lo[NP], hi[NP];
+  auto reset = [&]() {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    for (int i = 0; i < NP; ++i) {
+      lo[i] = P::bits(std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u);
+      hi[i] = P::bits(std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
+    }
+  };
+  auto finish = [&](const Item& it) {
 #pragma unroll
-      for (int e = 0; e < NP; ++e) {
-        const V v = P::bits(FP8 ? e4m3x2_to_f16x2(u[e / 2] >> (16 * (e & 1))) : u[e]);
-        lo[e] = __hmin2(lo[e], v);
-        hi[e] = __hmax2(hi[e], v);
+    for (int e = 0; e < NP; ++e)
+#pragma unroll
+      for (int o = LPR; o < 32; o <<= 1) {
+        lo[e] = __hmin2(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
+        hi[e] = __hmax2(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
+      }
+    V far = __hmax2(hi[0], __hneg2(lo[0]));  // the largest magnitude
+#pragma unroll
+    for (int e = 1; e < NP; ++e) far = __hmax2(far, __hmax2(hi[e], __hneg2(lo[e])));
+    const float2 f = P::wide(far);
+    float top = fmaxf(fabsf(f.x), fabsf(f.y));
+    if (FP8) top = __fmul_rn(top, p.k_scale);
+    top = fminf(warp_max(top), FLT_MAX);
+    const float s = __fdiv_rn(top, 127.f), inv = top > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    // rint(x / s), the quotient rounded to 32 bits first: x * inv is within 2^-15 of it, so that it rounds to
+    // the same whole number (by the sum with 1.5 * 2^23, whose low byte it then is) unless it comes near
+    // half of one; then, and for infinities, the division is made
+    constexpr float kMagic = 12582912.f;
+    auto put = [&](const V* v, int8_t* to) {
+      uint32_t u[NP / 2];
+#pragma unroll
+      for (int e = 0; e < NP / 2; ++e) {
+        const float2 a = P::wide(v[2 * e]), c = P::wide(v[2 * e + 1]);
+        float x[4] = {a.x, a.y, c.x, c.y}, t[4];
+        bool near = top >= FLT_MAX || inv >= FLT_MAX;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (FP8) x[i] = __fmul_rn(x[i], p.k_scale);
+          t[i] = fmaf(x[i], inv, kMagic);
+          near |= fabsf(fmaf(x[i], inv, kMagic - t[i])) > 0.499f;
+        }
+        u[e] = prmt(prmt(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
+                    prmt(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+        if (near) {
+          u[e] = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[e] |= uint32_t(uint8_t(code_of(x[i], s, top > 0.f))) << (8 * i);
+        }
+      }
+      if (FP8) *reinterpret_cast<uint4*>(to + part * 16) = make_uint4(u[0], u[1], u[NP / 2 - 2], u[NP / 2 - 1]);
+      else *reinterpret_cast<uint2*>(to + part * 8) = make_uint2(u[0], u[1]);
+    };
+    int8_t* code = p.code + it.page * p.c_sb + h * p.c_sh;
+    if (GROUPS == 1) {
+      put(lo, code);
+      put(hi, code + D);
+    } else if (group < 2) {
+#pragma unroll
+      for (int e = 0; e < NP; ++e) lo[e] = group ? hi[e] : lo[e];
+      put(lo, code + group * D);
+    }
+    if (lane == 0) p.scale[it.page * p.s_sb + h * p.s_sh] = s;
+  };
+  Item it = next_item(i), next = next_item(i + stride);
+  int r0 = 0;
+  uint4 x[2][8];
+  load(x[0], it, 0);
+  reset();
+  // one step on x, the next one's rows into y; false after the last
+  auto step = [&](uint4 (&x)[8], uint4 (&y)[8]) {
+    const bool last = r0 + STEP >= it.n;
+    load(y, last ? next : it, last ? 0 : r0 + STEP);
+    Item after = next;
+    if (last) after = next_item(i + 2 * int64_t(stride));
+    if (it.n > 0) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t u[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+        for (int e = 0; e < NP; ++e) {
+          const V v = P::bits(FP8 ? e4m3x2_to_f16x2(u[e / 2] >> (16 * (e & 1))) : u[e]);
+          lo[e] = __hmin2(lo[e], v);
+          hi[e] = __hmax2(hi[e], v);
+        }
+      }
+      if (last) {
+        finish(it);
+        reset();
       }
     }
-  }
-  float lof[2 * NP], hif[2 * NP], top = 0.f;
-#pragma unroll
-  for (int e = 0; e < NP; ++e) {
-#pragma unroll
-    for (int o = LPR; o < 32; o <<= 1) {
-      lo[e] = __hmin2(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
-      hi[e] = __hmax2(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
+    if (!last) {
+      r0 += STEP;
+      return true;
     }
-    const float2 a = P::wide(lo[e]), c = P::wide(hi[e]);
-    lof[2 * e] = __fmul_rn(a.x, p.k_scale); lof[2 * e + 1] = __fmul_rn(a.y, p.k_scale);
-    hif[2 * e] = __fmul_rn(c.x, p.k_scale); hif[2 * e + 1] = __fmul_rn(c.y, p.k_scale);
-    top = fmaxf(top, fmaxf(fmaxf(fabsf(lof[2 * e]), fabsf(lof[2 * e + 1])), fmaxf(fabsf(hif[2 * e]), fabsf(hif[2 * e + 1]))));
-  }
-  top = fminf(warp_max(top), FLT_MAX);
-  const float s = __fdiv_rn(top, 127.f);
-  int8_t* code = p.code + page * p.c_sb + h * p.c_sh;
-  auto put = [&](const float* x, int8_t* to) {
-    uint32_t u[NP / 2];
-#pragma unroll
-    for (int e = 0; e < NP / 2; ++e) {
-      u[e] = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[e] |= uint32_t(uint8_t(code_of(x[4 * e + i], s, top > 0.f))) << (8 * i);
-    }
-    if (FP8) *reinterpret_cast<uint4*>(to + part * 16) = make_uint4(u[0], u[1], u[NP / 2 - 2], u[NP / 2 - 1]);
-    else *reinterpret_cast<uint2*>(to + part * 8) = make_uint2(u[0], u[1]);
+    r0 = 0;
+    it = next;
+    next = after;
+    i += stride;
+    return i < pages;
   };
-  if (GROUPS == 1) {
-    put(lof, code);
-    put(hif, code + D);
-  } else if (group < 2) {
-#pragma unroll
-    for (int e = 0; e < 2 * NP; ++e) lof[e] = group ? hif[e] : lof[e];
-    put(lof, code + group * D);
+#pragma unroll 1
+  while (step(x[0], x[1]) && step(x[1], x[0])) {
   }
-  if (lane == 0) p.scale[page * p.s_sb + h * p.s_sh] = s;
 }
 
 int launch_summary(const SummaryParams& p, bool vector, cudaStream_t st) {
-  const int64_t items = p.T == 0 ? int64_t(p.g.B) * p.g.wide
+  const int64_t pages = p.T == 0 ? int64_t(p.g.B) * p.g.wide
                         : !p.cu  ? int64_t(p.g.B)
                                  : 2 * int64_t(p.g.B) + (int64_t(p.T) + p.g.block - 1) / p.g.block;
-  const int per = vector ? 8 : 4;
-  const int64_t ctas = (items * p.g.Hk + per - 1) / per;
-  if (ctas == 0) return BD_OK;
-  if (ctas > 0x7fffffff) return fail(BD_ERR_SHAPE, "too many pages for one launch");
+  const int64_t items = pages * p.g.Hk;
+  if (items == 0) return BD_OK;
+  if (!vector) {
+    if (items > 4 * int64_t(0x7fffffff)) return fail(BD_ERR_SHAPE, "too many pages for one launch");
+    paged_summary_generic_kernel<<<unsigned((items + 3) / 4), 128, 0, st>>>(p);
+    return cuda_check(cudaGetLastError(), "paged_summary_generic_kernel launch");
+  }
+  // two CTAs an SM, and a warp for every KV head at least
+  const unsigned ctas = unsigned(std::max<int64_t>((p.g.Hk + 7) / 8, std::min<int64_t>((items + 7) / 8, 2 * num_sms())));
   auto go = [&](auto kern) {
-    kern<<<unsigned(ctas), per * 32, 0, st>>>(p);
+    kern<<<ctas, 256, 0, st>>>(p, pages);
     return cuda_check(cudaGetLastError(), "paged_summary_kernel launch");
   };
-  if (!vector) return go(paged_summary_generic_kernel);
+  auto with = [&](auto k64, auto k128, auto k256) { return p.g.D == 64 ? go(k64) : p.g.D == 128 ? go(k128) : go(k256); };
   switch (p.dtype) {
     case BD_BF16:
-      return p.g.D == 64 ? go(paged_summary_kernel<__nv_bfloat16, false, 8>)
-             : p.g.D == 128 ? go(paged_summary_kernel<__nv_bfloat16, false, 16>)
-                            : go(paged_summary_kernel<__nv_bfloat16, false, 32>);
+      return with(paged_summary_kernel<__nv_bfloat16, false, 8>, paged_summary_kernel<__nv_bfloat16, false, 16>,
+                  paged_summary_kernel<__nv_bfloat16, false, 32>);
     case BD_F16:
-      return p.g.D == 64 ? go(paged_summary_kernel<__half, false, 8>)
-             : p.g.D == 128 ? go(paged_summary_kernel<__half, false, 16>)
-                            : go(paged_summary_kernel<__half, false, 32>);
+      return with(paged_summary_kernel<__half, false, 8>, paged_summary_kernel<__half, false, 16>,
+                  paged_summary_kernel<__half, false, 32>);
     default:
-      return p.g.D == 64 ? go(paged_summary_kernel<__half, true, 4>)
-             : p.g.D == 128 ? go(paged_summary_kernel<__half, true, 8>) : go(paged_summary_kernel<__half, true, 16>);
+      return with(paged_summary_kernel<__half, true, 4>, paged_summary_kernel<__half, true, 8>,
+                  paged_summary_kernel<__half, true, 16>);
   }
 }
 
