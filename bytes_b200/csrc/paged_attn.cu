@@ -177,6 +177,12 @@ struct TileShape {
 // waits on tile copies that ran past their limit (a result is then NaN)
 __device__ unsigned int g_paged_timeouts = 0;
 
+// Four e4m3 bytes as two f16 pairs, the word's lower and upper half (exact).
+__device__ __forceinline__ void widen4(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+      : "=r"(lo), "=r"(hi) : "r"(x));
+}
+
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
 __device__ __forceinline__ void prefetch_tensormap(const void* map) {
@@ -638,10 +644,11 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
                 if (KIND == kBf16) mma_bf16(s[nt], r0, r1, r2, r3, qb[c][nt][0], qb[c][nt][1]);
                 else mma_f16(s[nt], r0, r1, r2, r3, qb[c][nt][0], qb[c][nt][1]);
             } else {
-              const uint32_t x0 = e4m3x2_to_f16x2(r0), x1 = e4m3x2_to_f16x2(r1);
-              const uint32_t x2 = e4m3x2_to_f16x2(r0 >> 16), x3 = e4m3x2_to_f16x2(r1 >> 16);
-              const uint32_t y0 = e4m3x2_to_f16x2(r2), y1 = e4m3x2_to_f16x2(r3);
-              const uint32_t y2 = e4m3x2_to_f16x2(r2 >> 16), y3 = e4m3x2_to_f16x2(r3 >> 16);
+              uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
+              widen4(r0, x0, x2);
+              widen4(r1, x1, x3);
+              widen4(r2, y0, y2);
+              widen4(r3, y1, y3);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 mma_f16(s[nt], x0, x1, x2, x3, qb[2 * c % KSTEPS][nt][0], qb[2 * c % KSTEPS][nt][1]);
@@ -716,10 +723,11 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
             ldmatrix_x4_trans(r0, r1, r2, r3, from + (m2 * 32 / T::SW) * slab + ((m2 * 32 % T::SW) ^ (hi ^ x)));
             // r0, r1: tokens 0-7, 8-15 of channels [32 m2, +16); r2, r3: of the next 16; each holds
             // (token 2tq: channels 2g, 2g+1 | token 2tq+1: the same)
-            const uint32_t a0 = e4m3x2_to_f16x2(prmt(r0, 0, 0x0020)), a1 = e4m3x2_to_f16x2(prmt(r0, 0, 0x0031));
-            const uint32_t a2 = e4m3x2_to_f16x2(prmt(r1, 0, 0x0020)), a3 = e4m3x2_to_f16x2(prmt(r1, 0, 0x0031));
-            const uint32_t c0 = e4m3x2_to_f16x2(prmt(r2, 0, 0x0020)), c1 = e4m3x2_to_f16x2(prmt(r2, 0, 0x0031));
-            const uint32_t c2 = e4m3x2_to_f16x2(prmt(r3, 0, 0x0020)), c3 = e4m3x2_to_f16x2(prmt(r3, 0, 0x0031));
+            uint32_t a0, a1, a2, a3, c0, c1, c2, c3;
+            widen4(prmt(r0, 0, 0x3120), a0, a1);
+            widen4(prmt(r1, 0, 0x3120), a2, a3);
+            widen4(prmt(r2, 0, 0x3120), c0, c1);
+            widen4(prmt(r3, 0, 0x3120), c2, c3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma_f16(o[2 * m2][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);

@@ -142,6 +142,9 @@ struct OptDesc {
   }
 };
 
+// Tables and lengths as the kernels read them.
+at::Tensor as_int32(const at::Tensor& t) { return t.scalar_type() == at::kInt ? t : t.to(at::kInt); }
+
 // A decode query or output: [B, H, D], or [B, H, 1, D] viewed so.
 bd_tensor desc_row(const at::Tensor& t, int device) {
   return t.dim() == 4 && t.size(2) == 1 ? desc_drop2(t, device) : desc(t, device);
@@ -150,10 +153,13 @@ bd_tensor desc_row(const at::Tensor& t, int device) {
 // bd_paged_append, then bd_paged_block_summary of the touched pages when a summary is kept
 // -> (status, rotated queries or None).
 std::tuple<int64_t, Opt> paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
-                                      const at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& lens,
-                                      const Opt& q, const Opt& cos, const Opt& sin, bool interleaved, const Opt& cu,
+                                      const at::Tensor& v_cache, const at::Tensor& table_, const at::Tensor& lens_,
+                                      const Opt& q, const Opt& cos, const Opt& sin, bool interleaved, const Opt& cu_,
                                       double k_scale, double v_scale, const Opt& summary, const Opt& summary_scale) {
   const int dev = k.get_device();
+  const at::Tensor table = as_int32(table_), lens = as_int32(lens_);
+  Opt cu;
+  if (cu_.has_value()) cu = as_int32(*cu_);
   const bd_tensor dk = desc(k, dev), dv = desc(v, dev), dkc = desc(k_cache, dev), dvc = desc(v_cache, dev),
                   dt = desc(table, dev), dl = desc(lens, dev);
   const OptDesc dq(q, dev), dcos(cos, dev), dsin(sin, dev), dcu(cu, dev), ds(summary, dev), dss(summary_scale, dev);
@@ -169,9 +175,10 @@ std::tuple<int64_t, Opt> paged_append(const at::Tensor& k, const at::Tensor& v, 
   return {rc, q_out};
 }
 
-int64_t paged_block_summary(const at::Tensor& k_cache, const at::Tensor& table, const at::Tensor& lens,
+int64_t paged_block_summary(const at::Tensor& k_cache, const at::Tensor& table_, const at::Tensor& lens_,
                             double k_scale, const at::Tensor& summary, const at::Tensor& summary_scale) {
   const int dev = k_cache.get_device();
+  const at::Tensor table = as_int32(table_), lens = as_int32(lens_);
   const bd_tensor dkc = desc(k_cache, dev), dt = desc(table, dev), dl = desc(lens, dev), ds = desc(summary, dev),
                   dss = desc(summary_scale, dev);
   const c10::cuda::CUDAGuard guard(k_cache.device());
@@ -181,10 +188,11 @@ int64_t paged_block_summary(const at::Tensor& k_cache, const at::Tensor& table, 
 
 // -> (status, selected int32 [B, Hk, budget])
 std::tuple<int64_t, at::Tensor> paged_select(const at::Tensor& q, const at::Tensor& summary,
-                                             const at::Tensor& summary_scale, const at::Tensor& table,
-                                             const at::Tensor& lens, int64_t block_size, int64_t budget, int64_t sink,
+                                             const at::Tensor& summary_scale, const at::Tensor& table_,
+                                             const at::Tensor& lens_, int64_t block_size, int64_t budget, int64_t sink,
                                              int64_t recent) {
   const int dev = q.get_device();
+  const at::Tensor table = as_int32(table_), lens = as_int32(lens_);
   const bd_tensor dq = desc_row(q, dev), ds = desc(summary, dev), dss = desc(summary_scale, dev),
                   dt = desc(table, dev), dl = desc(lens, dev);
   if (summary.dim() != 4) return {BD_ERR_SHAPE, at::Tensor()};
@@ -200,12 +208,15 @@ std::tuple<int64_t, at::Tensor> paged_select(const at::Tensor& q, const at::Tens
 
 // -> (status, out like q, lse [B, Hq] or None)
 std::tuple<int64_t, at::Tensor, Opt> paged_decode_attn(const at::Tensor& q, const at::Tensor& k_cache,
-                                                       const at::Tensor& v_cache, const at::Tensor& table,
-                                                       const at::Tensor& lens, const Opt& selected, double scaling,
+                                                       const at::Tensor& v_cache, const at::Tensor& table_,
+                                                       const at::Tensor& lens_, const Opt& selected_, double scaling,
                                                        double k_scale, double v_scale, bool want_lse) {
   const int dev = q.get_device();
+  const at::Tensor table = as_int32(table_), lens = as_int32(lens_);
   const bd_tensor dq = desc_row(q, dev), dk = desc(k_cache, dev), dv = desc(v_cache, dev), dt = desc(table, dev),
                   dl = desc(lens, dev);
+  Opt selected;
+  if (selected_.has_value()) selected = as_int32(*selected_);
   const OptDesc dsel(selected, dev);
   const c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = at::empty(q.sizes(), q.options());
@@ -224,9 +235,10 @@ std::tuple<int64_t, at::Tensor, Opt> paged_decode_attn(const at::Tensor& q, cons
 // -> (status, out like q, selected int32 [B, Hk, budget])
 std::tuple<int64_t, at::Tensor, at::Tensor> paged_sparse_decode_attn(
     const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& summary,
-    const at::Tensor& summary_scale, const at::Tensor& table, const at::Tensor& lens, int64_t budget, int64_t sink,
+    const at::Tensor& summary_scale, const at::Tensor& table_, const at::Tensor& lens_, int64_t budget, int64_t sink,
     int64_t recent, double scaling, double k_scale, double v_scale) {
   const int dev = q.get_device();
+  const at::Tensor table = as_int32(table_), lens = as_int32(lens_);
   const bd_tensor dq = desc_row(q, dev), dk = desc(k_cache, dev), dv = desc(v_cache, dev), ds = desc(summary, dev),
                   dss = desc(summary_scale, dev), dt = desc(table, dev), dl = desc(lens, dev);
   if (summary.dim() != 4) return {BD_ERR_SHAPE, at::Tensor(), at::Tensor()};

@@ -22,12 +22,6 @@ import torch
 from . import _native as N
 
 
-def _int32(t, name):
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name} must be a tensor")
-    return t if t.dtype == torch.int32 else t.to(torch.int32)
-
-
 def _pair(a, b, names):
     if (a is None) != (b is None):
         raise ValueError(f"{names} go together")
@@ -55,12 +49,8 @@ def paged_append(k, v, k_cache, v_cache, block_table, context_lens, *, q=None, c
     past the block table or past the rows of cos, or an entry that names no page) are not written;
     their query rows come back as zeros.
     """
-    N.require_cuda(k, v, k_cache, v_cache, block_table, context_lens, q, cos, sin, cu_seqlens, summary, summary_scale)
     _pair(cos, sin, "cos and sin")
     _pair(summary, summary_scale, "summary and summary_scale")
-    block_table, context_lens = _int32(block_table, "block_table"), _int32(context_lens, "context_lens")
-    if cu_seqlens is not None:
-        cu_seqlens = _int32(cu_seqlens, "cu_seqlens")
     rc, q_out = N.glue().paged_append(k, v, k_cache, v_cache, block_table, context_lens, q, cos, sin, interleaved,
                                       cu_seqlens, k_scale, v_scale, summary, summary_scale)
     if rc:
@@ -75,9 +65,8 @@ def paged_block_summary(k_cache, block_table, context_lens, summary, summary_sca
     int8 codes rint(x / s), s = max|x| / 127. ``paged_append`` keeps them page by page; this rebuilds
     them for pages that came from elsewhere (a copied prefix, a swapped-in sequence).
     """
-    N.require_cuda(k_cache, block_table, context_lens, summary, summary_scale)
-    rc = N.glue().paged_block_summary(k_cache, _int32(block_table, "block_table"),
-                                      _int32(context_lens, "context_lens"), k_scale, summary, summary_scale)
+    rc = N.glue().paged_block_summary(k_cache, block_table,
+                                      context_lens, k_scale, summary, summary_scale)
     if rc:
         N.check(rc, "bd_paged_block_summary")
 
@@ -94,12 +83,11 @@ def paged_select_blocks(q, summary, summary_scale, block_table, context_lens, bu
     The ``sink_blocks`` first and ``recent_blocks`` last pages, then those with the largest bound of q.k over
     the page (8-bit q and summaries, the largest over the KV head's query heads, the lower page on ties).
     """
-    N.require_cuda(q, summary, summary_scale, block_table, context_lens)
     _check_row(q)
     if budget < 1:
         raise ValueError("budget must be at least one page")
-    rc, selected = N.glue().paged_select(q, summary, summary_scale, _int32(block_table, "block_table"),
-                                         _int32(context_lens, "context_lens"), block_size, budget, sink_blocks,
+    rc, selected = N.glue().paged_select(q, summary, summary_scale, block_table,
+                                         context_lens, block_size, budget, sink_blocks,
                                          recent_blocks)
     if rc:
         N.check(rc, "bd_paged_select")
@@ -116,12 +104,9 @@ def paged_decode_attn(q, k_cache, v_cache, block_table, context_lens, scaling, *
     natural log of the softmax denominator, f32 [B, H_q] (-inf without a token), to join parts of a
     sequence held elsewhere.
     """
-    N.require_cuda(q, k_cache, v_cache, block_table, context_lens, selected)
     _check_row(q)
-    if selected is not None:
-        selected = _int32(selected, "selected")
-    rc, out, lse = N.glue().paged_decode_attn(q, k_cache, v_cache, _int32(block_table, "block_table"),
-                                              _int32(context_lens, "context_lens"), selected, scaling, k_scale,
+    rc, out, lse = N.glue().paged_decode_attn(q, k_cache, v_cache, block_table,
+                                              context_lens, selected, scaling, k_scale,
                                               v_scale, return_lse)
     if rc:
         N.check(rc, "bd_paged_decode_attn")
@@ -133,13 +118,12 @@ def paged_sparse_decode_attn(q, k_cache, v_cache, summary, summary_scale, block_
                              return_selected=False):
     """``paged_decode_attn`` over the ``budget_blocks`` pages that ``paged_select_blocks`` chooses for each
     KV head; with ``return_selected`` (out, selected)."""
-    N.require_cuda(q, k_cache, v_cache, summary, summary_scale, block_table, context_lens)
     _check_row(q)
     if budget_blocks < 1:
         raise ValueError("budget_blocks must be at least one page")
     rc, out, selected = N.glue().paged_sparse_decode_attn(
-        q, k_cache, v_cache, summary, summary_scale, _int32(block_table, "block_table"),
-        _int32(context_lens, "context_lens"), budget_blocks, sink_blocks, recent_blocks, scaling, k_scale, v_scale)
+        q, k_cache, v_cache, summary, summary_scale, block_table,
+        context_lens, budget_blocks, sink_blocks, recent_blocks, scaling, k_scale, v_scale)
     if rc:
         N.check(rc, "bd_paged_sparse_decode_attn")
     return (out, selected) if return_selected else out
