@@ -401,6 +401,10 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
   if (lane == 0) mbar_fence_init();
   __syncwarp();
 
+  // a kernel that waits for this one finds what this one waits for done as well, whichever way it ends
+  auto leave = [&]() {
+    if (p.after_select) griddep_wait();
+  };
   Place in;           // the next unit to bring in
   int left;           // slots of this warp's share that are not worked off
   bool one_row, row_begins = true;
@@ -412,6 +416,7 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
       const int nheads = min(NH, p.G - chunk * NH);
       for (int e = threadIdx.x; e < nheads * (D / 4); e += T::WARPS * 32)
         Sum4::none().write(p, b, hk * p.G + chunk * NH + e / (D / 4), e % (D / 4));
+      leave();
       return;
     }
     in.within(p, b, len, (blockIdx.x - b * per) * slots);
@@ -425,7 +430,10 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     int first = sh.begin(w), end = sh.begin(w + 1);
     const int cta_first = sh.cta(blockIdx.x), cta_end = sh.cta(blockIdx.x + 1);
     if (p.starts && first == end && lane == 0) p.starts[w] = ShareStart{0, 0, 0, 0, 0, list.total, {0, 0}};
-    if (cta_end == cta_first) return;
+    if (cta_end == cta_first) {
+      leave();
+      return;
+    }
     in.find(p, list, groups, cta_first, lane);
     // with all of the CTA's share in one row that is cut its warps' parts are added up here, and one goes out
     one_row = in.s + (cta_end - cta_first) <= in.slots && in.slots > sh.whole;
@@ -434,7 +442,10 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     if (one_row) {
       in.s += first - cta_first;
     } else {
-      if (first == end) return;
+      if (first == end) {
+        leave();
+        return;
+      }
       if (end < list.total) {
         Place to;
         to.find(p, list, groups, end, lane);
@@ -447,7 +458,10 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     if (!one_row) {
       first += in.snap(sh.whole);
       end = snapped;
-      if (first >= end) return;
+      if (first >= end) {
+        leave();
+        return;
+      }
       if (in.s == in.slots) in.next_row(p);
     }
     left = end - first;
@@ -475,7 +489,7 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     }
   };
   to_unit();
-  if (p.after_select) griddep_wait();
+  leave();  // the chosen pages are there
 
   auto issue = [&](int stage) {
     if (to_issue == 0) return;

@@ -249,6 +249,41 @@ def test_decode_attn(cuda, Hq, Hk, D, block, qdt, cdt):
     check_attention(*x, cuda)
 
 
+# How the work is shared out depends on how many rows there are and how long they and the block table are:
+# a CTA a row, cut rows joined row by row (a head a CTA, eight heads a CTA), many rows joined by
+# what cuts them, running sums of one sequence a lane, of one and of several a group.
+SHARED_OUT = {
+    "a CTA a row": lambda g: ([700, 0, 333, 1, 90, 1024] * 3, 2),
+    "few rows, one CTA a head": lambda g: ([4000, 0, 9, 2500], 2),
+    "eight heads a CTA": lambda g: (torch.randint(0, 1500, (40,), generator=g).tolist() + [3001], 2),
+    "many rows, long and short": lambda g: (torch.randint(0, 90, (310,), generator=g).tolist() + [2777, 0, 1500], 2),
+    "many rows alike": lambda g: ([100] * 160, 4),
+    "several sequences a group": lambda g: (torch.randint(0, 20, (1500,), generator=g).tolist() + [600], 1),
+    "nothing": lambda g: ([0] * 50, 2),
+    "one among many empty": lambda g: ([0] * 1200 + [555] + [0] * 30, 1),
+}
+
+
+@pytest.mark.parametrize("heads,D,qdt,cdt", [(4, 128, BF16, BF16), (7, 128, BF16, FP8), (1, 64, F16, F16),
+                                             (16, 64, BF16, FP8), (8, 256, F16, FP8), (11, 128, F16, F16),
+                                             (2, 256, BF16, BF16), (9, 64, BF16, BF16)])
+@pytest.mark.parametrize("how", list(SHARED_OUT))
+def test_decode_attn_shared_out(cuda, how, heads, D, qdt, cdt):
+    lens, Hk = SHARED_OUT[how](gen(len(how)))
+    block = 16 if heads % 2 else 8
+    x = attention_inputs(lens, heads * Hk, Hk, D, block, qdt, cdt, heads + D)
+    check_attention(*x, cuda)
+
+
+@pytest.mark.parametrize("cdt", [BF16, FP8])
+def test_decode_attn_wide_table(cuda, cdt):
+    """A block table far wider than the lengths: what is planned from it must not show in the result."""
+    q, kc, vc, table, lens, ks, vs = attention_inputs([300, 20, 0, 1], 8, 2, 128, 16, BF16, cdt, 8)
+    wide = torch.full((4, 70000), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    check_attention(q, kc, vc, wide, lens, ks, vs, cuda)
+
+
 @pytest.mark.parametrize("cdt", [BF16, F16, FP8])
 def test_decode_attn_token_major_pages_and_4d_query(cuda, cdt):
     qdt = F16 if cdt == F16 else BF16
@@ -356,15 +391,18 @@ def test_select_and_sparse(cuda, Hq, Hk, D, block, budget, sink, recent, cdt):
     assert torch.equal(bits(out), bits(direct))
 
 
-@pytest.mark.parametrize("lens,budget", [([70000, 16, 33000], 64), ([5000] * 40, 17), ([131072], 1)])
-def test_select_long(cuda, lens, budget):
+@pytest.mark.parametrize("lens,budget,spread", [
+    ([70000, 16, 33000], 64, 3), ([5000] * 40, 17, 3), ([131072], 1, 3),
+    ([150000], 3000, 1),        # past the pages that registers hold, the threshold among equal scores
+    ([140000, 131072], 200, 10 ** 6), ([33000, 8192 * 16 + 1, 600 * 16], 513, 10 ** 6), ([2048 * 16 + 5], 2048, 2)])
+def test_select_long(cuda, lens, budget, spread):
     """Many pages and few sequences, many sequences, a budget of one; summaries drawn directly, with
-    many equal scores."""
+    many equal scores or (a large spread of the scales) hardly any."""
     g = gen(budget)
     Hq, Hk, D, block = 8, 2, 64, 16
     table, nb = table_for(lens, block, g)
     code = torch.randint(-4, 5, (nb, Hk, 2, D), generator=g).to(torch.int8)
-    scale = torch.randint(1, 4, (nb, Hk), generator=g).float()
+    scale = torch.randint(1, spread + 1, (nb, Hk), generator=g).float()
     q = torch.randint(-2, 3, (len(lens), Hq, D), generator=g).bfloat16()
     clen = torch.tensor(lens, dtype=torch.int32)
     got = paged.paged_select_blocks(q.to(cuda), code.to(cuda), scale.to(cuda), table.to(cuda), clen.to(cuda), budget,
@@ -382,6 +420,24 @@ def test_select_long(cuda, lens, budget):
             score[n - 1:] = math.inf
             want = score.sort(stable=True, dim=0, descending=True)[1][:budget].sort()[0].int()
             assert torch.equal(got[b, h, :want.numel()], want) and (got[b, h, want.numel():] == -1).all()
+
+
+def test_select_equal_scores_and_missing_pages(cuda):
+    """All scores equal (the lowest pages), all zero, negative ones, and entries of no page, which come last."""
+    Hq, Hk, D, block, n = 4, 1, 64, 16, 3000
+    table = torch.arange(n, dtype=torch.int32)[None].clone()
+    lens = torch.tensor([n * block], dtype=torch.int32)
+    q = torch.ones(1, Hq, D).bfloat16()
+    for value, scale in ((3, 1.0), (0, 0.0), (-5, 2.0)):
+        code = torch.full((n, Hk, 2, D), value, dtype=torch.int8)
+        s = torch.full((n, Hk), scale)
+        got = paged.paged_select_blocks(q.to(cuda), code.to(cuda), s.to(cuda), table.to(cuda), lens.to(cuda), 100, block,
+                                        sink_blocks=2, recent_blocks=3).cpu()
+        assert torch.equal(got[0, 0], torch.tensor(list(range(97)) + [n - 3, n - 2, n - 1], dtype=torch.int32))
+    table[0, 10:2990] = -1
+    got = paged.paged_select_blocks(q.to(cuda), code.to(cuda), s.to(cuda), table.to(cuda), lens.to(cuda), 30, block,
+                                    recent_blocks=1).cpu()
+    assert torch.equal(got[0, 0], torch.tensor(list(range(20)) + list(range(2990, 3000)), dtype=torch.int32))
 
 
 def test_selected_lists_of_the_caller(cuda):
