@@ -1,5 +1,6 @@
 // Host-side helpers shared by every entry point: error reporting and descriptor checks.
 #include "common.cuh"
+#include "paged.cuh"
 
 #include <cudaTypedefs.h>
 

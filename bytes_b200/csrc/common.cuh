@@ -42,7 +42,6 @@ long long kivi_wait_timeouts();
 long long pq_wait_timeouts();
 long long merge_wait_timeouts();
 long long exchange_wait_timeouts();
-long long paged_wait_timeouts();
 // Tiled TMA tensor map of rank 3..5 (dims[0] contiguous; strides in bytes of dims 1..rank-1),
 // encoded through the driver entry point fetched from the runtime. False if unavailable or
 // rejected.

@@ -32,6 +32,9 @@ __device__ __forceinline__ int paged_block(const PagedGeometry& g, int b, int j)
 int check_paged(const bd_tensor* k_cache, const bd_tensor* v_cache, const bd_tensor* block_table,
                 const bd_tensor* context_lens, PagedGeometry* g);
 
+// Host read of the paged kernels' counter of device waits that ran past their limit.
+long long paged_wait_timeouts();
+
 inline bool is_float16_32(int dt) { return dt == BD_BF16 || dt == BD_F16 || dt == BD_F32; }
 
 // Runs the body of an extern "C" entry point: nothing thrown in it (an allocation that fails
