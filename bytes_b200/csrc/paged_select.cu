@@ -12,7 +12,6 @@
 #include "decode_shared.cuh"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace bd {
 
@@ -432,37 +431,54 @@ size_t select_bytes(const SelectParams& p) {
   return size_t(p.g.B) * p.g.Hk * ((size_t(p.g.wide) + 3) & ~size_t(3)) * sizeof(unsigned) + 256;
 }
 
-// CTAs of a row: as many as fill the GPU twice, up to the eight of a portable cluster.
+// CTAs of a row: up to 16 (8 where the device has no room for a cluster of 16), while the rows' CTAs are no more
+// than SMs and every warp has pages (one row of 8192 pages and four KV heads: 21.5, 16.7, 13.7 us for 4, 8, 16).
 int launch_select(const SelectParams& p, cudaStream_t st) {
   const int D = p.g.D;
   const size_t smem = size_t((p.G + 7) & ~7) * (2 * D + sizeof(float));
   const bool tiles = (D == 64 || D == 128 || D == 256) &&
                      !((reinterpret_cast<uintptr_t>(p.code) | size_t(p.c_sb) | size_t(p.c_sh)) & 15);
-  auto of = [&](auto hold) {
-    constexpr int H = decltype(hold)::value;
-    return !tiles ? paged_select_kernel<0, H> : D == 64 ? paged_select_kernel<64, H>
-           : D == 128 ? paged_select_kernel<128, H> : paged_select_kernel<256, H>;
-  };
-  auto kern = p.g.wide <= 4 * kSelThreads ? of(std::integral_constant<int, 4>()) : of(std::integral_constant<int, 16>());
+  const int kind = !tiles ? 0 : D == 64 ? 1 : D == 128 ? 2 : 3, hold = p.g.wide > 4 * kSelThreads;
+  using Kernel = void (*)(SelectParams);
+  static const Kernel kernels[2][4] = {
+      {paged_select_kernel<0, 4>, paged_select_kernel<64, 4>, paged_select_kernel<128, 4>, paged_select_kernel<256, 4>},
+      {paged_select_kernel<0, 16>, paged_select_kernel<64, 16>, paged_select_kernel<128, 16>, paged_select_kernel<256, 16>}};
+  const Kernel kern = kernels[hold][kind];
   int rc;
   if (smem > 40 * 1024 && (rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
                                            "cudaFuncSetAttribute(paged_select_kernel)")))
     return rc;
-  const int64_t rows = int64_t(p.g.B) * p.g.Hk;
-  unsigned ctas = 1;
-  while (ctas < 8 && rows * ctas * 2 <= 2 * num_sms() && int64_t(ctas) * kSelWarps * 16 < p.g.wide) ctas *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, p.g.Hk, p.g.B);
   cfg.blockDim = dim3(kSelThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  const int64_t rows = int64_t(p.g.B) * p.g.Hk;
+  unsigned ctas = 1;
+  while (ctas < 16 && rows * ctas <= num_sms() && int64_t(ctas) * kSelWarps * 16 < p.g.wide) ctas *= 2;
+  if (ctas == 16) {
+    static signed char room[64][2][4] = {};  // 1: a cluster of 16 fits this device, -1: it does not
+    int dev = 0;
+    cudaGetDevice(&dev);
+    signed char& r = room[dev & 63][hold][kind];
+    if (r == 0) {
+      int n = 0;
+      cfg.gridDim = dim3(16);
+      attr[0].val.clusterDim.x = 16;
+      r = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                  cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0
+              ? 1 : -1;
+      (void)cudaGetLastError();
+    }
+    if (r < 0) ctas = 8;
+  }
+  cfg.gridDim = dim3(ctas, p.g.Hk, p.g.B);
+  attr[0].val.clusterDim.x = ctas;
   return cuda_check(cudaLaunchKernelEx(&cfg, kern, p), "paged_select_kernel launch");
 }
 

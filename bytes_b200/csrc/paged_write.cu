@@ -203,10 +203,10 @@ template <> struct Eight<__nv_fp8_e4m3> {
 // nothing turns. A head has D / 16 items, a power of two up to 16, so a lane has the same channels of
 // every head it visits and holds their eight cosines and sines in registers. A warp takes one token's
 // items it, it + 1, ... `each` times; the heads run over queries, keys and values.
-constexpr int kAppendWarps = 8;
+constexpr int kAppendWarps = 4;
 
 template <typename TI, typename TC>
-__global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 7) paged_append_kernel(const AppendParams p) {
   const int64_t w = int64_t(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, t = int(w / p.parts), part = int(w % p.parts);
   if (t >= p.T) return;
