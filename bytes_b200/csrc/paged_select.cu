@@ -77,16 +77,14 @@ __device__ __forceinline__ void mma_s8(int* d, uint32_t a0, uint32_t a1, uint32_
 // bytes of a row, loaded from global memory as such: no shared memory but for the queries.
 //
 // D = 0: any head dim, any alignment of the summaries, a lane a page.
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
-
-template <int D>
+template <int D, int THREADS>
 __device__ __forceinline__ void score_pages(const SelectParams& p, int b, int hk, int n, unsigned* keys, int8_t* q8,
                                             int rank, int ctas, int warp, int lane) {
+  constexpr int WARPS = THREADS / 32;
   const int heads = (p.G + 7) & ~7;
   float* q_scale = reinterpret_cast<float*>(q8 + heads * 2 * D);
-  const int g = lane >> 2, tq = lane & 3, step = ctas * kSelWarps * 16;
-  int j0 = (rank * kSelWarps + warp) * 16;
+  const int g = lane >> 2, tq = lane & 3, step = ctas * WARPS * 16;
+  int j0 = (rank * WARPS + warp) * 16;
   // rows g and g + 8 of the tile; the first tile's loads are under way while the queries are made
   // (and a tile's page numbers while the one before it is)
   int page[2], next[2];
@@ -110,7 +108,7 @@ __device__ __forceinline__ void score_pages(const SelectParams& p, int b, int hk
   load_next(j0);
   load_rows();
   load_next(j0 + step);
-  for (int h = warp; h < heads; h += kSelWarps) {
+  for (int h = warp; h < heads; h += WARPS) {
     if (h < p.G) {
       const float s = quantize_query(p, b, hk * p.G + h, q8 + h * 2 * D, lane);
       if (lane == 0) q_scale[h] = s;
@@ -158,17 +156,17 @@ __device__ __forceinline__ void score_pages(const SelectParams& p, int b, int hk
   }
 }
 
-template <>
-__device__ __forceinline__ void score_pages<0>(const SelectParams& p, int b, int hk, int n, unsigned* keys, int8_t* q8,
-                                               int rank, int ctas, int warp, int lane) {
+template <int THREADS>
+__device__ __forceinline__ void score_pages_any(const SelectParams& p, int b, int hk, int n, unsigned* keys, int8_t* q8,
+                                                int rank, int ctas, int warp, int lane) {
   const int D = p.g.D;
   float* q_scale = reinterpret_cast<float*>(q8 + ((p.G + 7) & ~7) * 2 * D);
-  for (int h = warp; h < p.G; h += kSelWarps) {
+  for (int h = warp; h < p.G; h += (THREADS / 32)) {
     const float s = quantize_query(p, b, hk * p.G + h, q8 + h * 2 * D, lane);
     if (lane == 0) q_scale[h] = s;
   }
   __syncthreads();
-  for (int j = rank * kSelThreads + warp * 32 + lane; j < n; j += ctas * kSelThreads) {
+  for (int j = rank * THREADS + warp * 32 + lane; j < n; j += ctas * THREADS) {
     unsigned key = 0xffffffffu;
     if (j >= p.sink && j < n - p.recent) {
       const int page = paged_block(p.g, b, j);
@@ -189,18 +187,19 @@ __device__ __forceinline__ void score_pages<0>(const SelectParams& p, int b, int
 }
 
 // The largest threshold that `want` of a row's n keys reach, then the pages: those above it, and the lowest of
-// those at it. Thread t holds keys [t each, (t + 1) each), each <= kHold, in registers (pages past 512
-// kHold are read again from L2 each time). The threshold is found eight bits at a time by a histogram, which starts at the
+// those at it. Thread t holds keys [t each, (t + 1) each), each <= kHold, in registers (pages past
+// THREADS kHold are read again from L2 each time). The threshold is found eight bits at a time by a histogram, which starts at the
 // first bit in which the keys differ (scores share their leading bits, and its counters would all be the
-// same few; the `forced` pages' keys, which differ from all in all bits, are left out). Of up to 512 keys that are left each thread goes on with one; up to 32 are ranked by a warp.
-template <int kHold>
+// same few; the `forced` pages' keys, which differ from all in all bits, are left out). Of up to THREADS keys that are left each thread goes on with one; up to 32 are ranked by a warp.
+template <int kHold, int THREADS>
 __device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int want, int forced, int* out, int64_t o_si) {
-  __shared__ unsigned left[kSelThreads], bound[2][kSelWarps];
-  __shared__ int hist[256], sums[kSelWarps];
+  constexpr int WARPS = THREADS / 32;
+  __shared__ unsigned left[THREADS], bound[2][WARPS];
+  __shared__ int hist[256], sums[WARPS];
   __shared__ int n_left;
   __shared__ unsigned found[3];  // bin or threshold, keys above, keys left
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int each = min(kHold, ((n + kSelThreads - 1) / kSelThreads + 3) & ~3), held = each * kSelThreads;
+  const int each = min(kHold, ((n + THREADS - 1) / THREADS + 3) & ~3), held = each * THREADS;
   unsigned key[kHold], lo = 0xffffffffu, hi = 0;
   auto scored = [](unsigned k) { return k - 1u < 0xfffffffeu; };  // neither 0 nor forced
 #pragma unroll
@@ -216,7 +215,7 @@ __device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int wa
     for (int e = 0; e < 4; ++e)
       if (scored(key[i + e])) hi = max(hi, key[i + e]), lo = min(lo, key[i + e]);
   }
-  for (int j = held + t; j < n; j += kSelThreads) {
+  for (int j = held + t; j < n; j += THREADS) {
     const unsigned k = __ldcg(keys + j);
     if (scored(k)) hi = max(hi, k), lo = min(lo, k);
   }
@@ -226,8 +225,8 @@ __device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int wa
   if (t < 256) hist[t] = 0;
   if (t == 0) n_left = 0;
   __syncthreads();
-  hi = __reduce_max_sync(0xffffffffu, bound[0][lane % kSelWarps]);
-  lo = __reduce_min_sync(0xffffffffu, bound[1][lane % kSelWarps]);
+  hi = __reduce_max_sync(0xffffffffu, bound[0][lane % WARPS]);
+  lo = __reduce_min_sync(0xffffffffu, bound[1][lane % WARPS]);
   // the threshold's known leading bits, how many are not known, the keys that share them, those above
   int low = hi == lo ? 0 : 32 - __clz(hi ^ lo);
   unsigned thr = low == 32 ? 0u : hi >> low << low;
@@ -249,14 +248,14 @@ __device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int wa
       for (int e = 0; e < 4; ++e)
         if (among(key[i + e])) f(key[i + e]);
     }
-    for (int j = held + t; j < n; j += kSelThreads) {
+    for (int j = held + t; j < n; j += THREADS) {
       const unsigned k = __ldcg(keys + j);
       if (among(k)) f(k);
     }
   };
 #pragma unroll 1
   while (low > 0) {
-    if (rest <= 32 || (!one && rest <= kSelThreads)) {
+    if (rest <= 32 || (!one && rest <= THREADS)) {
       each_key([&](unsigned k) { left[atomicAdd(&n_left, 1)] = k; });
       __syncthreads();
       if (rest <= 32) {  // their rank: need of them reach the threshold
@@ -327,7 +326,7 @@ __device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int wa
   }
   if (lane == 31) sums[warp] = sum;
   __syncthreads();
-  const int y = lane < kSelWarps ? sums[lane] : 0;
+  const int y = lane < WARPS ? sums[lane] : 0;
   const int before = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0) + sum - count;
   int up = before & 0xffff, at = before >> 16;
 #pragma unroll
@@ -342,17 +341,17 @@ __device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int wa
     }
   }
   if (n <= held) return;
-  // the pages that are not held, 512 at a time
+  // the pages that are not held, THREADS at a time
   const int all = __reduce_add_sync(0xffffffffu, y);
   int up0 = all & 0xffff, at0 = all >> 16;
 #pragma unroll 1
-  for (int j0 = held; j0 < n; j0 += kSelThreads) {
+  for (int j0 = held; j0 < n; j0 += THREADS) {
     const unsigned k = j0 + t < n ? __ldcg(keys + j0 + t) : 0;
     const unsigned ups = __ballot_sync(0xffffffffu, k > thr), ats = __ballot_sync(0xffffffffu, k == thr);
     __syncthreads();
     if (lane == 0) sums[warp] = __popc(ups) + (__popc(ats) << 16);
     __syncthreads();
-    const int z = lane < kSelWarps ? sums[lane] : 0;
+    const int z = lane < WARPS ? sums[lane] : 0;
     const int b4 = __reduce_add_sync(0xffffffffu, lane < warp ? z : 0), sum_all = __reduce_add_sync(0xffffffffu, z);
     const unsigned below = (1u << lane) - 1u;
     const int u = up0 + (b4 & 0xffff) + __popc(ups & below), q = at0 + (b4 >> 16) + __popc(ats & below);
@@ -362,8 +361,8 @@ __device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int wa
   }
 }
 
-template <int D, int HOLD>
-__global__ void __launch_bounds__(kSelThreads, D == 256 ? 1 : 2) paged_select_kernel(const SelectParams p) {
+template <int D, int HOLD, int THREADS>
+__global__ void __launch_bounds__(THREADS, (D == 256 ? 512 : 1024) / THREADS) paged_select_kernel(const SelectParams p) {
   extern __shared__ __align__(16) int8_t q8[];  // [heads, a multiple of 8][2D], then their scales
   griddep_launch_dependents();
   const int rank = blockIdx.x, ctas = gridDim.x, hk = blockIdx.y, b = blockIdx.z;
@@ -371,21 +370,22 @@ __global__ void __launch_bounds__(kSelThreads, D == 256 ? 1 : 2) paged_select_ke
   const int n = int((int64_t(paged_len(p.g, b)) + p.g.block - 1) / p.g.block), want = min(n, p.budget);
   int* out = p.selected + b * p.o_sb + hk * p.o_sh;
   if (rank == 0)
-    for (int i = want + t; i < p.budget; i += kSelThreads) out[i * p.o_si] = -1;
+    for (int i = want + t; i < p.budget; i += THREADS) out[i * p.o_si] = -1;
   if (n <= p.budget) {  // all of them
     if (rank == 0)
-      for (int i = t; i < n; i += kSelThreads) out[i * p.o_si] = i;
+      for (int i = t; i < n; i += THREADS) out[i * p.o_si] = i;
     return;
   }
   unsigned* keys = p.keys + (int64_t(b) * p.g.Hk + hk) * p.pitch;
-  score_pages<D>(p, b, hk, n, keys, q8, rank, ctas, t >> 5, t & 31);
+  if constexpr (D == 0) score_pages_any<THREADS>(p, b, hk, n, keys, q8, rank, ctas, t >> 5, t & 31);
+  else score_pages<D, THREADS>(p, b, hk, n, keys, q8, rank, ctas, t >> 5, t & 31);
   if (ctas > 1) {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
     if (rank) return;
   } else {
     __syncthreads();
   }
-  choose_pages<HOLD>(keys, n, want, p.sink + p.recent, out, p.o_si);
+  choose_pages<HOLD, THREADS>(keys, n, want, p.sink + p.recent, out, p.o_si);
 }
 
 int check_select(const bd_tensor* q, const bd_tensor* summary, const bd_tensor* summary_scale,
@@ -438,18 +438,25 @@ int launch_select(const SelectParams& p, cudaStream_t st) {
   const size_t smem = size_t((p.G + 7) & ~7) * (2 * D + sizeof(float));
   const bool tiles = (D == 64 || D == 128 || D == 256) &&
                      !((reinterpret_cast<uintptr_t>(p.code) | size_t(p.c_sb) | size_t(p.c_sh)) & 15);
-  const int kind = !tiles ? 0 : D == 64 ? 1 : D == 128 ? 2 : 3, hold = p.g.wide > 4 * kSelThreads;
+  // rows of up to 1024 pages: half the threads, twice the CTAs (64 sequences of 2000 to 16000 tokens, 8 KV heads:
+  // 21.7 us against 26.1; one row of 8192: 22.3 against 13.7)
+  const int kind = !tiles ? 0 : D == 64 ? 1 : D == 128 ? 2 : 3, size = p.g.wide <= 1024 ? 0 : p.g.wide <= 2048 ? 1 : 2;
+  const int threads = size == 0 ? 256 : 512;
   using Kernel = void (*)(SelectParams);
-  static const Kernel kernels[2][4] = {
-      {paged_select_kernel<0, 4>, paged_select_kernel<64, 4>, paged_select_kernel<128, 4>, paged_select_kernel<256, 4>},
-      {paged_select_kernel<0, 16>, paged_select_kernel<64, 16>, paged_select_kernel<128, 16>, paged_select_kernel<256, 16>}};
-  const Kernel kern = kernels[hold][kind];
+  static const Kernel kernels[3][4] = {
+      {paged_select_kernel<0, 4, 256>, paged_select_kernel<64, 4, 256>, paged_select_kernel<128, 4, 256>,
+       paged_select_kernel<256, 4, 256>},
+      {paged_select_kernel<0, 4, 512>, paged_select_kernel<64, 4, 512>, paged_select_kernel<128, 4, 512>,
+       paged_select_kernel<256, 4, 512>},
+      {paged_select_kernel<0, 16, 512>, paged_select_kernel<64, 16, 512>, paged_select_kernel<128, 16, 512>,
+       paged_select_kernel<256, 16, 512>}};
+  const Kernel kern = kernels[size][kind];
   int rc;
   if (smem > 40 * 1024 && (rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
                                            "cudaFuncSetAttribute(paged_select_kernel)")))
     return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kSelThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -460,12 +467,12 @@ int launch_select(const SelectParams& p, cudaStream_t st) {
   cfg.numAttrs = 1;
   const int64_t rows = int64_t(p.g.B) * p.g.Hk;
   unsigned ctas = 1;
-  while (ctas < 16 && rows * ctas <= num_sms() && int64_t(ctas) * kSelWarps * 16 < p.g.wide) ctas *= 2;
+  while (ctas < 16 && rows * ctas * threads <= 512 * num_sms() && int64_t(ctas) * (threads / 2) < p.g.wide) ctas *= 2;
   if (ctas == 16) {
-    static signed char room[64][2][4] = {};  // 1: a cluster of 16 fits this device, -1: it does not
+    static signed char room[64][3][4] = {};  // 1: a cluster of 16 fits this device, -1: it does not
     int dev = 0;
     cudaGetDevice(&dev);
-    signed char& r = room[dev & 63][hold][kind];
+    signed char& r = room[dev & 63][size][kind];
     if (r == 0) {
       int n = 0;
       cfg.gridDim = dim3(16);
