@@ -167,7 +167,12 @@ struct TileShape {
   static constexpr int SW = ROWB < 128 ? ROWB : 128;  // bytes of a row in one slab (the swizzle's span)
   static constexpr int SLABS = ROWB / SW;
   static constexpr int HALF = kUnit * ROWB;           // keys (or values) of a unit
-  static constexpr int WARPS = D == 256 ? (KIND == kFp8 ? 8 : 6) : NT == 2 ? 8 : D == 64 || KIND == kFp8 ? 16 : 12;
+  // As many warps as keep their sums in registers and 4 units or more each in flight. Heads 9 to 16 of a KV head
+  // take a second n of the products (NT 2). 32 heads over 2, 300 MB of cache, us with this, with fewer, with more:
+  // D 64 57.6 (12 warps), 67.8 (8), 60.8 (16); fp8 87.4 (16), 96.5 (12); D 128 59.8 (8), 59.6 (10); fp8 74.0 (12), 81.6 (8).
+  // D 256 64.0 and fp8 75.9, against 93.0 and 90.9 as two chunks of 8 heads, which read the cache twice.
+  static constexpr int WARPS = KIND == kFp8 ? (D == 256 ? 8 : D == 128 && NT == 2 ? 12 : 16)
+                                            : (D == 256 ? 6 : D == 128 && NT == 2 ? 8 : D == 64 && NT == 1 ? 16 : 12);
   static constexpr int FIT = 200 * 1024 / (WARPS * HALF * 2);
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   static_assert(STAGES >= 2, "a unit in flight beside the one at hand");
@@ -1095,11 +1100,11 @@ auto with_shape(const AttnParams& p, F&& f) {
   constexpr std::integral_constant<int, 2> two{};
   if (p.g.D == 64) return p.heads == 16 ? kind(std::integral_constant<int, 64>(), two) : kind(std::integral_constant<int, 64>(), one);
   if (p.g.D == 128) return p.heads == 16 ? kind(std::integral_constant<int, 128>(), two) : kind(std::integral_constant<int, 128>(), one);
-  return kind(std::integral_constant<int, 256>(), one);
+  return p.heads == 16 ? kind(std::integral_constant<int, 256>(), two) : kind(std::integral_constant<int, 256>(), one);
 }
 
 void plan_tiles(AttnParams* p) {
-  p->heads = p->G > 8 && p->g.D <= 128 ? 16 : 8;
+  p->heads = p->G > 8 ? 16 : 8;
   p->chunks = (p->G + p->heads - 1) / p->heads;
   const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(num_sms(), most_slots(*p, p->chunks) / kMinSlots));
   const int warps = with_shape(*p, [](auto d, auto kind, auto nt) {

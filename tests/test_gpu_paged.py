@@ -266,7 +266,8 @@ SHARED_OUT = {
 
 @pytest.mark.parametrize("heads,D,qdt,cdt", [(4, 128, BF16, BF16), (7, 128, BF16, FP8), (1, 64, F16, F16),
                                              (16, 64, BF16, FP8), (8, 256, F16, FP8), (11, 128, F16, F16),
-                                             (2, 256, BF16, BF16), (9, 64, BF16, BF16)])
+                                             (2, 256, BF16, BF16), (9, 64, BF16, BF16), (16, 256, BF16, BF16),
+                                             (12, 256, BF16, FP8), (10, 256, F16, F16), (13, 128, BF16, FP8)])
 @pytest.mark.parametrize("how", list(SHARED_OUT))
 def test_decode_attn_shared_out(cuda, how, heads, D, qdt, cdt):
     lens, Hk = SHARED_OUT[how](gen(len(how)))
