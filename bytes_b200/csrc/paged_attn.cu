@@ -1110,18 +1110,24 @@ void plan_tiles(AttnParams* p) {
   const int warps = with_shape(*p, [](auto d, auto kind, auto nt) {
     return TileShape<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>::WARPS;
   });
-  // rows of few tokens (as far as the block table goes), no more of them than SMs: a CTA a row, and no join
+  // Rows of few tokens (as far as the block table goes), no more of them than SMs: a CTA a row, and no join. How many
+  // units of a warp are few depends on how many SMs the rows leave idle. 128 channels, us with it and without, by rows
+  // and units: 4 rows 8.6, 8.5 (3), 10.2, 8.5 (4); 16 rows 10.3, 11.7 (4), 11.3, 11.9 (5), 13.4, 12.4 (8); 40 rows 11.1,
+  // 12.9 (5), 13.3, 14.1 (8); 80 rows 15.3, 17.6 (10); 128 rows 25.0, 29.8 (10), 35.7, 40.5 (16), but of lengths from
+  // 1 to all of it 15.0, 13.7 (10), 20.7, 16.9 (16).
   const int64_t rows = int64_t(p->g.B) * p->g.Hk * p->chunks;
-  const int units = 2 * rows >= num_sms() ? 10 : 2;  // of a warp at most
+  const int units = 2 * rows >= num_sms() ? 10 : 10 * rows >= num_sms() ? 5 : 2;
   p->row_mode = rows <= num_sms() && most_slots(*p, p->chunks) <= rows * (units * warps + kRowCost);
   p->warps = int(p->row_mode ? rows : ctas) * warps;
   p->block_shift = 31 - __builtin_clz(unsigned(p->g.block));
 }
 
-// Many rows are joined by what cuts them (one CTA a share of the list), few by themselves.
+// Many rows are joined by what cuts them (one CTA a share of the list), others by themselves. 32 heads over 8, 128 channels,
+// us by cuts and by rows: 64 sequences of 33 to 8192 tokens 94.6, 74.4; 256 of 33 to 4000 171, 166; 296 of 2000 377, 385;
+// 512 of 33 to 2000 187, 206; 1024 of 100 86, 173. Two groups of heads at 256 channels: 64 of 33 to 4000 123, 92.
 bool join_by_cuts(const AttnParams& p) {
   const int most = p.g.D == 256 ? 4 : 8, groups = (std::min(p.heads, p.G) + most - 1) / most;
-  return int64_t(p.g.B) * p.g.Hk * p.chunks * groups > 4 * num_sms();
+  return int64_t(p.g.B) * p.g.Hk * p.chunks * groups > 14 * num_sms();
 }
 
 size_t tile_bytes(const AttnParams& p) {
@@ -1176,6 +1182,8 @@ int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor*
   if (p.starts)
     return launch_programmatic(paged_tile_join_cuts_kernel<D, T::WARPS>, dim3(ctas), dim3(kCutsThreads), 0, st, p,
                                "paged_tile_join_cuts_kernel launch");
+  // one head a CTA while that is four CTAs an SM or fewer (one sequence of 32768 tokens, 28 heads over 4: 19.1 us against
+  // 34.0; 64 sequences of 33 to 8192, 32 over 8: 81.2 against 74.4)
   if (rows * heads <= 4 * num_sms())
     return launch_programmatic(paged_tile_join_kernel<D, T::WARPS, 1>, dim3(p.g.Hk * p.chunks * heads, p.g.B),
                                dim3(kJoinThreads), 0, st, p, "paged_tile_join_kernel launch");

@@ -259,6 +259,9 @@ SHARED_OUT = {
     "many rows, long and short": lambda g: (torch.randint(0, 90, (310,), generator=g).tolist() + [2777, 0, 1500], 2),
     "many rows alike": lambda g: ([100] * 160, 4),
     "several sequences a group": lambda g: (torch.randint(0, 20, (1500,), generator=g).tolist() + [600], 1),
+    "by cuts, long and short": lambda g: (torch.randint(0, 90, (600,), generator=g).tolist() + [2777, 0, 1500], 4),
+    "by cuts, alike": lambda g: ([100] * 530, 4),
+    "by cuts, several sequences a group": lambda g: ([900] + torch.randint(0, 20, (2200,), generator=g).tolist(), 1),
     "nothing": lambda g: ([0] * 50, 2),
     "one among many empty": lambda g: ([0] * 1200 + [555] + [0] * 30, 1),
 }
