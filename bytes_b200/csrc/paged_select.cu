@@ -76,6 +76,10 @@ __device__ __forceinline__ void mma_s8(int* d, uint32_t a0, uint32_t a1, uint32_
 // heads). The order of the 2D numbers is free, so that a thread's operand registers are 16 contiguous
 // bytes of a row, loaded from global memory as such: no shared memory but for the queries.
 //
+// Bound by memory as it scores (2D + 4 bytes a page and head), then by the latency of the choice, some 6 us. 16
+// sequences of 2048 pages, 8 KV heads of 128 channels: 68 MB in 19 us, 64 pages chosen; half as many pages 13 us; one
+// sequence of 2048 pages 8.5 us, of 8192 pages (four KV heads) 13.
+//
 // D = 0: any head dim, any alignment of the summaries, a lane a page.
 template <int D, int THREADS>
 __device__ __forceinline__ void score_pages(const SelectParams& p, int b, int hk, int n, unsigned* keys, int8_t* q8,
@@ -188,9 +192,10 @@ __device__ __forceinline__ void score_pages_any(const SelectParams& p, int b, in
 
 // The largest threshold that `want` of a row's n keys reach, then the pages: those above it, and the lowest of
 // those at it. Thread t holds keys [t each, (t + 1) each), each <= kHold, in registers (pages past
-// THREADS kHold are read again from L2 each time). The threshold is found eight bits at a time by a histogram, which starts at the
-// first bit in which the keys differ (scores share their leading bits, and its counters would all be the
-// same few; the `forced` pages' keys, which differ from all in all bits, are left out). Of up to THREADS keys that are left each thread goes on with one; up to 32 are ranked by a warp.
+// THREADS kHold are read again from L2 each time). The threshold is found eight bits at a time by a histogram,
+// which starts at the first bit in which the keys differ (scores share their leading bits, and its counters
+// would all be the same few; the `forced` pages' keys, which differ from all in all bits, are left out). Of up
+// to THREADS keys that are left each thread goes on with one; up to 32 are ranked by a warp.
 template <int kHold, int THREADS>
 __device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int want, int forced, int* out, int64_t o_si) {
   constexpr int WARPS = THREADS / 32;
@@ -438,8 +443,9 @@ int launch_select(const SelectParams& p, cudaStream_t st) {
   const size_t smem = size_t((p.G + 7) & ~7) * (2 * D + sizeof(float));
   const bool tiles = (D == 64 || D == 128 || D == 256) &&
                      !((reinterpret_cast<uintptr_t>(p.code) | size_t(p.c_sb) | size_t(p.c_sh)) & 15);
-  // rows of up to 1024 pages: half the threads, twice the CTAs (64 sequences of 2000 to 16000 tokens, 8 KV heads:
-  // 21.7 us against 26.1; one row of 8192: 22.3 against 13.7)
+  // Rows of up to 1024 pages: half the threads, twice the CTAs (64 sequences of 1000 pages, 8 KV heads: 34.0 us
+  // against 40.0; 16 of 2048: 21.3 against 18.8). Up to 2048: four keys a thread in place of 16 (18.8 us against 19.7;
+  // 8192 pages with four, the others read again: 22.3 against 13.7).
   const int kind = !tiles ? 0 : D == 64 ? 1 : D == 128 ? 2 : 3, size = p.g.wide <= 1024 ? 0 : p.g.wide <= 2048 ? 1 : 2;
   const int threads = size == 0 ? 256 : 512;
   using Kernel = void (*)(SelectParams);

@@ -109,7 +109,8 @@ __device__ __forceinline__ void store_cache(void* base, int dt, int64_t off, flo
     store_as(base, dt, off, x);
 }
 
-// Any type, stride and head dim: one CTA per token, a thread a channel.
+// Any type, stride and head dim: one CTA per token, a thread a channel. For what the vector form cannot address: one
+// token 23.5 us against 2.6, 14991 tokens (32 query heads, 8 KV heads of 128 channels) 431 against 70.
 __global__ void __launch_bounds__(128) paged_append_generic_kernel(const AppendParams p) {
   const int t = blockIdx.x;
   const int2 place = place_of(p.g, p.cu, t);
@@ -203,6 +204,11 @@ template <> struct Eight<__nv_fp8_e4m3> {
 // nothing turns. A head has D / 16 items, a power of two up to 16, so a lane has the same channels of
 // every head it visits and holds their eight cosines and sines in registers. A warp takes one token's
 // items it, it + 1, ... `each` times; the heads run over queries, keys and values.
+//
+// Bound by memory: every number is read and written once, and 6 operations a rotated pair are nothing beside it.
+// 14991 tokens of 11 prompts (32 query heads, 8 KV heads of 128 channels, bf16): 371 MB in 70 us, 5.3 TB/s, 81 % of
+// what a copy reaches; a step of one token 2.6 us, of 128 tokens 3.2, a launch's own time. Four warps a CTA, seven CTAs
+// an SM: 72 registers hold two items' loads in flight and turned.
 constexpr int kAppendWarps = 4;
 
 template <typename TI, typename TC>
@@ -276,8 +282,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 7) paged_append_kernel(cons
   }
 }
 
-// Warps that the vector form spreads a call over before it gives each of them more items of its token:
-// about 16 an SM.
+// Warps that the vector form spreads a call over before it gives each of them more items of its token: about 16 an
+// SM. 128 tokens 3.2 us with 16, 3.6 with 4, 3.2 with 64; 500 tokens 5.0, 7.7, 6.3; 4000 tokens 18.0, 18.1, 19.4.
 int launch_append(AppendParams p, cudaStream_t st) {
   const int heads = 32 / (p.g.D >> 4), all = (p.q.H + 2 * p.k.H + heads - 1) / heads;
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(all, int64_t(16) * num_sms() / p.T));
@@ -359,7 +365,8 @@ __device__ __forceinline__ int8_t code_of(float x, float s, bool some) {
   return some ? int8_t(max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))))) : int8_t(0);
 }
 
-// Any type, stride and head dim: one warp per (page, KV head), a lane every 32nd channel.
+// Any type, stride and head dim: one warp per (page, KV head), a lane every 32nd channel. For what the vector form
+// cannot address (8 sequences of 30001 tokens, four KV heads of 128 channels: 92 us against 48).
 __global__ void __launch_bounds__(128) paged_summary_generic_kernel(const SummaryParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
@@ -414,6 +421,10 @@ template <> struct Pair<__half> {
 // (of this page, or the next one's first) in flight while one is worked off, and the page number after that
 // as well. At a page's end the row groups meet by shuffles; the first of them writes the minima, the
 // second the maxima.
+//
+// Bound by memory: the keys are read once, and of a page of 16 rows 1/15 as many bytes written. 8 sequences of 30001 to
+// 32768 tokens, four KV heads of 128 channels, bf16: 273 MB in 50 us, 5.4 TB/s, 83 % of what a copy reaches. Two
+// CTAs of 8 warps an SM, each with eight 16-byte loads a lane in flight, are 64 KB an SM.
 template <typename T, bool FP8, int LPR>
 __global__ void __launch_bounds__(256, 2) paged_summary_kernel(const SummaryParams p, int64_t pages) {
   using P = Pair<T>;
