@@ -721,6 +721,8 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
             pv[2 + j] = fast_exp2(c[j] - ref);
             lrow[nt][j] += pv[j] + pv[2 + j];
           }
+          // the weights as the matrix product takes them: rounded once to 16 bits (to 2^-9 of themselves, in f16 2^-12), an
+          // error that the output's own rounding to 16 bits covers; their sum is taken before
           if (KIND == kBf16) {
             pb[nt][0] = movmatrix_trans(pack_bf16x2(pv[0], pv[1]));
             pb[nt][1] = movmatrix_trans(pack_bf16x2(pv[2], pv[3]));

@@ -63,7 +63,8 @@ def paged_block_summary(k_cache, block_table, context_lens, summary, summary_sca
 
     Per page and KV head, over the page's tokens: channelwise minimum and maximum of k_scale * key as
     int8 codes rint(x / s), s = max|x| / 127. ``paged_append`` keeps them page by page; this rebuilds
-    them for pages that came from elsewhere (a copied prefix, a swapped-in sequence).
+    them for pages that came from elsewhere (a copied prefix, a swapped-in sequence). A page that several
+    sequences share is summarised once for each of them, so it should be full in all.
     """
     rc = N.glue().paged_block_summary(k_cache, block_table,
                                       context_lens, k_scale, summary, summary_scale)
