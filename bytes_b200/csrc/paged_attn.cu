@@ -34,7 +34,7 @@ struct AttnParams {
   float* part_o; float* part_m; float* part_l;  // [B*Hq][n_splits]([D]); m in log2 units
   // tile form: warps of the grid, its partials [2 * warps][heads]([D])
   int warps, heads, block_shift;
-  int row_mode;  // a CTA has a row, and nothing is joined
+  int row_mode;  // CTAs (a cluster of them) that have a row, which no kernel joins; 0: rows are shared out by the list
   int after_select;  // launched as a programmatic dependent of the choice of pages, which it waits for
   ShareStart* starts;  // one a warp, where paged_tile_join_cuts_kernel follows
   void* out; int out_dtype; int64_t o_sb, o_sh, o_sd;
@@ -387,6 +387,27 @@ struct Sum4 {
   }
 };
 
+// All threads of the cluster's CTAs; what they wrote to shared memory before is there after.
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
+// What CTA `rank` of the cluster holds at this CTA's shared address.
+__device__ __forceinline__ float2 cluster_float2(uint32_t at, int rank) {
+  float2 x;
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %2, %3;\n ld.shared::cluster.v2.f32 {%0, %1}, [a];\n}\n"
+               : "=f"(x.x), "=f"(x.y) : "r"(at), "r"(rank) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 cluster_float4(uint32_t at, int rank) {
+  float4 x;
+  asm volatile(
+      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %4, %5;\n ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n}\n"
+      : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at), "r"(rank) : "memory");
+  return x;
+}
+
 template <int D, int KIND, int NT>
 __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     paged_attn_tile_kernel(const AttnParams p, const __grid_constant__ CUtensorMap kmap,
@@ -420,21 +441,24 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
   Place in;           // the next unit to bring in
   int left;           // slots of this warp's share that are not worked off
   bool one_row, row_begins = true;
-  if (p.row_mode) {   // a CTA has a row
+  if (p.row_mode) {   // a cluster has a row
     one_row = true;
-    const int per = p.g.Hk * p.chunks, b = blockIdx.x / per, len = paged_len(p.g, b), slots = row_slots(p, len);
-    if (slots == 0) {
-      const int hc = blockIdx.x - b * per, hk = hc / p.chunks, chunk = hc - hk * p.chunks;
+    const int per = p.g.Hk * p.chunks, row = blockIdx.x / p.row_mode, rank = blockIdx.x - row * p.row_mode;
+    const int b = row / per, len = paged_len(p.g, b), slots = row_slots(p, len);
+    if (slots == 0) {  // (the same for all of the cluster's CTAs)
+      const int hc = row - b * per, hk = hc / p.chunks, chunk = hc - hk * p.chunks;
       const int nheads = min(NH, p.G - chunk * NH);
-      for (int e = threadIdx.x; e < nheads * (D / 4); e += T::WARPS * 32)
+      for (int e = threadIdx.x; !rank && e < nheads * (D / 4); e += T::WARPS * 32)
         Sum4::none().write(p, b, hk * p.G + chunk * NH + e / (D / 4), e % (D / 4));
       leave();
       return;
     }
-    in.within(p, b, len, (blockIdx.x - b * per) * slots);
-    const int units = slots - kRowCost, n = units / T::WARPS, m = units % T::WARPS;
-    in.s = kRowCost + n * warp + min(warp, m);
-    left = n + (warp < m);
+    in.within(p, b, len, (row - b * per) * slots);
+    // units to warps in turn over the cluster's CTAs first, so that few are spread over all of them
+    const int units = slots - kRowCost, all = T::WARPS * p.row_mode, n = units / all, m = units % all;
+    const int i = rank + warp * p.row_mode, mine = n + (i < m);
+    in.s = kRowCost + n * i + min(i, m);
+    left = mine;
   } else {
     ListSums list;
     list.build<T::WARPS>(p, groups, warp, lane);
@@ -846,6 +870,9 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
   float* sm = reinterpret_cast<float*>(smem_raw);  // [warps][NH] maxima, sums, then [warps][NH][D]
   float* sl = sm + T::WARPS * NH;
   float* so = sl + T::WARPS * NH;
+  float4* co = reinterpret_cast<float4*>(so + T::WARPS * NH * D);  // the CTA's sum: [NH][D], and [NH] maxima and sums
+  float2* cm = reinterpret_cast<float2*>(co + NH * D / 4);
+  static_assert((T::WARPS * NH * (D + 2) + NH * (D + 2)) * 4 <= T::SMEM, "the parts fit the rings' memory");
   if (g == 0) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -887,8 +914,13 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
 #pragma unroll
     for (int i = 0; i < T::WARPS; ++i)
       x.l += sm[i * NH + h] == -INFINITY ? 0.f : sl[i * NH + h] * exp2f(sm[i * NH + h] - x.m);
-    if (p.row_mode) {
+    if (p.row_mode == 1) {
       x.write(p, at.b, at.hk * p.G + at.chunk * NH + h, c);
+      continue;
+    }
+    if (p.row_mode) {
+      co[e] = x.o;
+      if (c == 0) cm[h] = make_float2(x.m, x.l);
       continue;
     }
     reinterpret_cast<float4*>(p.part_o + (slot * NH + h) * D)[c] = x.o;
@@ -897,6 +929,30 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
       p.part_l[slot * NH + h] = x.l;
     }
   }
+  if (p.row_mode <= 1) return;
+  // ---- the cluster's CTAs have a sum each, read over the cluster's shared memory
+  cluster_sync();
+  const int rank = blockIdx.x % p.row_mode;
+  for (int e = rank + p.row_mode * int(threadIdx.x); e < nheads * (D / 4); e += p.row_mode * T::WARPS * 32) {
+    const int h = e / (D / 4), c = e % (D / 4);
+    const uint32_t from_m = smem_u32(cm + h), from_o = smem_u32(co + e);
+    float M = -INFINITY;
+#pragma unroll 8
+    for (int i = 0; i < p.row_mode; ++i) M = fmaxf(M, cluster_float2(from_m, i).x);
+    Sum4 x = Sum4::none();
+    x.m = M;
+#pragma unroll 8
+    for (int i = 0; i < p.row_mode; ++i) {
+      const float2 ml = cluster_float2(from_m, i);
+      const float4 y = cluster_float4(from_o, i);
+      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+      x.l = fmaf(ml.y, f, x.l);
+      x.o.x = fmaf(y.x, f, x.o.x); x.o.y = fmaf(y.y, f, x.o.y);
+      x.o.z = fmaf(y.z, f, x.o.z); x.o.w = fmaf(y.w, f, x.o.w);
+    }
+    x.write(p, at.b, at.hk * p.G + at.chunk * NH + h, c);
+  }
+  cluster_sync();  // no CTA leaves while another reads its memory
 }
 
 // The parts of a row: one for every CTA of the tile kernel whose share lies in it, one for every warp of the
@@ -1095,6 +1151,12 @@ bool use_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor* v
   return p.g.num_blocks > 0 && rows_on(p.q, p.q_dtype, p.q_sb, p.q_sh, p.q_sd, 4) && tile_layout(k_cache) && tile_layout(v_cache);
 }
 
+void cluster_attribute(cudaLaunchAttribute* a, int ctas) {
+  a->id = cudaLaunchAttributeClusterDimension;
+  a->val.clusterDim.x = unsigned(ctas);
+  a->val.clusterDim.y = a->val.clusterDim.z = 1;
+}
+
 // Warps of the grid: the CTAs fill the GPU once, if the block table has work for them.
 template <typename F>
 auto with_shape(const AttnParams& p, F&& f) {
@@ -1113,6 +1175,36 @@ auto with_shape(const AttnParams& p, F&& f) {
   return p.heads == 16 ? kind(std::integral_constant<int, 256>(), two) : kind(std::integral_constant<int, 256>(), one);
 }
 
+// Clusters of `ctas` CTAs that the device holds at once.
+int cluster_room(const AttnParams& p, int ctas) {
+  return with_shape(p, [&](auto d, auto kind, auto nt) {
+    using T = TileShape<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>;
+    static int room[64][5] = {};  // one more than there are
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int& r = room[dev & 63][31 - __builtin_clz(unsigned(ctas))];
+    if (r == 0) {
+      auto kern = paged_attn_tile_kernel<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>;
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      cluster_attribute(attr, ctas);
+      cfg.gridDim = dim3(ctas);
+      cfg.blockDim = dim3(T::WARPS * 32);
+      cfg.dynamicSmemBytes = T::SMEM;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      const bool some =
+          cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM) == cudaSuccess &&
+          (ctas <= 8 || cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) &&
+          cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess;
+      (void)cudaGetLastError();
+      r = 1 + (some ? n : 0);
+    }
+    return r - 1;
+  });
+}
+
 void plan_tiles(AttnParams* p) {
   p->heads = p->G > 8 ? 16 : 8;
   p->chunks = (p->G + p->heads - 1) / p->heads;
@@ -1120,15 +1212,26 @@ void plan_tiles(AttnParams* p) {
   const int warps = with_shape(*p, [](auto d, auto kind, auto nt) {
     return TileShape<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>::WARPS;
   });
-  // Rows of few tokens (as far as the block table goes), no more of them than SMs: a CTA a row, and no join. How many
-  // units of a warp are few depends on how many SMs the rows leave idle. 128 channels, us with it and without, by rows
-  // and units: 4 rows 8.6, 8.5 (3), 10.2, 8.5 (4); 16 rows 10.3, 11.7 (4), 11.3, 11.9 (5), 13.4, 12.4 (8); 40 rows 11.1,
-  // 12.9 (5), 13.3, 14.1 (8); 80 rows 15.3, 17.6 (10); 128 rows 25.0, 29.8 (10), 35.7, 40.5 (16), but of lengths from
-  // 1 to all of it 15.0, 13.7 (10), 20.7, 16.9 (16).
+  // Rows of not too many tokens (as far as the block table goes): a cluster of CTAs each, and no kernel to join them. Such a
+  // kernel costs some 2 us, and 4 more once the list fills the SMs, as its CTAs then find room only when that ends; the
+  // cluster costs what its SMs wait for the longest row, and the SMs that no cluster has. 128 channels, us so and by the
+  // list: 28 heads over 4, one sequence of 777 tokens 8.2, 8.4, 2000 8.8, 9.4, 4000 9.8, 13.8, 16000 14.4, 17.0, 32768
+  // 19.9, 19.1; 4 of 2000 10.6, 13.5, of 8000 18.2, 17.1; 8 of 4000 14.3, 17.0, of 100 to 4000 13.5, 14.9; 32 over 8, 16
+  // of 1900 25.0, 29.8, of 1 to 1900 15.0, 13.7, of 3000 35.7, 40.5, of 100 to 3000 20.7, 16.9. 32 over 2 (16 heads a
+  // pass), one of 777 10.2, 9.4, 4000 12.4, 11.3, 8000 14.5, 17.2.
   const int64_t rows = int64_t(p->g.B) * p->g.Hk * p->chunks;
-  const int units = 2 * rows >= num_sms() ? 10 : 10 * rows >= num_sms() ? 5 : 2;
-  p->row_mode = rows <= num_sms() && most_slots(*p, p->chunks) <= rows * (units * warps + kRowCost);
-  p->warps = int(p->row_mode ? rows : ctas) * warps;
+  const int64_t units = rows ? most_slots(*p, p->chunks) / rows - kRowCost : 0;
+  // as many CTAs as leave each of them 8 units or more; one for up to two units a warp (one sequence of 300 tokens: 7.5 us
+  // against 8.2; of 777 with 8, 16 units or more: 8.2, 9.0)
+  int c = 1;
+  while (c < 16 && units > std::max(8 * c, 2 * warps) && rows * 2 * c <= num_sms() && rows <= cluster_room(*p, 2 * c)) c *= 2;
+  const int64_t busy = rows * c;
+  const int most = 2 * busy >= num_sms()       ? 10  // units of a warp at most
+                   : ctas == num_sms()         ? (5 * busy >= 2 * num_sms() ? 8 : 5)
+                   : c > 1 && p->heads == 16   ? 0
+                                               : 2;
+  p->row_mode = busy <= num_sms() && units <= c * most * warps ? c : 0;
+  p->warps = int(p->row_mode ? busy : ctas) * warps;
   p->block_shift = 31 - __builtin_clz(unsigned(p->g.block));
 }
 
@@ -1177,13 +1280,19 @@ int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor*
       return rc;
     set[dev & 63] = true;
   }
-  const dim3 grid(p.warps / T::WARPS), block(T::WARPS * 32);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(p.warps / T::WARPS);
+  cfg.blockDim = dim3(T::WARPS * 32);
+  cfg.dynamicSmemBytes = T::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
   if (p.after_select) {
-    if ((rc = launch_pdl(kern, grid, block, T::SMEM, st, "paged_attn_tile_kernel launch", p, km, vm))) return rc;
-  } else {
-    kern<<<grid, block, T::SMEM, st>>>(p, km, vm);
-    if ((rc = cuda_check(cudaGetLastError(), "paged_attn_tile_kernel launch"))) return rc;
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
+  if (p.row_mode > 1) cluster_attribute(&attr[cfg.numAttrs++], p.row_mode);
+  if ((rc = cuda_check(cudaLaunchKernelEx(&cfg, kern, p, km, vm), "paged_attn_tile_kernel launch"))) return rc;
   if (p.row_mode) return BD_OK;
   const int ctas = p.warps / T::WARPS;
   constexpr int MANY = D == 256 ? 4 : 8;  // heads that 256 threads hold at 4 channels each, 8 at most

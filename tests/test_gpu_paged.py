@@ -254,7 +254,11 @@ def test_decode_attn(cuda, Hq, Hk, D, block, qdt, cdt):
 # what cuts them, running sums of one sequence a lane, of one and of several a group.
 SHARED_OUT = {
     "a CTA a row": lambda g: ([700, 0, 333, 1, 90, 1024] * 3, 2),
+    "two CTAs a row": lambda g: ([1200, 0, 333, 1, 90, 2024, 16, 17] * 3, 2),
+    "eight CTAs a row": lambda g: ([3000, 0, 1777, 16], 2),
+    "sixteen CTAs a row": lambda g: ([5000, 15], 2),
     "few rows, one CTA a head": lambda g: ([4000, 0, 9, 2500], 2),
+    "few long rows": lambda g: ([30000, 0, 9, 2500], 2),
     "eight heads a CTA": lambda g: (torch.randint(0, 1500, (40,), generator=g).tolist() + [3001], 2),
     "many rows, long and short": lambda g: (torch.randint(0, 90, (310,), generator=g).tolist() + [2777, 0, 1500], 2),
     "many rows alike": lambda g: ([100] * 160, 4),
