@@ -4,6 +4,12 @@
 
 namespace bd {
 
+// The paged kernels but the choice of pages are launched as programmatic dependents of whatever ran before them in the
+// stream, so that they are on the SMs when that ends (a step's append 2.4 us in a graph against 2.7, one sequence's
+// attention 7.9 against 8.2). Each waits for it before it touches global memory, and lets the next one begin, where that
+// is part of the same call, only after that. The choice is launched in stream order: CTAs of it that come early crowd
+// on the SMs that the kernel before has left (choice and attention of 16 sequences 45.9 us against 37.5).
+
 // A paged cache as the kernels address it: pages [num_blocks, Hk, block, D], any strides
 // (elements; the innermost one too), and the block table that maps a sequence's logical
 // pages to them. Entries outside [0, num_blocks) name no page.

@@ -419,7 +419,6 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
   constexpr float kUp = KIND == kBf16 ? 0.f : 14.f;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __shared__ GroupSums groups;
-  griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t ring = base + uint32_t(warp) * T::STAGES * 2 * T::HALF;
@@ -433,6 +432,10 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
   if (lane < T::STAGES) mbar_init(bars + lane * 8, 1);
   if (lane == 0) mbar_fence_init();
   __syncwarp();
+  // what ran before this call is done from here on (with chosen pages: since the choice began); only then may the join
+  // begin, which reads the lengths
+  if (!p.after_select) griddep_wait();
+  if (!p.row_mode) griddep_launch_dependents();
 
   // a kernel that waits for this one finds what this one waits for done as well, whichever way it ends
   auto leave = [&]() {
@@ -1287,10 +1290,8 @@ int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor*
   cfg.dynamicSmemBytes = T::SMEM;
   cfg.stream = st;
   cfg.attrs = attr;
-  if (p.after_select) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-  }
+  attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   if (p.row_mode > 1) cluster_attribute(&attr[cfg.numAttrs++], p.row_mode);
   if ((rc = cuda_check(cudaLaunchKernelEx(&cfg, kern, p, km, vm), "paged_attn_tile_kernel launch"))) return rc;
   if (p.row_mode) return BD_OK;

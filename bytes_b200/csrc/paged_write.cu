@@ -8,6 +8,7 @@
 // Summary of a page and KV head: channelwise min and max of the stored keys times k_scale, as
 // int8 code = rint(x / s), s = max|.| / 127.
 #include "paged.cuh"
+#include "decode_shared.cuh"
 
 #include <algorithm>
 #include <cfloat>
@@ -112,6 +113,8 @@ __device__ __forceinline__ void store_cache(void* base, int dt, int64_t off, flo
 // Any type, stride and head dim: one CTA per token, a thread a channel. For what the vector form cannot address: one
 // token 23.5 us against 2.6, 14991 tokens (32 query heads, 8 KV heads of 128 channels) 431 against 70.
 __global__ void __launch_bounds__(128) paged_append_generic_kernel(const AppendParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int t = blockIdx.x;
   const int2 place = place_of(p.g, p.cu, t);
   int page = -1;
@@ -213,6 +216,8 @@ constexpr int kAppendWarps = 4;
 
 template <typename TI, typename TC>
 __global__ void __launch_bounds__(kAppendWarps * 32, 7) paged_append_kernel(const AppendParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int64_t w = int64_t(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, t = int(w / p.parts), part = int(w % p.parts);
   if (t >= p.T) return;
@@ -291,8 +296,7 @@ int launch_append(AppendParams p, cudaStream_t st) {
   p.parts = (all + p.each - 1) / p.each;
   const int64_t ctas = (int64_t(p.T) * p.parts + kAppendWarps - 1) / kAppendWarps;
   auto go = [&](auto kern) {
-    kern<<<unsigned(ctas), kAppendWarps * 32, 0, st>>>(p);
-    return cuda_check(cudaGetLastError(), "paged_append_kernel launch");
+    return launch_pdl(kern, dim3(unsigned(ctas)), dim3(kAppendWarps * 32), 0, st, "paged_append_kernel launch", p);
   };
   auto with = [&](auto in) {
     using TI = decltype(in);
@@ -368,6 +372,7 @@ __device__ __forceinline__ int8_t code_of(float x, float s, bool some) {
 // Any type, stride and head dim: one warp per (page, KV head), a lane every 32nd channel. For what the vector form
 // cannot address (8 sequences of 30001 tokens, four KV heads of 128 channels: 92 us against 48).
 __global__ void __launch_bounds__(128) paged_summary_generic_kernel(const SummaryParams p) {
+  griddep_wait();
   const int lane = threadIdx.x & 31;
   const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int h = int(w % p.g.Hk);
@@ -430,6 +435,7 @@ __global__ void __launch_bounds__(256, 2) paged_summary_kernel(const SummaryPara
   using P = Pair<T>;
   using V = typename P::V;
   constexpr int NP = FP8 ? 8 : 4, GROUPS = 32 / LPR, D = LPR * NP * 2, ES = FP8 ? 1 : 2, STEP = 8 * GROUPS;
+  griddep_wait();
   const int lane = threadIdx.x & 31, part = lane % LPR, group = lane / LPR;
   const int w = blockIdx.x * 8 + (threadIdx.x >> 5), stride = int(gridDim.x) * 8 / p.g.Hk, h = w % p.g.Hk;
   int64_t i = w / p.g.Hk;
@@ -578,14 +584,13 @@ int launch_summary(const SummaryParams& p, bool vector, cudaStream_t st) {
   if (items == 0) return BD_OK;
   if (!vector) {
     if (items > 4 * int64_t(0x7fffffff)) return fail(BD_ERR_SHAPE, "too many pages for one launch");
-    paged_summary_generic_kernel<<<unsigned((items + 3) / 4), 128, 0, st>>>(p);
-    return cuda_check(cudaGetLastError(), "paged_summary_generic_kernel launch");
+    return launch_pdl(paged_summary_generic_kernel, dim3(unsigned((items + 3) / 4)), dim3(128), 0, st,
+                      "paged_summary_generic_kernel launch", p);
   }
   // two CTAs an SM, and a warp for every KV head at least
   const unsigned ctas = unsigned(std::max<int64_t>((p.g.Hk + 7) / 8, std::min<int64_t>((items + 7) / 8, 2 * num_sms())));
   auto go = [&](auto kern) {
-    kern<<<ctas, 256, 0, st>>>(p, pages);
-    return cuda_check(cudaGetLastError(), "paged_summary_kernel launch");
+    return launch_pdl(kern, dim3(ctas), dim3(256), 0, st, "paged_summary_kernel launch", p, pages);
   };
   auto with = [&](auto k64, auto k128, auto k256) { return p.g.D == 64 ? go(k64) : p.g.D == 128 ? go(k128) : go(k256); };
   switch (p.dtype) {
@@ -688,8 +693,8 @@ int bd_paged_append(const bd_tensor* k, const bd_tensor* v, const bd_tensor* q, 
                         by_eight(v) && (!q || (by_eight(q) && by_eight(q_out))) && by_eight(k_cache) &&
                         by_eight(v_cache) && (!cos || (by_eight(cos) && by_eight(sin)));
     if (vector) return launch_append(p, stream);
-    paged_append_generic_kernel<<<unsigned(T), 128, 0, stream>>>(p);
-    return cuda_check(cudaGetLastError(), "paged_append_generic_kernel launch");
+    return launch_pdl(paged_append_generic_kernel, dim3(unsigned(T)), dim3(128), 0, stream,
+                      "paged_append_generic_kernel launch", p);
   });
 }
 
