@@ -4,11 +4,12 @@
 
 namespace bd {
 
-// The paged kernels but the choice of pages are launched as programmatic dependents of whatever ran before them in the
-// stream, so that they are on the SMs when that ends (a step's append 2.4 us in a graph against 2.7, one sequence's
-// attention 7.9 against 8.2). Each waits for it before it touches global memory, and lets the next one begin, where that
-// is part of the same call, only after that. The choice is launched in stream order: CTAs of it that come early crowd
-// on the SMs that the kernel before has left (choice and attention of 16 sequences 45.9 us against 37.5).
+// The paged kernels are launched as programmatic dependents of whatever ran before them in the stream, so that they are
+// on the SMs when that ends (among other work: an append of one token 6.4 us against 6.8, attention of one sequence 8.2
+// against 10.2, choice and attention of 16 sequences 38.4 against 40.9). Each waits for it before it touches global
+// memory. A kernel lets the next one begin early only where that is a part of the same call or usually follows it, and
+// after its own wait; the choice after its scores only, and the attention of a cluster a row not at all: CTAs of
+// another call that come early crowd on the SMs that are free (45.9 us in a graph against 37.2 for the 16 sequences).
 
 // A paged cache as the kernels address it: pages [num_blocks, Hk, block, D], any strides
 // (elements; the innermost one too), and the block table that maps a sequence's logical

@@ -47,7 +47,7 @@ constexpr int kGenHeads = 4;
 
 // One CTA per (split, KV head and chunk of 4 query heads, sequence); a warp takes every fourth
 // token, its lanes every 32nd channel. For what the tiles cannot address: one sequence of 16 tokens 17.5 us against
-// 5.5, of 777 52 against 8.5; 8 of 32768 (28 heads over 4, 128 channels) 3.7 ms against 89 us.
+// 5.2, of 777 52 against 7.9; 8 of 32768 (28 heads over 4, 128 channels) 3.7 ms against 89 us.
 __global__ void __launch_bounds__(kGenWarps * 32) paged_attn_generic_kernel(const AttnParams p) {
   __shared__ float red_m[kGenWarps][kGenHeads], red_l[kGenWarps][kGenHeads];
   __shared__ float red_o[kGenWarps][kGenHeads][256];
@@ -157,11 +157,14 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const AttnParams p) {
 // (maximum, sum, numerator) go to the workspace, two at most for a warp, and paged_tile_join_kernel joins
 // them.
 //
+// Few rows of not too many tokens (row_mode) are not put in the list: a cluster of CTAs has a row, its units in equal
+// shares for all of the cluster's warps, and adds up what they have over its shared memory.
+//
 // Bound by memory once there is enough of it: 8 sequences of 131072 tokens (28 heads over 4, 128 channels, bf16) 2148
 // MB in 323 us, 6.65 TB/s, what a copy reaches; 64 of 33 to 8192 tokens (32 over 8) 400 MB in 74 us, 5.4 TB/s. The
 // difference is some 8 us for the launch, the way to the first units, and the join. 8-bit caches are issue-bound as well,
 // since a byte costs twice the work: 8 sequences of 32768 tokens 268 MB in 55 us, 4.9 TB/s. One sequence of 777 tokens
-// takes 8.5 us, all of it latency.
+// takes 7.9 us, all of it latency: a launch, the reads of length, table, page and query, a sum over the cluster, a write.
 
 constexpr int kUnit = 16;
 

@@ -76,9 +76,9 @@ __device__ __forceinline__ void mma_s8(int* d, uint32_t a0, uint32_t a1, uint32_
 // heads). The order of the 2D numbers is free, so that a thread's operand registers are 16 contiguous
 // bytes of a row, loaded from global memory as such: no shared memory but for the queries.
 //
-// Bound by memory as it scores (2D + 4 bytes a page and head), then by the latency of the choice, some 6 us. 16
+// Bound by memory as it scores (2D + 4 bytes a page and head), then by the latency of the choice, 3 us for 2048 pages. 16
 // sequences of 2048 pages, 8 KV heads of 128 channels: 68 MB in 19 us, 64 pages chosen; half as many pages 13 us; one
-// sequence of 2048 pages 8.5 us, of 8192 pages (four KV heads) 13.
+// sequence of 2048 pages 8.1 us, of 8192 pages (four KV heads) 12.3 (5 of them after the scores).
 //
 // D = 0: any head dim, any alignment of the summaries, a lane a page.
 template <int D, int THREADS>
@@ -369,7 +369,7 @@ __device__ __forceinline__ void choose_pages(const unsigned* keys, int n, int wa
 template <int D, int HOLD, int THREADS>
 __global__ void __launch_bounds__(THREADS, (D == 256 ? 512 : 1024) / THREADS) paged_select_kernel(const SelectParams p) {
   extern __shared__ __align__(16) int8_t q8[];  // [heads, a multiple of 8][2D], then their scales
-  griddep_launch_dependents();
+  griddep_wait();
   const int rank = blockIdx.x, ctas = gridDim.x, hk = blockIdx.y, b = blockIdx.z;
   const int t = threadIdx.x;
   const int n = int((int64_t(paged_len(p.g, b)) + p.g.block - 1) / p.g.block), want = min(n, p.budget);
@@ -384,6 +384,7 @@ __global__ void __launch_bounds__(THREADS, (D == 256 ? 512 : 1024) / THREADS) pa
   unsigned* keys = p.keys + (int64_t(b) * p.g.Hk + hk) * p.pitch;
   if constexpr (D == 0) score_pages_any<THREADS>(p, b, hk, n, keys, q8, rank, ctas, t >> 5, t & 31);
   else score_pages<D, THREADS>(p, b, hk, n, keys, q8, rank, ctas, t >> 5, t & 31);
+  griddep_launch_dependents();
   if (ctas > 1) {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
     if (rank) return;
@@ -465,7 +466,7 @@ int launch_select(const SelectParams& p, cudaStream_t st) {
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
@@ -492,6 +493,9 @@ int launch_select(const SelectParams& p, cudaStream_t st) {
   }
   cfg.gridDim = dim3(ctas, p.g.Hk, p.g.B);
   attr[0].val.clusterDim.x = ctas;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
   return cuda_check(cudaLaunchKernelEx(&cfg, kern, p), "paged_select_kernel launch");
 }
 

@@ -111,7 +111,7 @@ __device__ __forceinline__ void store_cache(void* base, int dt, int64_t off, flo
 }
 
 // Any type, stride and head dim: one CTA per token, a thread a channel. For what the vector form cannot address: one
-// token 23.5 us against 2.6, 14991 tokens (32 query heads, 8 KV heads of 128 channels) 431 against 70.
+// token 23.5 us against 2.4, 14991 tokens (32 query heads, 8 KV heads of 128 channels) 431 against 70.
 __global__ void __launch_bounds__(128) paged_append_generic_kernel(const AppendParams p) {
   griddep_wait();
   griddep_launch_dependents();
@@ -209,8 +209,8 @@ template <> struct Eight<__nv_fp8_e4m3> {
 // items it, it + 1, ... `each` times; the heads run over queries, keys and values.
 //
 // Bound by memory: every number is read and written once, and 6 operations a rotated pair are nothing beside it.
-// 14991 tokens of 11 prompts (32 query heads, 8 KV heads of 128 channels, bf16): 371 MB in 70 us, 5.3 TB/s, 81 % of
-// what a copy reaches; a step of one token 2.6 us, of 128 tokens 3.2, a launch's own time. Four warps a CTA, seven CTAs
+// 14991 tokens of 11 prompts (32 query heads, 8 KV heads of 128 channels, bf16): 371 MB in 69 us, 5.4 TB/s, 82 % of
+// what a copy reaches; a step of one token 2.4 us, of 128 tokens 2.9, a launch's own time. Four warps a CTA, seven CTAs
 // an SM: 72 registers hold two items' loads in flight and turned.
 constexpr int kAppendWarps = 4;
 
