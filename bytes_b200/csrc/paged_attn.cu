@@ -204,8 +204,10 @@ __device__ __forceinline__ void prefetch_tensormap(const void* map) {
   asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
 }
 
-// A row's place in the list: its slots are kRowCost and its units; 0 without a token.
-constexpr int kRowCost = 1;
+// A row's place in the list: its slots are kRowCost and its units; 0 without a token. With 1, 2, 3 for a row: 64 sequences
+// of 33 to 8192 tokens (32 heads over 8), fp8 52.0, 50.7, 49.3 us, bf16 74.5, 75.1, 74.5; 100 of 20 to 3000 (12 over 12,
+// 64 channels, f16) 46.1, 44.8, 44.3; 64 of 16 (32 over 8) 9.8, 10.0, 10.4.
+constexpr int kRowCost = 3;
 
 __device__ __forceinline__ int row_slots(const AttnParams& p, int len) {
   if (len <= 0) return 0;
@@ -270,10 +272,12 @@ struct ListSums {
 // (one sequence of 777 tokens, 28 heads over 4: 12.5, 9.5, 9.2, 9.8 us for 1, 2, 4, 8).
 constexpr int kMinSlots = 4;
 
-// A border inside a row of up to `whole` slots, half a share or 8, moves to the nearer end of the row: so
+// A border inside a row of up to `whole` slots, half a share or 7 units, moves to the nearer end of the row: so
 // short a row costs less unevenly shared than joined. What cuts a longer row stays where it is (64 sequences
-// of 33 to 8192 tokens: 73.8, 74.7, 82 us for 8, half a share, a share and a half; 148 sequences of 100
-// tokens: 14.9 us against 27 with 4).
+// of 33 to 8192 tokens: 73.8, 74.7, 82 us for 7 units, half a share, a share and a half; 148 sequences of 100
+// tokens: 14.9 us against 27 with 3 units).
+constexpr int kWholeUnits = 7;
+
 template <int WARPS>
 struct Shares {
   int each, rest, ctas, whole;
@@ -281,7 +285,7 @@ struct Shares {
     ctas = max(1, min(warps / WARPS, total / kMinSlots));
     each = total / ctas;
     rest = total - each * ctas;
-    whole = max(8, each / (2 * WARPS));
+    whole = max(kWholeUnits + kRowCost, each / (2 * WARPS));
   }
   __device__ __forceinline__ int cta(int c) const { c = min(c, ctas); return each * c + min(c, rest); }
   __device__ __forceinline__ int begin(int w) const {
@@ -1241,12 +1245,14 @@ void plan_tiles(AttnParams* p) {
   p->block_shift = 31 - __builtin_clz(unsigned(p->g.block));
 }
 
-// Many rows are joined by what cuts them (one CTA a share of the list), others by themselves. 32 heads over 8, 128 channels,
-// us by cuts and by rows: 64 sequences of 33 to 8192 tokens 94.6, 74.4; 256 of 33 to 4000 171, 166; 296 of 2000 377, 385;
-// 512 of 33 to 2000 187, 206; 1024 of 100 86, 173. Two groups of heads at 256 channels: 64 of 33 to 4000 123, 92.
+// Many rows are joined by what cuts them (one CTA a share of the list), and rows too short to be cut; others by
+// themselves. 32 heads over 8, 128 channels, us by cuts and by rows: 80 sequences of 100 tokens 13.9, 16.2, of 300 30.5,
+// 23.1; 200 of 100 15.8, 24.2, of 300 57.6, 58.5; 64 of 33 to 8192 94.6, 74.4; 256 of 33 to 4000 171, 166; 296 of 2000 377,
+// 385; 512 of 33 to 2000 187, 206; 1024 of 100 86, 173. Two groups of heads at 256 channels: 64 of 33 to 4000 123, 92.
 bool join_by_cuts(const AttnParams& p) {
   const int most = p.g.D == 256 ? 4 : 8, groups = (std::min(p.heads, p.G) + most - 1) / most;
-  return int64_t(p.g.B) * p.g.Hk * p.chunks * groups > 14 * num_sms();
+  const int64_t rows = int64_t(p.g.B) * p.g.Hk * p.chunks;
+  return rows * groups > 14 * num_sms() || most_slots(p, p.chunks) <= rows * (kWholeUnits + kRowCost);
 }
 
 size_t tile_bytes(const AttnParams& p) {
