@@ -436,8 +436,10 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
-  if (lane < T::STAGES) mbar_init(bars + lane * 8, 1);
-  if (lane == 0) mbar_fence_init();
+  if (lane == 0) {  // all by one lane: the fence orders the inits of the thread that executes it
+    for (int s = 0; s < T::STAGES; ++s) mbar_init(bars + s * 8, 1);
+    mbar_fence_init();
+  }
   __syncwarp();
   // what ran before this call is done from here on (with chosen pages: since the choice began); only then may the join
   // begin, which reads the lengths

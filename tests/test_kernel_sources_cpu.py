@@ -1,0 +1,42 @@
+"""Rules of synchronisation that the kernels' sources have to keep and that no run shows reliably (no GPU)."""
+import glob
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bytes_b200", "csrc")
+KERNELS = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
+
+
+def code(path):
+    """The source without comments."""
+    src = re.sub(r"/\*.*?\*/", "", open(path).read(), flags=re.S)
+    return re.sub(r"//[^\n]*", "", src)
+
+
+def enclosing_block(src, at):
+    """(the text before the brace that opens the innermost block around `at`, the block)."""
+    depth, start = 0, at
+    while True:
+        start -= 1
+        depth += {"}": 1, "{": -1}.get(src[start], 0)
+        if depth < 0:
+            break
+    depth, end = 0, at
+    while depth >= 0:
+        depth += {"{": 1, "}": -1}.get(src[end], 0)
+        end += 1
+    return src[:start].rstrip(), src[start:end]
+
+
+@pytest.mark.parametrize("path", KERNELS, ids=os.path.basename)
+def test_barriers_are_initialised_by_the_thread_that_fences_them(path):
+    """fence.mbarrier_init orders the executing thread's own inits ahead of the copies that complete on
+    them: one thread makes all of a set of barriers, and the same one fences."""
+    src = code(path)
+    for m in re.finditer(r"\bmbar_init\(", src):
+        head, block = enclosing_block(src, m.start())
+        assert re.search(r"if \([^{};]*(threadIdx\.x|lane) == 0\)$", head), head[-80:]
+        inits = [i.start() for i in re.finditer(r"\bmbar_init\(", block)]
+        assert "mbar_fence_init()" in block[inits[-1]:]
