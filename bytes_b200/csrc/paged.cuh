@@ -55,6 +55,13 @@ int guarded(F&& body) noexcept {
   }
 }
 
+// All threads of the cluster's CTAs; what they wrote to shared or global memory before is there after. The barrier's
+// aligned form wants a warp's lanes together, which loops of unlike lengths leave apart.
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
 // Loads and stores by element type, for the forms that take any of them.
 __device__ __forceinline__ float load_as(const void* base, int dt, int64_t off) {
   switch (dt) {

@@ -394,12 +394,6 @@ struct Sum4 {
   }
 };
 
-// All threads of the cluster's CTAs; what they wrote to shared memory before is there after.
-__device__ __forceinline__ void cluster_sync() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-
 // What CTA `rank` of the cluster holds at this CTA's shared address.
 __device__ __forceinline__ float2 cluster_float2(uint32_t at, int rank) {
   float2 x;

@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(THREADS, (D == 256 ? 512 : 1024) / THREADS) pa
   else score_pages<D, THREADS>(p, b, hk, n, keys, q8, rank, ctas, t >> 5, t & 31);
   griddep_launch_dependents();
   if (ctas > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    cluster_sync();
     if (rank) return;
   } else {
     __syncthreads();

@@ -7,6 +7,7 @@ import pytest
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bytes_b200", "csrc")
 KERNELS = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
+SOURCES = sorted(KERNELS + glob.glob(os.path.join(CSRC, "*.cuh")))
 
 
 def code(path):
@@ -40,3 +41,12 @@ def test_barriers_are_initialised_by_the_thread_that_fences_them(path):
         assert re.search(r"if \([^{};]*(threadIdx\.x|lane) == 0\)$", head), head[-80:]
         inits = [i.start() for i in re.finditer(r"\bmbar_init\(", block)]
         assert "mbar_fence_init()" in block[inits[-1]:]
+
+
+@pytest.mark.parametrize("path", SOURCES, ids=os.path.basename)
+def test_aligned_cluster_barriers_have_their_warps_together(path):
+    """barrier.cluster.*.aligned wants all lanes of a warp at it together: the statement before it sees to that."""
+    src = code(path)
+    for m in re.finditer(r"barrier\.cluster\.arrive[a-z.]*\.aligned", src):
+        before = src[:m.start()].rsplit("asm", 1)[0].rstrip()
+        assert before.endswith(("__syncwarp();", "__syncthreads();")), before[-80:]
