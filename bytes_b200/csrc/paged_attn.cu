@@ -435,8 +435,8 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
     mbar_fence_init();
   }
   __syncwarp();
-  // what ran before this call is done from here on (with chosen pages: since the choice began); only then may the join
-  // begin, which reads the lengths
+  // what ran before this call is done from here on (after a choice: since that let this kernel begin); only then may the
+  // join begin, which reads the lengths
   if (!p.after_select) griddep_wait();
   if (!p.row_mode) griddep_launch_dependents();
 
@@ -1380,8 +1380,8 @@ int check_out(const bd_tensor* q, const bd_tensor* k_cache, float k_scale, float
   return BD_OK;
 }
 
-// The whole call; after_select: `selected` is written by the kernel launched just before, which was itself
-// launched in stream order (so all that came before it is done).
+// The whole call; after_select: `selected` is written by the kernel launched just before, all CTAs of which wait for what
+// came before the call before they let this one's begin.
 int run_attn(const bd_tensor* q, const bd_tensor* k_cache, const bd_tensor* v_cache, const bd_tensor* block_table,
              const bd_tensor* context_lens, const bd_tensor* selected, bool after_select, float scaling, float k_scale,
              float v_scale, const bd_tensor* out, const bd_tensor* lse, void* workspace, size_t workspace_bytes,

@@ -50,3 +50,11 @@ def test_aligned_cluster_barriers_have_their_warps_together(path):
     for m in re.finditer(r"barrier\.cluster\.arrive[a-z.]*\.aligned", src):
         before = src[:m.start()].rsplit("asm", 1)[0].rstrip()
         assert before.endswith(("__syncwarp();", "__syncthreads();")), before[-80:]
+
+
+def test_lengths_that_are_read_ahead_of_a_wait_come_from_l2():
+    """The joins, and the attention after a choice, read the lengths before they wait for the kernel ahead of them: past
+    L1, which may hold them from an earlier step."""
+    geometry = code(os.path.join(CSRC, "paged.cuh"))
+    assert [m.group(1) for m in re.finditer(r"(\S+)\blens\b[^;]*l_s\)?;", geometry)] == ["__ldcg(g."]
+    assert not re.search(r"\blens\s*\[|\blens\s*\+", code(os.path.join(CSRC, "paged_attn.cu")))
