@@ -576,17 +576,19 @@ __global__ void __launch_bounds__(256, 2) paged_summary_kernel(const SummaryPara
   }
 }
 
-int launch_summary(const SummaryParams& p, bool vector, cudaStream_t st) {
-  const int64_t pages = p.T == 0 ? int64_t(p.g.B) * p.g.wide
-                        : !p.cu  ? int64_t(p.g.B)
-                                 : 2 * int64_t(p.g.B) + (int64_t(p.T) + p.g.block - 1) / p.g.block;
-  const int64_t items = pages * p.g.Hk;
+struct SummaryCall {
+  SummaryParams p{};
+  int64_t pages = 0;  // what page_of_item numbers
+  bool vector = false;
+};
+
+int launch_summary(const SummaryCall& call, cudaStream_t st) {
+  const SummaryParams& p = call.p;
+  const int64_t pages = call.pages, items = pages * p.g.Hk;
   if (items == 0) return BD_OK;
-  if (!vector) {
-    if (items > 4 * int64_t(0x7fffffff)) return fail(BD_ERR_SHAPE, "too many pages for one launch");
+  if (!call.vector)
     return launch_pdl(paged_summary_generic_kernel, dim3(unsigned((items + 3) / 4)), dim3(128), 0, st,
                       "paged_summary_generic_kernel launch", p);
-  }
   // two CTAs an SM, and a warp for every KV head at least
   const unsigned ctas = unsigned(std::max<int64_t>((p.g.Hk + 7) / 8, std::min<int64_t>((items + 7) / 8, 2 * num_sms())));
   auto go = [&](auto kern) {
@@ -633,6 +635,111 @@ int check_cu(const bd_tensor* cu, const PagedGeometry& g, int64_t T) {
   return BD_OK;
 }
 
+struct AppendCall {
+  AppendParams p{};
+  bool vector = false;
+};
+
+// Checks an append and lays out its launch.
+int plan_append(const bd_tensor* k, const bd_tensor* v, const bd_tensor* q, const bd_tensor* cos, const bd_tensor* sin,
+                int interleaved, const bd_tensor* cu_seqlens, const bd_tensor* block_table, const bd_tensor* context_lens,
+                float k_scale, float v_scale, const bd_tensor* k_cache, const bd_tensor* v_cache, const bd_tensor* q_out,
+                AppendCall* call) {
+  int rc;
+  AppendParams& p = call->p;
+  if (!v_cache) return fail(BD_ERR_NULL, "v_cache descriptor is NULL");
+  if ((rc = check_paged(k_cache, v_cache, block_table, context_lens, &p.g))) return rc;
+  if ((rc = check_tensor(k, "k", 3))) return rc;
+  const int64_t T = k->shape[0], D = p.g.D;
+  if (!is_float16_32(k->dtype)) return fail(BD_ERR_DTYPE, "k must be bf16, f16 or f32");
+  if ((rc = check_new(k, "k", T, D, -1)) || (rc = check_new(v, "v", T, D, k->dtype))) return rc;
+  if (k->shape[1] != p.g.Hk || v->shape[1] != p.g.Hk)
+    return fail(BD_ERR_SHAPE, "k and v must have the cache's " + std::to_string(p.g.Hk) + " heads");
+  if (T > (int64_t(1) << 30)) return fail(BD_ERR_SHAPE, "more than 2^30 new tokens");
+  if ((rc = check_cu(cu_seqlens, p.g, T))) return rc;
+  if (!q != !q_out) return fail(BD_ERR_NULL, "q and q_out go together");
+  if (q) {
+    if ((rc = check_new(q, "q", T, D, k->dtype)) || (rc = check_new(q_out, "q_out", T, D, k->dtype))) return rc;
+    if (q_out->shape[1] != q->shape[1]) return fail(BD_ERR_SHAPE, "q_out must have q's shape");
+    p.q = rows_of(q);
+    p.q_out = q_out->data; p.o_st = q_out->stride[0]; p.o_sh = q_out->stride[1]; p.o_sd = q_out->stride[2];
+  }
+  if (!cos != !sin) return fail(BD_ERR_NULL, "cos and sin go together");
+  if (cos) {
+    if ((rc = check_tensor(cos, "cos", 2, BD_F32)) || (rc = check_tensor(sin, "sin", 2, BD_F32))) return rc;
+    if (cos->shape[0] != sin->shape[0] || cos->shape[1] != sin->shape[1])
+      return fail(BD_ERR_SHAPE, "cos " + shape_str(cos) + " and sin " + shape_str(sin) + " differ");
+    if (cos->shape[1] < 1 || 2 * cos->shape[1] > D)
+      return fail(BD_ERR_SHAPE, "cos and sin must have 1 to head_dim/2 columns, got " + std::to_string(cos->shape[1]));
+    if (cos->shape[0] > (int64_t(1) << 30)) return fail(BD_ERR_SHAPE, "cos has more than 2^30 rows");
+    if (cos->shape[1] > 1 && (cos->stride[1] != 1 || sin->stride[1] != 1))
+      return fail(BD_ERR_STRIDE, "cos and sin rows must be contiguous");
+    p.cos = static_cast<const float*>(cos->data); p.sin = static_cast<const float*>(sin->data);
+    p.c_s = cos->stride[0]; p.s_s = sin->stride[0];
+    p.positions = int(cos->shape[0]); p.half = int(cos->shape[1]);
+  }
+  const bool fp8 = k_cache->dtype == BD_F8E4M3;
+  if (!(k_scale > 0.f) || !(v_scale > 0.f)) return fail(BD_ERR_VALUE, "k_scale and v_scale must be positive");
+  if (!fp8 && (k_scale != 1.f || v_scale != 1.f))
+    return fail(BD_ERR_VALUE, "k_scale and v_scale belong to an fp8 cache");
+  p.k = rows_of(k); p.v = rows_of(v);
+  p.k_cache = k_cache->data; p.v_cache = v_cache->data;
+  p.T = int(T); p.in_dtype = k->dtype; p.cache_dtype = k_cache->dtype;
+  p.interleaved = interleaved != 0;
+  p.cu = cu_seqlens ? static_cast<const int*>(cu_seqlens->data) : nullptr;
+  p.k_inv = 1.f / k_scale; p.v_inv = 1.f / v_scale;
+  const int items = int(D / 16);
+  call->vector = D % 16 == 0 && items <= 16 && !(items & (items - 1)) && p.half % 8 == 0 && by_eight(k) &&
+                 by_eight(v) && (!q || (by_eight(q) && by_eight(q_out))) && by_eight(k_cache) &&
+                 by_eight(v_cache) && (!cos || (by_eight(cos) && by_eight(sin)));
+  return BD_OK;
+}
+
+int run_append(const AppendCall& call, cudaStream_t stream) {
+  if (call.p.T == 0) return BD_OK;
+  if (call.vector) return launch_append(call.p, stream);
+  return launch_pdl(paged_append_generic_kernel, dim3(unsigned(call.p.T)), dim3(128), 0, stream,
+                    "paged_append_generic_kernel launch", call.p);
+}
+
+// Checks a summary and lays out its launch.
+int plan_summary(const bd_tensor* k_cache, const bd_tensor* block_table, const bd_tensor* context_lens,
+                 const bd_tensor* cu_seqlens, int new_tokens, float k_scale, const bd_tensor* summary,
+                 const bd_tensor* summary_scale, SummaryCall* call) {
+  int rc;
+  SummaryParams& p = call->p;
+  if ((rc = check_paged(k_cache, nullptr, block_table, context_lens, &p.g))) return rc;
+  if ((rc = check_tensor(summary, "summary", 4, BD_I8)) || (rc = check_tensor(summary_scale, "summary_scale", 2, BD_F32)))
+    return rc;
+  if (summary->shape[0] != p.g.num_blocks || summary->shape[1] != p.g.Hk || summary->shape[2] != 2 ||
+      summary->shape[3] != p.g.D)
+    return fail(BD_ERR_SHAPE, "summary " + shape_str(summary) + " must be [num_blocks, Hk, 2, D] of the cache");
+  if (summary_scale->shape[0] != p.g.num_blocks || summary_scale->shape[1] != p.g.Hk)
+    return fail(BD_ERR_SHAPE, "summary_scale " + shape_str(summary_scale) + " must be [num_blocks, Hk]");
+  if (summary->stride[3] != 1 || summary->stride[2] != p.g.D)
+    return fail(BD_ERR_STRIDE, "summary's last two dims must be contiguous");
+  if (!(k_scale > 0.f)) return fail(BD_ERR_VALUE, "k_scale must be positive");
+  if (k_cache->dtype != BD_F8E4M3 && k_scale != 1.f) return fail(BD_ERR_VALUE, "k_scale belongs to an fp8 cache");
+  if (new_tokens < 0) return fail(BD_ERR_VALUE, "new_tokens must not be negative");
+  if (cu_seqlens && new_tokens == 0) return fail(BD_ERR_VALUE, "cu_seqlens goes with new_tokens");
+  if (new_tokens > 0 && (rc = check_cu(cu_seqlens, p.g, new_tokens))) return rc;
+  p.k_cache = k_cache->data; p.dtype = k_cache->dtype;
+  p.code = static_cast<int8_t*>(summary->data); p.c_sb = summary->stride[0]; p.c_sh = summary->stride[1];
+  p.scale = static_cast<float*>(summary_scale->data);
+  p.s_sb = summary_scale->stride[0]; p.s_sh = summary_scale->stride[1];
+  p.k_scale = k_scale; p.T = new_tokens;
+  p.cu = cu_seqlens ? static_cast<const int*>(cu_seqlens->data) : nullptr;
+  const bool types = p.dtype == BD_BF16 || p.dtype == BD_F16 || p.dtype == BD_F8E4M3;
+  call->vector = types && (p.g.D == 64 || p.g.D == 128 || p.g.D == 256) && !check_rows_aligned(k_cache, "k_cache") &&
+                 !((reinterpret_cast<uintptr_t>(p.code) | size_t(p.c_sb) | size_t(p.c_sh)) & 15);
+  call->pages = p.T == 0 ? int64_t(p.g.B) * p.g.wide
+                : !p.cu  ? int64_t(p.g.B)
+                         : 2 * int64_t(p.g.B) + (int64_t(p.T) + p.g.block - 1) / p.g.block;
+  if (!call->vector && call->pages > 4 * int64_t(0x7fffffff) / p.g.Hk)
+    return fail(BD_ERR_SHAPE, "too many pages for one launch");
+  return BD_OK;
+}
+
 }  // namespace
 }  // namespace bd
 
@@ -644,57 +751,30 @@ int bd_paged_append(const bd_tensor* k, const bd_tensor* v, const bd_tensor* q, 
                     const bd_tensor* v_cache, const bd_tensor* q_out, bd_stream_t stream) {
   using namespace bd;
   return guarded([&]() -> int {
+    AppendCall append;
+    const int rc = plan_append(k, v, q, cos, sin, interleaved, cu_seqlens, block_table, context_lens, k_scale, v_scale,
+                               k_cache, v_cache, q_out, &append);
+    return rc ? rc : run_append(append, stream);
+  });
+}
+
+int bd_paged_append_summary(const bd_tensor* k, const bd_tensor* v, const bd_tensor* q, const bd_tensor* cos,
+                            const bd_tensor* sin, int interleaved, const bd_tensor* cu_seqlens,
+                            const bd_tensor* block_table, const bd_tensor* context_lens, float k_scale, float v_scale,
+                            const bd_tensor* k_cache, const bd_tensor* v_cache, const bd_tensor* q_out,
+                            const bd_tensor* summary, const bd_tensor* summary_scale, bd_stream_t stream) {
+  using namespace bd;
+  return guarded([&]() -> int {
     int rc;
-    AppendParams p{};
-    if (!v_cache) return fail(BD_ERR_NULL, "v_cache descriptor is NULL");
-    if ((rc = check_paged(k_cache, v_cache, block_table, context_lens, &p.g))) return rc;
-    if ((rc = check_tensor(k, "k", 3))) return rc;
-    const int64_t T = k->shape[0], D = p.g.D;
-    if (!is_float16_32(k->dtype)) return fail(BD_ERR_DTYPE, "k must be bf16, f16 or f32");
-    if ((rc = check_new(k, "k", T, D, -1)) || (rc = check_new(v, "v", T, D, k->dtype))) return rc;
-    if (k->shape[1] != p.g.Hk || v->shape[1] != p.g.Hk)
-      return fail(BD_ERR_SHAPE, "k and v must have the cache's " + std::to_string(p.g.Hk) + " heads");
-    if (T > (int64_t(1) << 30)) return fail(BD_ERR_SHAPE, "more than 2^30 new tokens");
-    if ((rc = check_cu(cu_seqlens, p.g, T))) return rc;
-    if (!q != !q_out) return fail(BD_ERR_NULL, "q and q_out go together");
-    if (q) {
-      if ((rc = check_new(q, "q", T, D, k->dtype)) || (rc = check_new(q_out, "q_out", T, D, k->dtype))) return rc;
-      if (q_out->shape[1] != q->shape[1]) return fail(BD_ERR_SHAPE, "q_out must have q's shape");
-      p.q = rows_of(q);
-      p.q_out = q_out->data; p.o_st = q_out->stride[0]; p.o_sh = q_out->stride[1]; p.o_sd = q_out->stride[2];
-    }
-    if (!cos != !sin) return fail(BD_ERR_NULL, "cos and sin go together");
-    if (cos) {
-      if ((rc = check_tensor(cos, "cos", 2, BD_F32)) || (rc = check_tensor(sin, "sin", 2, BD_F32))) return rc;
-      if (cos->shape[0] != sin->shape[0] || cos->shape[1] != sin->shape[1])
-        return fail(BD_ERR_SHAPE, "cos " + shape_str(cos) + " and sin " + shape_str(sin) + " differ");
-      if (cos->shape[1] < 1 || 2 * cos->shape[1] > D)
-        return fail(BD_ERR_SHAPE, "cos and sin must have 1 to head_dim/2 columns, got " + std::to_string(cos->shape[1]));
-      if (cos->shape[0] > (int64_t(1) << 30)) return fail(BD_ERR_SHAPE, "cos has more than 2^30 rows");
-      if (cos->shape[1] > 1 && (cos->stride[1] != 1 || sin->stride[1] != 1))
-        return fail(BD_ERR_STRIDE, "cos and sin rows must be contiguous");
-      p.cos = static_cast<const float*>(cos->data); p.sin = static_cast<const float*>(sin->data);
-      p.c_s = cos->stride[0]; p.s_s = sin->stride[0];
-      p.positions = int(cos->shape[0]); p.half = int(cos->shape[1]);
-    }
-    const bool fp8 = k_cache->dtype == BD_F8E4M3;
-    if (!(k_scale > 0.f) || !(v_scale > 0.f)) return fail(BD_ERR_VALUE, "k_scale and v_scale must be positive");
-    if (!fp8 && (k_scale != 1.f || v_scale != 1.f))
-      return fail(BD_ERR_VALUE, "k_scale and v_scale belong to an fp8 cache");
-    if (T == 0) return BD_OK;
-    p.k = rows_of(k); p.v = rows_of(v);
-    p.k_cache = k_cache->data; p.v_cache = v_cache->data;
-    p.T = int(T); p.in_dtype = k->dtype; p.cache_dtype = k_cache->dtype;
-    p.interleaved = interleaved != 0;
-    p.cu = cu_seqlens ? static_cast<const int*>(cu_seqlens->data) : nullptr;
-    p.k_inv = 1.f / k_scale; p.v_inv = 1.f / v_scale;
-    const int items = int(D / 16);
-    const bool vector = D % 16 == 0 && items <= 16 && !(items & (items - 1)) && p.half % 8 == 0 && by_eight(k) &&
-                        by_eight(v) && (!q || (by_eight(q) && by_eight(q_out))) && by_eight(k_cache) &&
-                        by_eight(v_cache) && (!cos || (by_eight(cos) && by_eight(sin)));
-    if (vector) return launch_append(p, stream);
-    return launch_pdl(paged_append_generic_kernel, dim3(unsigned(T)), dim3(128), 0, stream,
-                      "paged_append_generic_kernel launch", p);
+    AppendCall append;
+    SummaryCall sum;  // what the second half refuses is refused before the first is launched
+    if ((rc = plan_append(k, v, q, cos, sin, interleaved, cu_seqlens, block_table, context_lens, k_scale, v_scale,
+                          k_cache, v_cache, q_out, &append)) ||
+        (rc = plan_summary(k_cache, block_table, context_lens, append.p.T ? cu_seqlens : nullptr, append.p.T, k_scale,
+                           summary, summary_scale, &sum)) ||
+        append.p.T == 0 || (rc = run_append(append, stream)))
+      return rc;
+    return launch_summary(sum, stream);
   });
 }
 
@@ -703,33 +783,10 @@ int bd_paged_block_summary(const bd_tensor* k_cache, const bd_tensor* block_tabl
                            const bd_tensor* summary_scale, bd_stream_t stream) {
   using namespace bd;
   return guarded([&]() -> int {
-    int rc;
-    SummaryParams p{};
-    if ((rc = check_paged(k_cache, nullptr, block_table, context_lens, &p.g))) return rc;
-    if ((rc = check_tensor(summary, "summary", 4, BD_I8)) || (rc = check_tensor(summary_scale, "summary_scale", 2, BD_F32)))
-      return rc;
-    if (summary->shape[0] != p.g.num_blocks || summary->shape[1] != p.g.Hk || summary->shape[2] != 2 ||
-        summary->shape[3] != p.g.D)
-      return fail(BD_ERR_SHAPE, "summary " + shape_str(summary) + " must be [num_blocks, Hk, 2, D] of the cache");
-    if (summary_scale->shape[0] != p.g.num_blocks || summary_scale->shape[1] != p.g.Hk)
-      return fail(BD_ERR_SHAPE, "summary_scale " + shape_str(summary_scale) + " must be [num_blocks, Hk]");
-    if (summary->stride[3] != 1 || summary->stride[2] != p.g.D)
-      return fail(BD_ERR_STRIDE, "summary's last two dims must be contiguous");
-    if (!(k_scale > 0.f)) return fail(BD_ERR_VALUE, "k_scale must be positive");
-    if (k_cache->dtype != BD_F8E4M3 && k_scale != 1.f) return fail(BD_ERR_VALUE, "k_scale belongs to an fp8 cache");
-    if (new_tokens < 0) return fail(BD_ERR_VALUE, "new_tokens must not be negative");
-    if (cu_seqlens && new_tokens == 0) return fail(BD_ERR_VALUE, "cu_seqlens goes with new_tokens");
-    if (new_tokens > 0 && (rc = check_cu(cu_seqlens, p.g, new_tokens))) return rc;
-    p.k_cache = k_cache->data; p.dtype = k_cache->dtype;
-    p.code = static_cast<int8_t*>(summary->data); p.c_sb = summary->stride[0]; p.c_sh = summary->stride[1];
-    p.scale = static_cast<float*>(summary_scale->data);
-    p.s_sb = summary_scale->stride[0]; p.s_sh = summary_scale->stride[1];
-    p.k_scale = k_scale; p.T = new_tokens;
-    p.cu = cu_seqlens ? static_cast<const int*>(cu_seqlens->data) : nullptr;
-    const bool types = p.dtype == BD_BF16 || p.dtype == BD_F16 || p.dtype == BD_F8E4M3;
-    const bool vector = types && (p.g.D == 64 || p.g.D == 128 || p.g.D == 256) && !check_rows_aligned(k_cache, "k_cache") &&
-                        !((reinterpret_cast<uintptr_t>(p.code) | size_t(p.c_sb) | size_t(p.c_sh)) & 15);
-    return launch_summary(p, vector, stream);
+    SummaryCall sum;
+    const int rc = plan_summary(k_cache, block_table, context_lens, cu_seqlens, new_tokens, k_scale, summary,
+                                summary_scale, &sum);
+    return rc ? rc : launch_summary(sum, stream);
   });
 }
 

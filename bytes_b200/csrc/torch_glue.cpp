@@ -150,8 +150,7 @@ bd_tensor desc_row(const at::Tensor& t, int device) {
   return t.dim() == 4 && t.size(2) == 1 ? desc_drop2(t, device) : desc(t, device);
 }
 
-// bd_paged_append, then bd_paged_block_summary of the touched pages when a summary is kept
-// -> (status, rotated queries or None).
+// bd_paged_append, or bd_paged_append_summary when a summary is kept -> (status, rotated queries or None).
 std::tuple<int64_t, Opt> paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
                                       const at::Tensor& v_cache, const at::Tensor& table_, const at::Tensor& lens_,
                                       const Opt& q, const Opt& cos, const Opt& sin, bool interleaved, const Opt& cu_,
@@ -168,10 +167,11 @@ std::tuple<int64_t, Opt> paged_append(const at::Tensor& k, const at::Tensor& v, 
   Opt q_out;
   if (dq.p) q_out = at::empty(q->sizes(), q->options());
   const OptDesc dqo(q_out, dev);
-  int rc = bd_paged_append(&dk, &dv, dq.p, dcos.p, dsin.p, interleaved, dcu.p, &dt, &dl, float(k_scale),
-                           float(v_scale), &dkc, &dvc, dqo.p, st);
-  if (rc == 0 && ds.p && k.size(0) > 0)
-    rc = bd_paged_block_summary(&dkc, &dt, &dl, dcu.p, int(k.size(0)), float(k_scale), ds.p, dss.p, st);
+  const int rc = ds.p || dss.p
+                     ? bd_paged_append_summary(&dk, &dv, dq.p, dcos.p, dsin.p, interleaved, dcu.p, &dt, &dl,
+                                               float(k_scale), float(v_scale), &dkc, &dvc, dqo.p, ds.p, dss.p, st)
+                     : bd_paged_append(&dk, &dv, dq.p, dcos.p, dsin.p, interleaved, dcu.p, &dt, &dl, float(k_scale),
+                                       float(v_scale), &dkc, &dvc, dqo.p, st);
   return {rc, q_out};
 }
 

@@ -352,7 +352,8 @@ int bd_asym_fakequant(const bd_tensor* x, int levels, const bd_tensor* y, bd_str
  * (last two dims contiguous) holds rint(min / s) and rint(max / s) over the page's tokens of each
  * channel of k_scale * key, summary_scale f32 [num_blocks,Hk] s = max|.| / 127. new_tokens = 0:
  * every page that holds tokens; T > 0: the pages that the last T appended tokens (cu_seqlens as
- * above) lie in.
+ * above) lie in. bd_paged_append_summary is bd_paged_append, then bd_paged_block_summary of the pages
+ * that its tokens lie in; what either refuses is refused before anything is written.
  *
  * bd_paged_select chooses pages for one new token a sequence from the summaries. With q8 =
  * rint(q * (127 / max|q|)), s_q = max|q| / 127 per query head: I = sum_d max(q8 min8, q8 max8),
@@ -375,6 +376,11 @@ int bd_paged_append(const bd_tensor* k, const bd_tensor* v, const bd_tensor* q, 
                     const bd_tensor* sin, int interleaved, const bd_tensor* cu_seqlens, const bd_tensor* block_table,
                     const bd_tensor* context_lens, float k_scale, float v_scale, const bd_tensor* k_cache,
                     const bd_tensor* v_cache, const bd_tensor* q_out, bd_stream_t stream);
+int bd_paged_append_summary(const bd_tensor* k, const bd_tensor* v, const bd_tensor* q, const bd_tensor* cos,
+                            const bd_tensor* sin, int interleaved, const bd_tensor* cu_seqlens,
+                            const bd_tensor* block_table, const bd_tensor* context_lens, float k_scale, float v_scale,
+                            const bd_tensor* k_cache, const bd_tensor* v_cache, const bd_tensor* q_out,
+                            const bd_tensor* summary, const bd_tensor* summary_scale, bd_stream_t stream);
 int bd_paged_block_summary(const bd_tensor* k_cache, const bd_tensor* block_table, const bd_tensor* context_lens,
                            const bd_tensor* cu_seqlens, int new_tokens, float k_scale, const bd_tensor* summary,
                            const bd_tensor* summary_scale, bd_stream_t stream);

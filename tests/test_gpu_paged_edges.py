@@ -46,3 +46,23 @@ def test_lengths_changed_right_before_a_captured_call(cuda, lens):
             assert torch.equal(bits(a), bits(b))
         for b in (now == 0).nonzero()[:, 0].tolist():
             assert (kept[0][b] == 0).all() and (kept[1][b] == 0).all()
+
+
+# ------------------------------------------------------------------------------------ refusals
+@pytest.mark.parametrize("tokens", [2, 0])
+def test_a_refused_append_has_written_nothing(cuda, tokens):
+    nb, Hk, D, block = 6, 2, 64, 16
+    kc = torch.zeros(nb, Hk, block, D, dtype=BF16, device=cuda)
+    vc = torch.zeros_like(kc)
+    table = torch.arange(6, dtype=torch.int32, device=cuda).view(2, 3)[:tokens]
+    lens = torch.ones(tokens, dtype=torch.int32, device=cuda)
+    k = torch.ones(tokens, Hk, D, dtype=BF16, device=cuda)
+    code, scale = paged.new_block_summary(kc)
+    for c, s in ((code[:1], scale), (code.float(), scale), (code, scale[:, :1]), (code, scale.double().half()),
+                 (code.transpose(2, 3).contiguous().transpose(2, 3), scale), (code.cpu(), scale)):
+        with pytest.raises(ValueError):
+            paged.paged_append(k, k, kc, vc, table, lens, summary=c, summary_scale=s)
+    torch.cuda.synchronize()
+    assert not kc.any() and not vc.any() and not code.any()
+    paged.paged_append(k, k, kc, vc, table, lens, summary=code, summary_scale=scale)
+    assert bool(kc.any()) == bool(code.any()) == (tokens > 0)

@@ -1,0 +1,33 @@
+"""Host checks of the paged-cache entry points at their edges (no GPU): refused before any launch."""
+import pytest
+import torch
+
+from bytes_b200 import _native as N
+from test_paged_cpu import F, I, at, cache, fake
+
+
+def append_summary(code=None, scale=None, tokens=3, kc=None, k_scale=1.0):
+    c = cache()
+    kc = kc or c["k"]
+    if tokens == 0:
+        c["table"], c["lens"] = fake((0, 4), N.BD_I32), fake((0,), N.BD_I32)
+    k = fake((tokens, 2, 64), N.BD_BF16)
+    f = N.lib().bd_paged_append_summary
+    f.restype = I
+    return f(at(k), at(k), None, None, None, I(0), None, at(c["table"]), at(c["lens"]), F(k_scale), F(1.0), at(kc),
+             at(fake((6, 2, 16, 64), kc.dtype)), None, at(code), at(scale), None)
+
+
+@pytest.mark.parametrize("tokens", [3, 0])
+def test_append_with_a_bad_summary_is_refused_as_a_whole(tokens):
+    """The summary's own refusal comes before the append's launch, which without a GPU would answer 8 (BD_ERR_CUDA)."""
+    if torch.cuda.is_available() and tokens:
+        pytest.skip("made-up pointers: only where nothing can be launched")
+    code, scale = fake((6, 2, 2, 64), N.BD_I8), fake((6, 2), N.BD_F32)
+    assert append_summary(code, scale, tokens) == (8 if tokens else 0)
+    assert append_summary(fake((5, 2, 2, 64), N.BD_I8), scale, tokens) == 3
+    assert append_summary(fake((6, 2, 2, 64), N.BD_F32), scale, tokens) == 2
+    assert append_summary(fake((6, 2, 2, 64), N.BD_I8, strides=(256, 128, 1, 2)), scale, tokens) == 4
+    assert append_summary(code, fake((6, 3), N.BD_F32), tokens) == 3
+    assert append_summary(code, None, tokens) == 1
+    assert append_summary(None, scale, tokens) == 1
