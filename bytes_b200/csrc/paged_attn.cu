@@ -3,7 +3,8 @@
 //
 // out_h = sum_t p_t v_t / sum_t p_t * v_scale, p_t = exp(scaling * k_scale * q_h.k_t - max),
 // t < context_len and, with a choice, t in a chosen page. Running maximum and sum, scores and
-// sums in 32 bits. A row with no token gives zeros (and lse = -inf).
+// sums in 32 bits. A row with no token gives zeros (and lse = -inf), and so does one all of whose scores are -inf. A
+// score that is NaN or +inf makes its row NaN.
 #include "paged.cuh"
 #include "decode_shared.cuh"
 
@@ -94,7 +95,8 @@ __global__ void __launch_bounds__(kGenWarps * 32) paged_attn_generic_kernel(cons
       for (int i = 0; i < 8; ++i) s = fmaf(q[h][i], k[i], s);
       s = warp_sum(s) * p.scale_log2;
       const float mn = fmaxf(m[h], s);
-      const float a = mn == -INFINITY ? 1.f : exp2f(m[h] - mn), w = mn == -INFINITY ? 0.f : exp2f(s - mn);
+      // (fmaxf passes a score over that is NaN; its weight is NaN all the same)
+      const float a = mn == -INFINITY ? 1.f : exp2f(m[h] - mn), w = s == -INFINITY ? 0.f : exp2f(s - mn);
       m[h] = mn;
       l[h] = fmaf(l[h], a, w);
 #pragma unroll
@@ -121,7 +123,7 @@ __global__ void __launch_bounds__(kGenWarps * 32) paged_attn_generic_kernel(cons
     }
     const int64_t at = (int64_t(b) * p.Hq + hk * p.G + h0 + h) * p.n_splits + split;
     p.part_o[at * D + d] = O;
-    if (d == 0) { p.part_m[at] = M; p.part_l[at] = L; }
+    if (d == 0) { p.part_m[at] = L != L ? 0.f : M; p.part_l[at] = L; }  // a sum that is NaN is not passed over for its maximum
   }
 }
 
@@ -809,7 +811,8 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         lrow[nt][j] = lost ? NAN : l;
-        mrow[nt][j] = lost ? 0.f : mrow[nt][j] - kUp;  // of sums that are 2^kUp times as large
+        // of sums that are 2^kUp times as large; a sum that is NaN is not passed over for its maximum
+        mrow[nt][j] = lost || l != l ? 0.f : mrow[nt][j] - kUp;
       }
     if (one_row) break;  // the warp's only row: joined with the others' parts below
     if (whole) {

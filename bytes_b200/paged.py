@@ -101,9 +101,10 @@ def paged_decode_attn(q, k_cache, v_cache, block_table, context_lens, scaling, *
 
     q [B, H_q, D] or [B, H_q, 1, D] (bf16 / f16 / f32) -> the same shape and type; query head h reads KV
     head h // (H_q / H_k). ``selected`` int32 [B, H_k, n] (as ``paged_select_blocks`` gives it) limits each KV
-    head to those logical pages. Sequences without a token give zeros. With ``return_lse`` also the
-    natural log of the softmax denominator, f32 [B, H_q] (-inf without a token), to join parts of a
-    sequence held elsewhere.
+    head to those logical pages. Sequences without a token give zeros, and so do rows all of whose scores
+    are -inf; a score that is NaN or +inf makes its row NaN. With ``return_lse`` also the natural log of the
+    softmax denominator, f32 [B, H_q] (-inf for such rows of zeros), to join parts of a sequence held
+    elsewhere.
     """
     _check_row(q)
     rc, out, lse = N.glue().paged_decode_attn(q, k_cache, v_cache, block_table,

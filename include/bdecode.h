@@ -366,7 +366,8 @@ int bd_asym_fakequant(const bd_tensor* x, int levels, const bd_tensor* y, bd_str
  * v_scale over a sequence's tokens, or over those of its chosen pages (selected int32
  * [B,Hk,pages], NULL: all; entries that hold no token do not count, duplicates count once per
  * occurrence). lse f32 [B,Hq] (may be NULL) = natural log of the softmax denominator. A row
- * without a token gives zeros and lse = -inf. q [B,Hq,D] bf16/f16/f32.
+ * without a token gives zeros and lse = -inf, and so does one all of whose scores are -inf; a score that is
+ * NaN or +inf makes its row NaN (lse too). q [B,Hq,D] bf16/f16/f32.
  *
  * bd_paged_sparse_decode_attn: bd_paged_select into `selected`, then bd_paged_decode_attn over it.
  * ref: none -- the reference pages its PQ caches only (paged_attn_pq_lut_kv,

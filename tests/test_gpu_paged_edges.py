@@ -66,3 +66,76 @@ def test_a_refused_append_has_written_nothing(cuda, tokens):
     assert not kc.any() and not vc.any() and not code.any()
     paged.paged_append(k, k, kc, vc, table, lens, summary=code, summary_scale=scale)
     assert bool(kc.any()) == bool(code.any()) == (tokens > 0)
+
+
+# ---------------------------------------------------------------------------- not quite numbers
+FORMS = {  # lengths; q heads, kv heads, D, block, q, cache
+    "a cluster a row": ([1, 40, 700, 2000], 8, 2, 128, 16, BF16, BF16),
+    "a cluster a row, f16": ([1, 40, 700, 2000], 20, 2, 64, 8, F16, F16),
+    "a cluster a row, 8-bit": ([1, 40, 700, 2000], 8, 2, 128, 16, BF16, FP8),
+    "shared out, joined by rows": ([1, 40, 700, 9000] + [300] * 36, 8, 2, 128, 16, BF16, BF16),
+    "shared out, joined by cuts": ([1, 40, 700, 9000] + [100] * 530, 8, 2, 64, 16, F16, FP8),
+    "any type": ([1, 40, 700, 2000], 8, 2, 128, 16, F32, BF16),
+    "any head dim": ([1, 40, 700, 9000], 6, 3, 40, 5, F16, F16),
+}
+
+
+def check_rows(q, kc, vc, table, lens, ks, vs, cuda):
+    """As check_attention, where a row of the plain form may be NaN."""
+    scaling = q.shape[-1] ** -0.5
+    want, want_lse, weight, reach = plain.decode_attn(q, kc, vc, table, lens, scaling, ks, vs)
+    got, lse = paged.paged_decode_attn(q.to(cuda), kc.to(cuda), vc.to(cuda), table.to(cuda), lens.to(cuda), scaling,
+                                       k_scale=ks, v_scale=vs, return_lse=True)
+    got, lse = got.double().cpu(), lse.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(lse.isnan(), want_lse.isnan())
+    # (a value that is NaN leaves its row's other channels as they are, but not the bound of the whole)
+    good = ~want.isnan()
+    score = ((q.shape[-1] + 4) * 2.0 ** -23 * reach)[..., None].expand_as(want)
+    p = 0.0 if kc.dtype == F32 or q.dtype == F32 else torch.finfo(BF16 if kc.dtype == BF16 else F16).eps / 2
+    unit = torch.finfo(q.dtype).eps / 2
+    tol = (p + 2 * score + 2.0 ** -16) * weight + unit * want.abs() * 1.01 + 2.0 ** -25
+    assert ((got - want).abs() <= tol)[good].all()
+
+
+@pytest.mark.parametrize("where", ["first", "last", "all"])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_live_nan_reaches_its_rows_and_no_others(cuda, form, where):
+    """A key that is NaN makes the rows of its KV head NaN wherever it lies, a value only its channel of them."""
+    lens, Hq, Hk, D, block, qdt, cdt = FORMS[form]
+    q, kc, vc, table, clen, ks, vs = attention_inputs(lens, Hq, Hk, D, block, qdt, cdt, 31)
+    nan = torch.tensor(float("nan")).to(cdt)
+
+    def at(b):
+        t = {"first": [0], "last": [lens[b] - 1], "all": range(lens[b])}[where]
+        return [(int(table[b, i // block]), i % block) for i in t]
+
+    for b, h in ((0, 0), (1, 1), (3, 1)):
+        for page, row in at(b):
+            kc[page, h, row, D // 2] = nan
+    for page, row in at(2):
+        vc[page, 0, row, 3] = nan
+    check_rows(q, kc, vc, table, clen, ks, vs, cuda)
+
+
+@pytest.mark.parametrize("form", [f for f in FORMS if FORMS[f][-1] != FP8])
+def test_scores_of_infinity(cuda, form):
+    """-inf throughout: a row of zeros. -inf in some tokens: they have no weight. +inf: NaN, as inf - inf is."""
+    lens, Hq, Hk, D, block, qdt, cdt = FORMS[form]
+    q, kc, vc, table, clen, ks, vs = attention_inputs(lens, Hq, Hk, D, block, qdt, cdt, 32)
+    q[..., 1] = q[..., 1].abs() + 0.5  # the sign of an infinite score is its key's
+    for b, every, to in ((0, 1, -math.inf), (1, 1, -math.inf), (2, 3, -math.inf), (3, 1000, math.inf)):
+        for i in range(0, lens[b], every):
+            kc[int(table[b, i // block]), :, i % block, 1] = to
+    keep = [0, 1]
+    got, lse = paged.paged_decode_attn(q.to(cuda), kc.to(cuda), vc.to(cuda), table.to(cuda), clen.to(cuda), D ** -0.5,
+                                       return_lse=True)
+    assert (got[keep] == 0).all() and (lse[keep] == -math.inf).all()
+    want, want_lse, weight, _ = plain.decode_attn(q, kc, vc, table, clen, D ** -0.5)
+    assert want[3].isnan().all() and got[3].isnan().all() and lse[3].isnan().all()
+    # sequence 2 as if every third token were not there
+    assert not want[2].isnan().any()
+    reach = (q[2].double().abs().amax(-1) * 16).max() * D ** 0.5  # |k| < 16, some sum of |q k| at most
+    p = 0.0 if F32 in (qdt, cdt) else torch.finfo(BF16 if cdt == BF16 else F16).eps / 2
+    tol = (p + 2 * (D + 4) * 2.0 ** -23 * reach + 2.0 ** -16) * weight[2] + torch.finfo(qdt).eps / 2 * want[2].abs() * 1.01 \
+        + 2.0 ** -25
+    assert ((got[2].double().cpu() - want[2]).abs() <= tol).all()
