@@ -622,20 +622,22 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
       }
     }
     if (FP8 && p.q_dtype == BD_BF16) {
-      // as f16 times a power of two that puts the largest at 2^14..2^15 (exact down to 2^-31 of it)
+      // as f16 times a power of two that puts the largest finite one of these heads at 2^14..2^15 (exact down to 2^-31
+      // of it; infinities stay what they are)
       float amax = 0.f;
+      auto finite = [](float x) { return fabsf(x) <= FLT_MAX ? fabsf(x) : 0.f; };
 #pragma unroll
       for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(qb[kk][nt][i] << 16)),
-                                     fabsf(__uint_as_float(qb[kk][nt][i] & 0xffff0000u))));
+            amax = fmaxf(amax, fmaxf(finite(__uint_as_float(qb[kk][nt][i] << 16)),
+                                     finite(__uint_as_float(qb[kk][nt][i] & 0xffff0000u))));
       amax = warp_max(amax);
       int ex = 0;
       frexpf(amax, &ex);
-      const int shift = amax > 0.f && amax <= FLT_MAX ? max(ex - 15, -100) : 0;
+      const int shift = amax > 0.f ? max(ex - 15, -100) : 0;
       const float f = ldexpf(1.f, -shift);
       mul = ldexpf(p.scale_log2, shift);
 #pragma unroll

@@ -139,3 +139,15 @@ def test_scores_of_infinity(cuda, form):
     tol = (p + 2 * (D + 4) * 2.0 ** -23 * reach + 2.0 ** -16) * weight[2] + torch.finfo(qdt).eps / 2 * want[2].abs() * 1.01 \
         + 2.0 ** -25
     assert ((got[2].double().cpu() - want[2]).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("heads", [4, 12])
+@pytest.mark.parametrize("lens", [[40, 700], [9000, 3]])
+def test_infinite_query_beside_large_ones(cuda, heads, lens):
+    """Over an 8-bit cache a KV head's bf16 queries share a power of two: one that is infinite makes its own row NaN and
+    leaves the others, which f16 could not hold unscaled, what they are."""
+    q, kc, vc, table, clen, _, vs = attention_inputs(lens, 2 * heads, 2, 128, 16, BF16, FP8, 33)
+    q = (q.float() * 1e5).bfloat16()
+    q[0, 1, 5] = math.inf
+    q[1, 0, 7] = float("nan")
+    check_rows(q, kc, vc, table, clen, 1e-6, vs, cuda)
