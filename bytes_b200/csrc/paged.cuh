@@ -11,8 +11,8 @@ namespace bd {
 // the lengths, and write what depends on these alone (rows without a token, the notes for a join), ahead of their wait.
 // That rests on this: whoever wrote the lengths came before the call; the call's first kernel waits in all its CTAs
 // for what came before, to its end and in memory, and only then lets the next begin; a later one does so once it has
-// begun itself. The lengths are read from L2, as an SM's L1 may hold them from an earlier step (paged_len). With the
-// waits ahead of these reads 24 sequences of 1 to 3001 tokens take 15.5 us against 13.5, choice and attention of 16
+// begun itself. Such early reads are made from L2, as an SM's L1 may hold the lengths from an earlier step. With the
+// waits ahead of these reads 24 sequences of 1 to 3001 tokens take 15.5 us against 13.7, choice and attention of 16
 // sequences 38.0 against 37.3.
 // A kernel lets the next one begin early only where that is a part of the same call or usually follows it, the choice
 // after its scores only, and the attention of a cluster a row not at all: CTAs of another call that come early crowd on
@@ -29,9 +29,10 @@ struct PagedGeometry {
   int64_t v_sb, v_sh, v_st, v_sd;
 };
 
-// Tokens a sequence holds: its length, cut to what the block table can address. Read from L2 (see above).
-__device__ __forceinline__ int paged_len(const PagedGeometry& g, int b) {
-  const int n = __ldcg(g.lens + int64_t(b) * g.l_s);
+// Tokens a sequence holds: its length, cut to what the block table can address. early: read ahead of the kernel's wait.
+__device__ __forceinline__ int paged_len(const PagedGeometry& g, int b, bool early = false) {
+  const int* at = g.lens + int64_t(b) * g.l_s;
+  const int n = early ? __ldcg(at) : *at;
   const int64_t cap = int64_t(g.wide) * g.block;
   return n < 0 ? 0 : (int64_t(n) > cap ? int(cap) : n);
 }

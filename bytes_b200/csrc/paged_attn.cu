@@ -242,7 +242,7 @@ struct ListSums {
   __device__ __forceinline__ void build(const AttnParams& p, GroupSums& g, int warp, int lane) {
     const int per = p.g.Hk * p.chunks;
     if (p.g.B <= 32) {
-      len = lane < p.g.B ? paged_len(p.g, lane) : 0;
+      len = lane < p.g.B ? paged_len(p.g, lane, p.after_select) : 0;
       sum = warp_prefix(row_slots(p, len) * per, lane);
       total = __shfl_sync(0xffffffffu, sum, 31);
       return;
@@ -254,7 +254,7 @@ struct ListSums {
     for (int i = first + lane; i - lane < min(groups, first + each); i += 32) {
       int n = 0;
       if (i < groups)
-        for (int b = i * size; b < min(p.g.B, (i + 1) * size); ++b) n += row_slots(p, paged_len(p.g, b));
+        for (int b = i * size; b < min(p.g.B, (i + 1) * size); ++b) n += row_slots(p, paged_len(p.g, b, p.after_select));
       n = warp_prefix(n * per, lane) + carry;
       if (i < groups) g.sum[i] = n;
       carry = __shfl_sync(0xffffffffu, n, 31);
@@ -338,7 +338,7 @@ struct Place {
     int b0 = i * l.size;
 #pragma unroll 1
     for (;;) {  // the group's sequences
-      const int length = paged_len(p.g, b0), n = row_slots(p, length) * per;
+      const int length = paged_len(p.g, b0, p.after_select), n = row_slots(p, length) * per;
       if (at < n) {
         within(p, b0, length, at);
         return;
@@ -363,7 +363,7 @@ struct Place {
     hk = 0;
     do {
       ++b;
-      len = paged_len(p.g, b);
+      len = paged_len(p.g, b, p.after_select);
       slots = row_slots(p, len);
     } while (slots == 0 && b + 1 < p.g.B);
     return true;
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
   if (p.row_mode) {   // a cluster has a row
     one_row = true;
     const int per = p.g.Hk * p.chunks, row = blockIdx.x / p.row_mode, rank = blockIdx.x - row * p.row_mode;
-    const int b = row / per, len = paged_len(p.g, b), slots = row_slots(p, len);
+    const int b = row / per, len = paged_len(p.g, b, p.after_select), slots = row_slots(p, len);
     if (slots == 0) {  // (the same for all of the cluster's CTAs)
       const int hc = row - b * per, hk = hc / p.chunks, chunk = hc - hk * p.chunks;
       const int nheads = min(NH, p.G - chunk * NH);
@@ -1027,13 +1027,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_tile_join_kernel(const Att
   const int part = threadIdx.x % PER, slice = threadIdx.x / (PER * HEADS), lane = threadIdx.x & 31;
   const int hl = threadIdx.x / PER % HEADS, h = (blockIdx.x - hc * groups) * HEADS + hl;
   const bool some = h < p.heads && chunk * p.heads + h < p.G;  // a head of this row
+  const int slots = row_slots(p, paged_len(p.g, b, true));
   int all = 0, before = 0;  // slots of all sequences, and of those before this one
   for (int i = lane; i < p.g.B; i += 32) {
-    const int n = row_slots(p, paged_len(p.g, i));
+    const int n = row_slots(p, paged_len(p.g, i, true));
     all += n;
     if (i < b) before += n;
   }
-  const int per = p.g.Hk * p.chunks, slots = row_slots(p, paged_len(p.g, b));
+  const int per = p.g.Hk * p.chunks;
   const Shares<WARPS> sh(__reduce_add_sync(0xffffffffu, all) * per, p.warps);
   const int s0 = __reduce_add_sync(0xffffffffu, before) * per + hc * slots;
   const Parts<WARPS> parts(sh, s0, s0 + max(slots, kRowCost + 1));
@@ -1065,7 +1066,7 @@ __global__ void __launch_bounds__(kCutsThreads) paged_tile_join_cuts_kernel(cons
   const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // sequences without a token
   for (int b = c * JW + warp; b < p.g.B; b += gridDim.x * JW)
-    if (row_slots(p, paged_len(p.g, b)) == 0)
+    if (row_slots(p, paged_len(p.g, b, true)) == 0)
       for (int i = lane; i < p.Hq * PER; i += 32) Sum4::none().write(p, b, i / PER, i % PER);
   griddep_wait();  // also for a kernel that waits for this one: it then finds the tile kernel done as well
   // warps 1.. the borders within the share, then all of them the one before it

@@ -53,8 +53,12 @@ def test_aligned_cluster_barriers_have_their_warps_together(path):
 
 
 def test_lengths_that_are_read_ahead_of_a_wait_come_from_l2():
-    """The joins, and the attention after a choice, read the lengths before they wait for the kernel ahead of them: past
-    L1, which may hold them from an earlier step."""
-    geometry = code(os.path.join(CSRC, "paged.cuh"))
-    assert [m.group(1) for m in re.finditer(r"(\S+)\blens\b[^;]*l_s\)?;", geometry)] == ["__ldcg(g."]
-    assert not re.search(r"\blens\s*\[|\blens\s*\+", code(os.path.join(CSRC, "paged_attn.cu")))
+    """The joins, and the tile kernel after a choice, read the lengths before they wait for the kernel ahead of them: past
+    L1, which may hold them from an earlier step. Nothing in that file reads them in another way."""
+    assert "early ? __ldcg(at) : *at" in code(os.path.join(CSRC, "paged.cuh"))
+    attn = code(os.path.join(CSRC, "paged_attn.cu"))
+    assert not re.search(r"\blens\s*[\[+]", attn)
+    tiles, joins = attn.index("int row_slots"), attn.index("struct Parts")
+    for m in re.finditer(r"paged_len\(([^()]*)\)", attn):
+        early = m.group(1).split(",")[2:]
+        assert early == ([] if m.start() < tiles else [" p.after_select"] if m.start() < joins else [" true"])
