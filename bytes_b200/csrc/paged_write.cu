@@ -6,7 +6,8 @@
 // type): channels (i, i + r/2), or (2i, 2i+1) when interleaved, of the first r channels:
 //   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin,  cos/sin row = the token's position.
 // Summary of a page and KV head: channelwise min and max of the stored keys times k_scale, as
-// int8 code = rint(x / s), s = max|.| / 127.
+// int8 code = rint(x / s), s = max|.| / 127. Keys that are NaN do not count, a channel of nothing else is zero; max|.| is
+// the largest finite fp32 number at most, so that the code of an infinity is 127 (or -127).
 #include "paged.cuh"
 #include "decode_shared.cuh"
 
@@ -366,7 +367,7 @@ __device__ __forceinline__ bool page_of_item(const SummaryParams& p, int64_t ite
 }
 
 __device__ __forceinline__ int8_t code_of(float x, float s, bool some) {
-  return some ? int8_t(max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))))) : int8_t(0);
+  return some ? int8_t(max(-127, min(127, __float2int_rn(__fdiv_rn(x, s))))) : int8_t(0);  // (NaN: 0)
 }
 
 // Any type, stride and head dim: one warp per (page, KV head), a lane every 32nd channel. For what the vector form
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(128) paged_summary_generic_kernel(const Summar
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int d = lane + 32 * i;
-    lo[i] = INFINITY; hi[i] = -INFINITY;
+    lo[i] = hi[i] = NAN;  // which gives way to any number
     if (d >= p.g.D) continue;
     for (int r = 0; r < n; ++r) {
       const float x = __fmul_rn(load_as(p.k_cache, p.dtype, base + r * p.g.k_st + d * p.g.k_sd), p.k_scale);
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(128) paged_summary_generic_kernel(const Summar
     }
     top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
   }
-  top = fminf(warp_max(top), FLT_MAX);  // an infinite key keeps its page at the top, not at NaN
+  top = fminf(warp_max(top), FLT_MAX);
   const float s = __fdiv_rn(top, 127.f);
   int8_t* code = p.code + page * p.c_sb + h * p.c_sh;
 #pragma unroll
@@ -474,10 +475,7 @@ __global__ void __launch_bounds__(256, 2) paged_summary_kernel(const SummaryPara
   V lo[NP], hi[NP];
   auto reset = [&]() {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      lo[i] = P::bits(std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u);
-      hi[i] = P::bits(std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
-    }
+    for (int i = 0; i < NP; ++i) lo[i] = hi[i] = P::bits(0x7fff7fffu);  // NaN, which gives way to any number
   };
   auto finish = [&](const Item& it) {
 #pragma unroll
@@ -491,13 +489,13 @@ __global__ void __launch_bounds__(256, 2) paged_summary_kernel(const SummaryPara
 #pragma unroll
     for (int e = 1; e < NP; ++e) far = __hmax2(far, __hmax2(hi[e], __hneg2(lo[e])));
     const float2 f = P::wide(far);
-    float top = fmaxf(fabsf(f.x), fabsf(f.y));
+    float top = fmaxf(fmaxf(f.x, f.y), 0.f);
     if (FP8) top = __fmul_rn(top, p.k_scale);
     top = fminf(warp_max(top), FLT_MAX);
     const float s = __fdiv_rn(top, 127.f), inv = top > 0.f ? __fdiv_rn(1.f, s) : 0.f;
     // rint(x / s), the quotient rounded to 32 bits first: x * inv is within 2^-15 of it, so that it rounds to
     // the same whole number (by the sum with 1.5 * 2^23, whose low byte it then is) unless it comes near
-    // half of one; then, and for infinities, the division is made
+    // half of one; then, and for infinities and NaN, the division is made
     constexpr float kMagic = 12582912.f;
     auto put = [&](const V* v, int8_t* to) {
       uint32_t u[NP / 2];
@@ -510,7 +508,7 @@ __global__ void __launch_bounds__(256, 2) paged_summary_kernel(const SummaryPara
         for (int i = 0; i < 4; ++i) {
           if (FP8) x[i] = __fmul_rn(x[i], p.k_scale);
           t[i] = fmaf(x[i], inv, kMagic);
-          near |= fabsf(fmaf(x[i], inv, kMagic - t[i])) > 0.499f;
+          near |= !(fabsf(fmaf(x[i], inv, kMagic - t[i])) <= 0.499f);
         }
         u[e] = prmt(prmt(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040),
                     prmt(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);

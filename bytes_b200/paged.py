@@ -62,7 +62,8 @@ def paged_block_summary(k_cache, block_table, context_lens, summary, summary_sca
     """Renew the summaries of every page that holds tokens of the sequences, in place.
 
     Per page and KV head, over the page's tokens: channelwise minimum and maximum of k_scale * key as
-    int8 codes rint(x / s), s = max|x| / 127. ``paged_append`` keeps them page by page; this rebuilds
+    int8 codes rint(x / s), s = max|x| / 127. Keys that are NaN do not count (a channel of nothing else is
+    zero); the largest finite fp32 number stands for an infinite max|x|. ``paged_append`` keeps them page by page; this rebuilds
     them for pages that came from elsewhere (a copied prefix, a swapped-in sequence). A page that several
     sequences share is summarised once for each of them, so it should be full in all.
     """

@@ -350,7 +350,8 @@ int bd_asym_fakequant(const bd_tensor* x, int levels, const bd_tensor* y, bd_str
  *
  * bd_paged_block_summary writes the 8-bit summary of pages' keys: summary i8 [num_blocks,Hk,2,D]
  * (last two dims contiguous) holds rint(min / s) and rint(max / s) over the page's tokens of each
- * channel of k_scale * key, summary_scale f32 [num_blocks,Hk] s = max|.| / 127. new_tokens = 0:
+ * channel of k_scale * key, summary_scale f32 [num_blocks,Hk] s = max|.| / 127. Keys that are NaN do not
+ * count (a channel of nothing else is zero); max|.| is the largest finite fp32 number at most. new_tokens = 0:
  * every page that holds tokens; T > 0: the pages that the last T appended tokens (cu_seqlens as
  * above) lie in. bd_paged_append_summary is bd_paged_append, then bd_paged_block_summary of the pages
  * that its tokens lie in; what either refuses is refused before anything is written.

@@ -63,8 +63,10 @@ def append(k, v, q, cos, sin, interleaved, cu_seqlens, block_table, context_lens
 
 def summary_of(keys):
     """keys f32 [n, D] of one page and head (scaled) -> (codes int8 [2, D], scale f32)."""
-    both = torch.stack([keys.amin(0), keys.amax(0)])
-    top = both.abs().max()
+    nan = keys.isnan()
+    both = torch.stack([keys.masked_fill(nan, float("inf")).amin(0), keys.masked_fill(nan, float("-inf")).amax(0)])
+    both = both.masked_fill(nan.all(0), 0.0)
+    top = both.abs().max().clamp(max=torch.finfo(torch.float32).max)
     s = top / torch.tensor(127.0)
     code = (both / s).round().clamp(-127, 127) if top > 0 else torch.zeros_like(both)
     return code.to(torch.int8), s

@@ -151,3 +151,38 @@ def test_infinite_query_beside_large_ones(cuda, heads, lens):
     q[0, 1, 5] = math.inf
     q[1, 0, 7] = float("nan")
     check_rows(q, kc, vc, table, clen, 1e-6, vs, cuda)
+
+
+ODD_KEYS = [(4, 128, 16, BF16), (12, 64, 32, F16), (1, 256, 64, FP8), (3, 40, 5, F32), (8, 128, 8, FP8), (2, 96, 16, BF16)]
+
+
+def odd_keys(Hk, D, block, cdt, g, lens):
+    """Keys of which some are NaN (in a channel's every row, in one, in all of a page) or infinite."""
+    table, nb = table_for(lens, block, g)
+    kc = to_cache(torch.randn(nb, Hk, block, D, generator=g) * 3, cdt, 1.0)
+    nan, inf = float("nan"), float("nan" if cdt == FP8 else "inf")
+    for i, (rows, ch, to) in enumerate([(slice(None), 3, nan), (0, slice(None), nan), (slice(1, 3), 7, nan),
+                                        (slice(None), slice(None), nan), (1, 5, inf), (0, 6, -inf), (slice(None), 2, inf)]):
+        kc[int(table[1, i]), :, rows, ch] = to
+    kc[int(table[0, 0]), :, 0, 1] = nan  # its only token
+    page = int(table[1, 7])  # every other channel half way between two codes, and no more than the smallest numbers
+    kc[page, :, :, 0] = 127.0
+    kc[page, :, :, 1::2] = 20.5 if cdt != FP8 else 20.0
+    kc[page, :, :, 2] = nan
+    kc[int(table[1, 8])] = torch.finfo(cdt).tiny * 2
+    kc[int(table[1, 8]), :, :, 5] = nan
+    return kc, table, nb
+
+
+@pytest.mark.parametrize("Hk,D,block,cdt", ODD_KEYS)
+def test_summary_of_keys_that_are_not_numbers(cuda, Hk, D, block, cdt):
+    lens = [1, block * 9 - 2]
+    kc, table, nb = odd_keys(Hk, D, block, cdt, gen(D + block), lens)
+    ks = 0.3 if cdt == FP8 else 1.0
+    gk = kc.to(cuda)
+    code, scale = paged.new_block_summary(gk)
+    want_code, want_scale = code.cpu().clone(), scale.cpu().clone()
+    paged.paged_block_summary(gk, table.to(cuda), torch.tensor(lens, device=cuda), code, scale, k_scale=ks)
+    expected_summary(kc, table, lens, block, torch.tensor(ks, dtype=F32), want_code, want_scale)
+    assert torch.isfinite(scale).all()
+    assert torch.equal(scale.cpu(), want_scale) and torch.equal(code.cpu(), want_code)
