@@ -7,11 +7,13 @@
 //   score(page) = max over the group's heads of (float(I) * s_q), times s,
 // two roundings to 32 bits, is the same everywhere: the choice can be compared for equality.
 // The first `sink` and last `recent` pages are taken first, then the largest scores, the lower
-// page on ties; the chosen pages come in ascending order, -1 after the last.
+// page on ties; the chosen pages come in ascending order, -1 after the last. A query's channels that are NaN count as
+// zero, and max|q| is the largest finite fp32 number at most.
 #include "paged.cuh"
 #include "decode_shared.cuh"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace bd {
 
@@ -45,7 +47,7 @@ __device__ __forceinline__ float quantize_query(const SelectParams& p, int b, in
     x[i] = d < p.g.D ? load_as(p.q, p.q_dtype, base + d * p.q_sd) : 0.f;
     top = fmaxf(top, fabsf(x[i]));
   }
-  top = warp_max(top);
+  top = fminf(warp_max(top), FLT_MAX);
   const float mul = __fdiv_rn(127.f, top);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {

@@ -83,7 +83,8 @@ def paged_select_blocks(q, summary, summary_scale, block_table, context_lens, bu
     """Logical pages for one new token of each sequence, int32 [B, H_k, budget], ascending, -1 after the last.
 
     The ``sink_blocks`` first and ``recent_blocks`` last pages, then those with the largest bound of q.k over
-    the page (8-bit q and summaries, the largest over the KV head's query heads, the lower page on ties).
+    the page (8-bit q and summaries, the largest over the KV head's query heads, the lower page on ties). A q
+    that is NaN counts as zero, an infinite one as the largest finite fp32 number.
     """
     _check_row(q)
     if budget < 1:

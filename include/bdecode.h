@@ -358,7 +358,8 @@ int bd_asym_fakequant(const bd_tensor* x, int levels, const bd_tensor* y, bd_str
  *
  * bd_paged_select chooses pages for one new token a sequence from the summaries. With q8 =
  * rint(q * (127 / max|q|)), s_q = max|q| / 127 per query head: I = sum_d max(q8 min8, q8 max8),
- * score(page) = (max over the KV head's query heads of float(I) * s_q) * s, in fp32. The first
+ * score(page) = (max over the KV head's query heads of float(I) * s_q) * s, in fp32 (a q that is NaN counts as
+ * zero, max|q| is the largest finite fp32 number at most). The first
  * `sink` and last `recent` pages of a sequence are taken first, then the largest scores, the
  * lower page on ties. selected int32 [B,Hk,budget]: logical pages in ascending order, -1 after
  * the last.

@@ -94,8 +94,10 @@ def select(q, summary, summary_scale, block_table, context_lens, budget, block, 
                     continue
                 best = None
                 for x in q[b, h * G:(h + 1) * G].float():
-                    top = x.abs().max()
-                    w = (x * (c127 / top)).round().to(torch.int64) if top > 0 else torch.zeros(D, dtype=torch.int64)
+                    x = x.masked_fill(x.isnan(), 0.0)
+                    top = x.abs().max().clamp(max=torch.finfo(torch.float32).max)
+                    w = (x * (c127 / top)).round().clamp(-127, 127) if top > 0 else torch.zeros(D)
+                    w = w.to(torch.int64)
                     lo, hi = summary[p, h, 0].to(torch.int64), summary[p, h, 1].to(torch.int64)
                     s = torch.maximum(w * lo, w * hi).sum().float() * (top / c127)
                     best = s if best is None else torch.maximum(best, s)

@@ -186,3 +186,24 @@ def test_summary_of_keys_that_are_not_numbers(cuda, Hk, D, block, cdt):
     expected_summary(kc, table, lens, block, torch.tensor(ks, dtype=F32), want_code, want_scale)
     assert torch.isfinite(scale).all()
     assert torch.equal(scale.cpu(), want_scale) and torch.equal(code.cpu(), want_code)
+
+
+@pytest.mark.parametrize("Hk,D,block,cdt", ODD_KEYS)
+def test_choice_for_queries_and_keys_that_are_not_numbers(cuda, Hk, D, block, cdt):
+    g = gen(D + block + 1)
+    lens = [1, block * 40 - 2]
+    kc, table, nb = odd_keys(Hk, D, block, cdt, g, lens)
+    qdt = {BF16: BF16, F16: F16, FP8: BF16, F32: F32}[cdt]
+    q = torch.randn(2, 3 * Hk, D, generator=g).to(qdt)
+    q[1, 0, 4] = float("nan")
+    q[1, 1] = float("nan")
+    if Hk > 1:
+        q[1, 3, 9], q[1, 4, 0] = math.inf, -math.inf
+    q[0, 0, 0] = math.inf
+    gk = kc.to(cuda)
+    code, scale = paged.new_block_summary(gk)
+    clen = torch.tensor(lens, dtype=torch.int32)
+    paged.paged_block_summary(gk, table.to(cuda), clen.to(cuda), code, scale)
+    for budget in (3, 11):
+        got = paged.paged_select_blocks(q.to(cuda), code, scale, table.to(cuda), clen.to(cuda), budget, block)
+        assert torch.equal(got.cpu(), plain.select(q, code.cpu(), scale.cpu(), table, clen, budget, block, 0, 1))
