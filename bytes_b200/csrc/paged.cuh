@@ -2,6 +2,8 @@
 #pragma once
 #include "common.cuh"
 
+#include <atomic>
+
 namespace bd {
 
 // The paged kernels are launched as programmatic dependents of whatever ran before them in the stream, so that they are
@@ -68,6 +70,20 @@ int guarded(F&& body) noexcept {
 __device__ __forceinline__ void cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
+// What `ask` answers for the current device (not 0, or it is asked again); kept in `slots`, which host threads share.
+template <typename F>
+int once_per_device(std::atomic<int> (&slots)[64], F&& ask) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<int>& slot = slots[dev & 63];
+  int v = slot.load(std::memory_order_acquire);
+  if (v == 0) {
+    v = ask();
+    slot.store(v, std::memory_order_release);
+  }
+  return v;
 }
 
 // Loads and stores by element type, for the forms that take any of them.

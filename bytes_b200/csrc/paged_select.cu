@@ -19,6 +19,8 @@ namespace bd {
 
 namespace {
 
+constexpr int kMostHeads = 128;  // query heads a KV head
+
 struct SelectParams {
   PagedGeometry g;  // its cache strides are unused; block = tokens a page
   const void* q; int64_t q_sb, q_sh, q_sd; int q_dtype;
@@ -414,7 +416,7 @@ int check_select(const bd_tensor* q, const bd_tensor* summary, const bd_tensor* 
     return fail(BD_ERR_SHAPE, "summary_scale " + shape_str(summary_scale) + " must be [num_blocks, Hk]");
   if (Hk < 1 || Hq < 1 || Hq % Hk) return fail(BD_ERR_SHAPE, "H_q must be a multiple of H_k");
   if (D < 1 || D > 256) return fail(BD_ERR_UNSUPPORTED, "head_dim must be at most 256");
-  if (Hq / Hk > 128) return fail(BD_ERR_UNSUPPORTED, "at most 128 query heads a KV head");
+  if (Hq / Hk > kMostHeads) return fail(BD_ERR_UNSUPPORTED, "at most 128 query heads a KV head");
   if (B > 65535 || Hk > 65535) return fail(BD_ERR_SHAPE, "more than 65535 sequences or heads");
   if (summary->stride[3] != 1 || summary->stride[2] != D)
     return fail(BD_ERR_STRIDE, "summary's last two dims must be contiguous");
@@ -460,10 +462,17 @@ int launch_select(const SelectParams& p, cudaStream_t st) {
       {paged_select_kernel<0, 16, 512>, paged_select_kernel<64, 16, 512>, paged_select_kernel<128, 16, 512>,
        paged_select_kernel<256, 16, 512>}};
   const Kernel kern = kernels[size][kind];
-  int rc;
-  if (smem > 40 * 1024 && (rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
-                                           "cudaFuncSetAttribute(paged_select_kernel)")))
-    return rc;
+  // allowed, and asked for below, once for the most that the checks let through: a call's own size would change under
+  // another host thread's launch
+  const size_t most = size_t(kMostHeads) * (2 * (kind ? D : 256) + sizeof(float));
+  static std::atomic<int> set[3][4][64];
+  int rc = BD_OK;
+  once_per_device(set[size][kind], [&] {
+    rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most)),
+                    "cudaFuncSetAttribute(paged_select_kernel)");
+    return rc == BD_OK;
+  });
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
@@ -478,20 +487,19 @@ int launch_select(const SelectParams& p, cudaStream_t st) {
   unsigned ctas = 1;
   while (ctas < 16 && rows * ctas * threads <= 512 * num_sms() && int64_t(ctas) * (threads / 2) < p.g.wide) ctas *= 2;
   if (ctas == 16) {
-    static signed char room[64][3][4] = {};  // 1: a cluster of 16 fits this device, -1: it does not
-    int dev = 0;
-    cudaGetDevice(&dev);
-    signed char& r = room[dev & 63][size][kind];
-    if (r == 0) {
+    static std::atomic<int> room[3][4][64];  // 1: a cluster of 16 fits this device, -1: it does not
+    const int fits = once_per_device(room[size][kind], [&] {
       int n = 0;
       cfg.gridDim = dim3(16);
+      cfg.dynamicSmemBytes = most;
       attr[0].val.clusterDim.x = 16;
-      r = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-                  cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0
-              ? 1 : -1;
+      const bool some = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0;
       (void)cudaGetLastError();
-    }
-    if (r < 0) ctas = 8;
+      cfg.dynamicSmemBytes = smem;
+      return some ? 1 : -1;
+    });
+    if (fits < 0) ctas = 8;
   }
   cfg.gridDim = dim3(ctas, p.g.Hk, p.g.B);
   attr[0].val.clusterDim.x = ctas;

@@ -1,10 +1,13 @@
 """The paged-cache operators at their edges: what reaches which kernel, lengths that change between calls, values that are
 not numbers, streams and host threads. Inputs and bounds are those of test_gpu_paged.py."""
+import ctypes
 import math
+import threading
 
 import pytest
 import torch
 
+from bytes_b200 import _native as N
 from bytes_b200 import paged
 from oracle import paged as plain
 from test_gpu_paged import (BF16, F16, F32, FP8, attention_inputs, bits, check_attention, expected_summary, gen, table_for,
@@ -207,3 +210,52 @@ def test_choice_for_queries_and_keys_that_are_not_numbers(cuda, Hk, D, block, cd
     for budget in (3, 11):
         got = paged.paged_select_blocks(q.to(cuda), code, scale, table.to(cuda), clen.to(cuda), budget, block)
         assert torch.equal(got.cpu(), plain.select(q, code.cpu(), scale.cpu(), table, clen, budget, block, 0, 1))
+
+
+# ----------------------------------------------------------------------- streams, host threads
+def select_through_c(q, code, scale, table, lens, block, out, ws, stream):
+    """A call of the C entry point itself: ctypes lets other host threads run meanwhile, the Python layer's glue does not."""
+    f = N.lib().bd_paged_select
+    f.restype = ctypes.c_int
+    d = [N.ref(N.desc(t)) for t in (q, code, scale, table, lens, out)]
+    I = ctypes.c_int  # noqa: E741
+    args = (*d[:5], I(block), I(0), I(1), d[5], ctypes.c_void_p(ws.data_ptr()), ctypes.c_size_t(ws.numel()),
+            ctypes.c_void_p(stream.cuda_stream))
+    return lambda: f(*args)
+
+
+def test_choice_from_two_host_threads_with_unlike_heads(cuda):
+    """Head counts that need different amounts of shared memory of the same kernel, launched by two threads at once."""
+    block, D, calls = 16, 256, 5000
+    work = []
+    for heads in (128, 97):
+        g = gen(heads)
+        table, nb = table_for([block * 90], block, g)
+        code = torch.randint(-127, 128, (nb, 1, 2, D), generator=g).to(torch.int8).to(cuda)
+        scale = torch.rand(nb, 1, generator=g).to(cuda)
+        q = torch.randn(1, heads, D, generator=g).bfloat16().to(cuda)
+        lens = torch.tensor([block * 90], dtype=torch.int32, device=cuda)
+        want = paged.paged_select_blocks(q, code, scale, table.to(cuda), lens, 7, block)
+        work.append((q, code, scale, table.to(cuda), lens, block, torch.empty_like(want),
+                     torch.empty(1 << 16, dtype=torch.uint8, device=cuda), torch.cuda.Stream(), want))
+    torch.cuda.synchronize()
+    bad, start = [], threading.Barrier(2)
+
+    def run(w):
+        call = select_through_c(*w[:9])
+        start.wait()
+        for _ in range(calls):
+            rc = call()
+            if rc:
+                bad.append((rc, N.lib().bd_last_error()))
+                return
+
+    threads = [threading.Thread(target=run, args=(w,)) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad
+    for w in work:
+        assert torch.equal(w[6], w[9])
