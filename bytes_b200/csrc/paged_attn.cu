@@ -1191,11 +1191,8 @@ auto with_shape(const AttnParams& p, F&& f) {
 int cluster_room(const AttnParams& p, int ctas) {
   return with_shape(p, [&](auto d, auto kind, auto nt) {
     using T = TileShape<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>;
-    static int room[64][5] = {};  // one more than there are
-    int dev = 0;
-    cudaGetDevice(&dev);
-    int& r = room[dev & 63][31 - __builtin_clz(unsigned(ctas))];
-    if (r == 0) {
+    static std::atomic<int> room[5][64];  // one more than there are
+    return once_per_device(room[31 - __builtin_clz(unsigned(ctas))], [&] {
       auto kern = paged_attn_tile_kernel<decltype(d)::value, decltype(kind)::value, decltype(nt)::value>;
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute attr[1];
@@ -1211,9 +1208,8 @@ int cluster_room(const AttnParams& p, int ctas) {
           (ctas <= 8 || cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) &&
           cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess;
       (void)cudaGetLastError();
-      r = 1 + (some ? n : 0);
-    }
-    return r - 1;
+      return 1 + (some ? n : 0);
+    }) - 1;
   });
 }
 
@@ -1285,15 +1281,14 @@ int launch_tiles(const AttnParams& p, const bd_tensor* k_cache, const bd_tensor*
   if (!tile_map(&km, k_cache, T::SW) || !tile_map(&vm, v_cache, T::SW))
     return fail(BD_ERR_CUDA, "cuTensorMapEncodeTiled refused the cache's layout");
   auto kern = paged_attn_tile_kernel<D, KIND, NT>;
-  static bool set[64] = {false};  // dynamic shared memory allowed, per device
-  int dev = 0, rc;
-  cudaGetDevice(&dev);
-  if (!set[dev & 63]) {
-    if ((rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM),
-                         "cudaFuncSetAttribute(paged_attn_tile_kernel)")))
-      return rc;
-    set[dev & 63] = true;
-  }
+  static std::atomic<int> set[64];  // dynamic shared memory allowed
+  int rc = BD_OK;
+  once_per_device(set, [&] {
+    rc = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM),
+                    "cudaFuncSetAttribute(paged_attn_tile_kernel)");
+    return rc == BD_OK;
+  });
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(p.warps / T::WARPS);

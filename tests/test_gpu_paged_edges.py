@@ -259,3 +259,36 @@ def test_choice_from_two_host_threads_with_unlike_heads(cuda):
     assert not bad
     for w in work:
         assert torch.equal(w[6], w[9])
+
+
+def test_calls_on_two_streams_at_once(cuda):
+    """The same chains of calls on two streams, whose kernels come early and overlap: each as it is alone."""
+    def inputs(seed):
+        x = attention_inputs([3000, 0, 40, 777], 28, 4, 128, 16, BF16, FP8 if seed % 2 else BF16, seed)
+        q, kc, vc, table, lens = (t.to(cuda) for t in x[:5])
+        return q, kc, vc, table, lens, x[5], x[6], *paged.new_block_summary(kc), \
+            torch.randn(4, 4, 128, generator=gen(seed)).bfloat16().to(cuda)
+
+    def chain(q, kc, vc, table, lens, ks, vs, code, scale, k):
+        n, out = lens.clone(), []
+        paged.paged_block_summary(kc, table, n, code, scale, k_scale=ks)
+        for _ in range(6):
+            n += 1
+            paged.paged_append(k, k, kc, vc, table, n, k_scale=ks, v_scale=vs, summary=code, summary_scale=scale)
+            out.append(paged.paged_sparse_decode_attn(q, kc, vc, code, scale, table, n, 9, 0.1, k_scale=ks, v_scale=vs))
+            out.append(paged.paged_decode_attn(q, kc, vc, table, n, 0.1, k_scale=ks, v_scale=vs))
+        return out
+
+    alone = [chain(*inputs(seed)) for seed in (41, 42)]
+    torch.cuda.synchronize()
+    ready = [inputs(seed) for seed in (41, 42)]
+    streams = [torch.cuda.Stream() for _ in ready]
+    torch.cuda.synchronize()
+    got = []
+    for s, x in zip(streams, ready):
+        with torch.cuda.stream(s):
+            got.append(chain(*x))
+    torch.cuda.synchronize()
+    for a, b in zip(alone, got):
+        for x, y in zip(a, b):
+            assert torch.equal(bits(x), bits(y))
