@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cmath>
+#include <cstdint>
 #include <stdexcept>
 #include <tuple>
 
@@ -142,8 +143,15 @@ struct OptDesc {
   }
 };
 
-// Tables and lengths as the kernels read them.
-at::Tensor as_int32(const at::Tensor& t) { return t.scalar_type() == at::kInt ? t : t.to(at::kInt); }
+// Tables and lengths as the kernels read them. A 64-bit number that 32 bits do not hold becomes the nearest that they do:
+// cut to its lower half, an entry that names no page could name one.
+at::Tensor as_int32(const at::Tensor& t) {
+  if (t.scalar_type() == at::kInt) return t;
+  if (!at::isIntegralType(t.scalar_type(), /*includeBool=*/false))
+    throw std::invalid_argument("bytes_b200: block tables, lengths and page lists must be integers");
+  if (t.scalar_type() != at::kLong) return t.to(at::kInt);
+  return t.clamp(int64_t(INT32_MIN), int64_t(INT32_MAX)).to(at::kInt);
+}
 
 // A decode query or output: [B, H, D], or [B, H, 1, D] viewed so.
 bd_tensor desc_row(const at::Tensor& t, int device) {

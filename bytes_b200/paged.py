@@ -2,7 +2,8 @@
 
 The cache is two tensors of pages, ``k_cache`` and ``v_cache`` [num_blocks, H_k, block, D] (bf16,
 f16, f32 or fp8 e4m3), a ``block_table`` int32 [B, W] from a sequence's logical pages to pages, and
-``context_lens`` int32 [B]. Per decode step and layer:
+``context_lens`` int32 [B] (other integers are converted, by a kernel or two a call). Per decode step and
+layer:
 
     q = paged.paged_append(k, v, k_cache, v_cache, block_table, context_lens, q=q, cos=cos, sin=sin)
     out = paged.paged_decode_attn(q, k_cache, v_cache, block_table, context_lens, D ** -0.5)

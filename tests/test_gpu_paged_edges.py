@@ -71,6 +71,41 @@ def test_a_refused_append_has_written_nothing(cuda, tokens):
     assert bool(kc.any()) == bool(code.any()) == (tokens > 0)
 
 
+def test_tables_and_lengths_of_other_types(cuda):
+    """64-bit entries that 32 bits do not hold name no page and are long lengths, whatever their lower halves say;
+    shorter integers are taken as they are; what is no integer is refused."""
+    q, kc, vc, table, lens, ks, vs = attention_inputs([100, 333], 8, 2, 128, 16, BF16, BF16, 51)
+    table[1, 2] = -1
+    table[0, 1] = -1
+    gq, gk, gv, gt, gl = (t.to(cuda) for t in (q, kc, vc, table, lens))
+    want = paged.paged_decode_attn(gq, gk, gv, gt, gl, 0.1)
+    wide = gt.long()
+    wide[1, 2] = (1 << 32) + 3
+    wide[0, 1] = -(1 << 32) + 4
+    assert torch.equal(paged.paged_decode_attn(gq, gk, gv, wide, gl.long(), 0.1), want)
+    assert torch.equal(paged.paged_decode_attn(gq, gk, gv, gt.short(), gl.short(), 0.1), want)
+    full = paged.paged_decode_attn(gq, gk, gv, gt, torch.full_like(gl, 2 ** 31 - 1), 0.1)
+    assert torch.equal(paged.paged_decode_attn(gq, gk, gv, gt, torch.full_like(gl, 2 ** 31 - 1).long() + (1 << 33), 0.1), full)
+    sel = torch.tensor([[[0, 2, (1 << 32) + 1], [0, 1 << 40, 3]]] * 2, device=cuda)
+    plain_sel = sel.clamp(max=1 << 20).int()
+    assert torch.equal(paged.paged_decode_attn(gq, gk, gv, gt, gl, 0.1, selected=sel),
+                       paged.paged_decode_attn(gq, gk, gv, gt, gl, 0.1, selected=plain_sel))
+    k = torch.ones(2, 2, 128, dtype=BF16, device=cuda)
+    kept = gk.clone()
+    paged.paged_append(k, k, gk, gv, wide, torch.tensor([17, 33], device=cuda))  # into those two entries
+    assert torch.equal(gk, kept)
+    for bad in (gt.float(), gt.bool()):
+        with pytest.raises(ValueError):
+            paged.paged_decode_attn(gq, gk, gv, bad, gl, 0.1)
+    with pytest.raises(ValueError):
+        paged.paged_append(k, k, gk, gv, gt, gl.float())
+    with pytest.raises(ValueError):
+        paged.paged_append(k, k, gk, gv, gt, gl, cu_seqlens=torch.tensor([0.0, 1.0, 2.0], device=cuda))
+    with pytest.raises(ValueError):
+        paged.paged_decode_attn(gq, gk, gv, gt, gl, 0.1, selected=plain_sel.float())
+    assert torch.equal(gk, kept)
+
+
 # ---------------------------------------------------------------------------- not quite numbers
 FORMS = {  # lengths; q heads, kv heads, D, block, q, cache
     "a cluster a row": ([1, 40, 700, 2000], 8, 2, 128, 16, BF16, BF16),
