@@ -14,6 +14,7 @@
 #include <cmath>
 #include <cstdint>
 #include <stdexcept>
+#include <string>
 #include <tuple>
 
 #include "bdecode.h"
@@ -153,6 +154,19 @@ at::Tensor as_int32(const at::Tensor& t) {
   return t.clamp(int64_t(INT32_MIN), int64_t(INT32_MAX)).to(at::kInt);
 }
 
+// A count as the C entry points take it.
+int as_int(int64_t x, const char* name) {
+  if (x < INT32_MIN || x > INT32_MAX) throw std::invalid_argument(std::string("bytes_b200: ") + name + " does not fit 32 bits");
+  return int(x);
+}
+
+// The chosen pages of a call, [B, Hk, budget].
+at::Tensor empty_selected(const at::Tensor& q, const at::Tensor& summary, int64_t budget) {
+  if (summary.dim() != 4) throw std::invalid_argument("bytes_b200: summary must be [num_blocks, Hk, 2, D]");
+  if (budget > int64_t(1) << 24) throw std::invalid_argument("bytes_b200: more than 2^24 chosen pages");
+  return at::empty({q.size(0), summary.size(1), budget}, q.options().dtype(at::kInt));
+}
+
 // A decode query or output: [B, H, D], or [B, H, 1, D] viewed so.
 bd_tensor desc_row(const at::Tensor& t, int device) {
   return t.dim() == 4 && t.size(2) == 1 ? desc_drop2(t, device) : desc(t, device);
@@ -203,14 +217,14 @@ std::tuple<int64_t, at::Tensor> paged_select(const at::Tensor& q, const at::Tens
   const at::Tensor table = as_int32(table_), lens = as_int32(lens_);
   const bd_tensor dq = desc_row(q, dev), ds = desc(summary, dev), dss = desc(summary_scale, dev),
                   dt = desc(table, dev), dl = desc(lens, dev);
-  if (summary.dim() != 4) return {BD_ERR_SHAPE, at::Tensor()};
   const c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor sel = at::empty({q.size(0), summary.size(1), budget}, q.options().dtype(at::kInt));
+  at::Tensor sel = empty_selected(q, summary, budget);
   const bd_tensor dsel = desc(sel, dev);
   const size_t nws = bd_paged_select_workspace(&dq, &ds, &dt);
   const at::Tensor ws = workspace(nws, q);
-  const int rc = bd_paged_select(&dq, &ds, &dss, &dt, &dl, int(block_size), int(sink), int(recent), &dsel,
-                                 ws.data_ptr(), nws, at::cuda::getCurrentCUDAStream(dev).stream());
+  const int rc = bd_paged_select(&dq, &ds, &dss, &dt, &dl, as_int(block_size, "block_size"), as_int(sink, "sink_blocks"),
+                                 as_int(recent, "recent_blocks"), &dsel, ws.data_ptr(), nws,
+                                 at::cuda::getCurrentCUDAStream(dev).stream());
   return {rc, sel};
 }
 
@@ -249,16 +263,16 @@ std::tuple<int64_t, at::Tensor, at::Tensor> paged_sparse_decode_attn(
   const at::Tensor table = as_int32(table_), lens = as_int32(lens_);
   const bd_tensor dq = desc_row(q, dev), dk = desc(k_cache, dev), dv = desc(v_cache, dev), ds = desc(summary, dev),
                   dss = desc(summary_scale, dev), dt = desc(table, dev), dl = desc(lens, dev);
-  if (summary.dim() != 4) return {BD_ERR_SHAPE, at::Tensor(), at::Tensor()};
   const c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = at::empty(q.sizes(), q.options());
-  at::Tensor sel = at::empty({q.size(0), summary.size(1), budget}, q.options().dtype(at::kInt));
+  at::Tensor sel = empty_selected(q, summary, budget);
   const bd_tensor dout = desc_row(out, dev), dsel = desc(sel, dev);
   const size_t nws = bd_paged_sparse_decode_attn_workspace(&dq, &dk, &dv, &ds, &dt, &dl, &dsel);
   const at::Tensor ws = workspace(nws, q);
-  const int rc = bd_paged_sparse_decode_attn(&dq, &dk, &dv, &ds, &dss, &dt, &dl, int(sink), int(recent),
-                                             float(scaling), float(k_scale), float(v_scale), &dsel, &dout, nullptr,
-                                             ws.data_ptr(), nws, at::cuda::getCurrentCUDAStream(dev).stream());
+  const int rc = bd_paged_sparse_decode_attn(&dq, &dk, &dv, &ds, &dss, &dt, &dl, as_int(sink, "sink_blocks"),
+                                             as_int(recent, "recent_blocks"), float(scaling), float(k_scale),
+                                             float(v_scale), &dsel, &dout, nullptr, ws.data_ptr(), nws,
+                                             at::cuda::getCurrentCUDAStream(dev).stream());
   return {rc, out, sel};
 }
 

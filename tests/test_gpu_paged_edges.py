@@ -327,3 +327,25 @@ def test_calls_on_two_streams_at_once(cuda):
     for a, b in zip(alone, got):
         for x, y in zip(a, b):
             assert torch.equal(bits(x), bits(y))
+
+
+def test_counts_past_32_bits_and_summaries_of_other_shapes(cuda):
+    """Refused with their own message, not cut to their lower halves; nothing as large as asked for is made first."""
+    kc = torch.zeros(6, 2, 16, 64, dtype=BF16, device=cuda)
+    code, scale = paged.new_block_summary(kc)
+    table, lens = torch.zeros(1, 3, dtype=torch.int32, device=cuda), torch.ones(1, dtype=torch.int32, device=cuda)
+    q = torch.zeros(1, 8, 64, dtype=BF16, device=cuda)
+    big = 1 << 32
+
+    def select(match, code=code, budget=2, block=16, **kw):
+        with pytest.raises(ValueError, match=match):
+            paged.paged_select_blocks(q, code, scale, table, lens, budget, block, **kw)
+        if block == 16:
+            with pytest.raises(ValueError, match=match):
+                paged.paged_sparse_decode_attn(q, kc, kc, code, scale, table, lens, budget, 1.0, **kw)
+
+    select("block_size", block=big + 16)
+    select("sink_blocks", sink_blocks=big)
+    select("recent_blocks", recent_blocks=big + 1)
+    select("chosen pages", budget=1 << 50)
+    select("summary", code=code[0])
