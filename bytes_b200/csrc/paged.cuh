@@ -3,6 +3,7 @@
 #include "common.cuh"
 
 #include <atomic>
+#include <cfloat>
 
 namespace bd {
 
@@ -53,6 +54,9 @@ int check_paged(const bd_tensor* k_cache, const bd_tensor* v_cache, const bd_ten
 long long paged_wait_timeouts();
 
 inline bool is_float16_32(int dt) { return dt == BD_BF16 || dt == BD_F16 || dt == BD_F32; }
+
+// Whether an 8-bit cache's scale can be multiplied by and divided by: positive, finite, and so is its reciprocal.
+inline bool is_scale(float x) { return x > 0.f && x <= FLT_MAX && 1.f / x <= FLT_MAX; }
 
 // Runs the body of an extern "C" entry point: nothing thrown in it (an allocation that fails
 // while a message is built) crosses the C boundary.

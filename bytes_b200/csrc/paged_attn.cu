@@ -9,7 +9,6 @@
 #include "decode_shared.cuh"
 
 #include <algorithm>
-#include <cfloat>
 #include <type_traits>
 
 namespace bd {
@@ -1373,7 +1372,8 @@ int check_out(const bd_tensor* q, const bd_tensor* k_cache, float k_scale, float
       return fail(BD_ERR_SHAPE, "lse must be [B, Hq]");
     p.lse = static_cast<float*>(lse->data); p.e_sb = lse->stride[0]; p.e_sh = lse->stride[1];
   }
-  if (!(k_scale > 0.f) || !(v_scale > 0.f)) return fail(BD_ERR_VALUE, "k_scale and v_scale must be positive");
+  if (!is_scale(k_scale) || !is_scale(v_scale))
+    return fail(BD_ERR_VALUE, "k_scale and v_scale must be positive, and they and their reciprocals finite");
   if (k_cache->dtype != BD_F8E4M3 && (k_scale != 1.f || v_scale != 1.f))
     return fail(BD_ERR_VALUE, "k_scale and v_scale belong to an fp8 cache");
   p.out = out->data; p.out_dtype = out->dtype;

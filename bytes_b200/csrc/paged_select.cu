@@ -13,7 +13,6 @@
 #include "decode_shared.cuh"
 
 #include <algorithm>
-#include <cfloat>
 
 namespace bd {
 

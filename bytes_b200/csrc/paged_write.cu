@@ -12,7 +12,6 @@
 #include "decode_shared.cuh"
 
 #include <algorithm>
-#include <cfloat>
 #include <type_traits>
 
 namespace bd {
@@ -677,7 +676,8 @@ int plan_append(const bd_tensor* k, const bd_tensor* v, const bd_tensor* q, cons
     p.positions = int(cos->shape[0]); p.half = int(cos->shape[1]);
   }
   const bool fp8 = k_cache->dtype == BD_F8E4M3;
-  if (!(k_scale > 0.f) || !(v_scale > 0.f)) return fail(BD_ERR_VALUE, "k_scale and v_scale must be positive");
+  if (!is_scale(k_scale) || !is_scale(v_scale))
+    return fail(BD_ERR_VALUE, "k_scale and v_scale must be positive, and they and their reciprocals finite");
   if (!fp8 && (k_scale != 1.f || v_scale != 1.f))
     return fail(BD_ERR_VALUE, "k_scale and v_scale belong to an fp8 cache");
   p.k = rows_of(k); p.v = rows_of(v);
@@ -716,7 +716,7 @@ int plan_summary(const bd_tensor* k_cache, const bd_tensor* block_table, const b
     return fail(BD_ERR_SHAPE, "summary_scale " + shape_str(summary_scale) + " must be [num_blocks, Hk]");
   if (summary->stride[3] != 1 || summary->stride[2] != p.g.D)
     return fail(BD_ERR_STRIDE, "summary's last two dims must be contiguous");
-  if (!(k_scale > 0.f)) return fail(BD_ERR_VALUE, "k_scale must be positive");
+  if (!is_scale(k_scale)) return fail(BD_ERR_VALUE, "k_scale must be positive, and it and its reciprocal finite");
   if (k_cache->dtype != BD_F8E4M3 && k_scale != 1.f) return fail(BD_ERR_VALUE, "k_scale belongs to an fp8 cache");
   if (new_tokens < 0) return fail(BD_ERR_VALUE, "new_tokens must not be negative");
   if (cu_seqlens && new_tokens == 0) return fail(BD_ERR_VALUE, "cu_seqlens goes with new_tokens");

@@ -336,7 +336,8 @@ int bd_asym_fakequant(const bd_tensor* x, int levels, const bd_tensor* y, bd_str
  * f32 or fp8 e4m3; D <= 256; any strides), block_table int32 [B,W] (logical page -> page), and
  * context_lens int32 [B]. Entries outside [0,num_blocks) name no page: nothing is written
  * there, and its tokens do not count. Lengths are cut to [0, W*block]. An fp8 cache holds
- * x / k_scale and x / v_scale; the other types take scales of 1.
+ * x / k_scale and x / v_scale (scales positive, they and their reciprocals finite); the other types take
+ * scales of 1.
  *
  * bd_paged_append writes new tokens into their pages, the keys rotated by their position, and
  * writes the rotated queries to q_out (q and q_out NULL: none). k,v [T,Hk,D], q,q_out [T,Hq,D]
