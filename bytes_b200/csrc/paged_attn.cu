@@ -1492,6 +1492,9 @@ int bd_paged_sparse_decode_attn(const bd_tensor* q, const bd_tensor* k_cache, co
     if ((rc = check_attn(q, k_cache, v_cache, block_table, context_lens, selected, &p)) ||
         (rc = check_out(q, k_cache, k_scale, v_scale, out, lse, &p)))
       return rc;
+    if (summary && summary->ndim == 4 && summary->shape[0] != p.g.num_blocks)
+      return fail(BD_ERR_SHAPE, "summary " + shape_str(summary) + " must have the cache's " +
+                                    std::to_string(p.g.num_blocks) + " pages");
     const size_t first = bd_paged_select_workspace(q, summary, block_table);
     if (!workspace || workspace_bytes < first + attn_bytes(q, k_cache, v_cache, block_table, context_lens, selected))
       return fail(BD_ERR_WORKSPACE, "workspace is smaller than bd_paged_sparse_decode_attn_workspace");

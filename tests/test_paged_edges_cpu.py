@@ -47,3 +47,15 @@ def test_scales_that_cannot_be_divided_by_are_refused(x):
         assert attn(at(q), at(kc), at(kc), at(table), at(lens), None, F(0.1), F(a), F(b), at(q), None, VP(0), SZ(0),
                     None) == rc
     assert summ(at(kc), at(table), at(lens), None, I(0), F(x), at(code), at(scale), None) == 9
+
+
+def test_chained_call_refuses_the_summary_of_another_cache():
+    """(A call of no sequences, which launches nothing if it is let through.)"""
+    f = N.lib().bd_paged_sparse_decode_attn
+    f.restype = I
+    q, kc = fake((0, 8, 64), N.BD_BF16), fake((6, 2, 16, 64), N.BD_BF16)
+    table, lens, sel = fake((0, 4), N.BD_I32), fake((0,), N.BD_I32), fake((0, 2, 3), N.BD_I32)
+    for blocks, rc in ((6, 0), (5, 3), (7, 3)):
+        code, scale = fake((blocks, 2, 2, 64), N.BD_I8), fake((blocks, 2), N.BD_F32)
+        assert f(at(q), at(kc), at(kc), at(code), at(scale), at(table), at(lens), I(0), I(1), F(0.1), F(1.0), F(1.0),
+                 at(sel), at(q), None, VP(0x10000), SZ(1 << 20), None) == rc
