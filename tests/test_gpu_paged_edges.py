@@ -2,6 +2,7 @@
 not numbers, streams and host threads. Inputs and bounds are those of test_gpu_paged.py."""
 import ctypes
 import math
+import re
 import threading
 
 import pytest
@@ -349,3 +350,190 @@ def test_counts_past_32_bits_and_summaries_of_other_shapes(cuda):
     select("recent_blocks", recent_blocks=big + 1)
     select("chosen pages", budget=1 << 50)
     select("summary", code=code[0])
+
+
+# ------------------------------------------------------------------- which kernels a call launches
+def launched(call):
+    """[(kernel's name and template arguments, CTAs of a cluster)] of a captured call."""
+    drv = pytest.importorskip("cuda.bindings.driver")
+
+    def ok(r):
+        assert int(r[0]) == 0, r
+        return r[1] if len(r) == 2 else r[1:]
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    handle, out = drv.CUgraph(graph.raw_cuda_graph()), []
+    n = ok(drv.cuGraphGetNodes(handle, 0))[1]
+    for node in ok(drv.cuGraphGetNodes(handle, n))[0][:n]:
+        if ok(drv.cuGraphNodeGetType(node)) != drv.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL:
+            continue
+        p = ok(drv.cuGraphKernelNodeGetParams(node))
+        name = (ok(drv.cuFuncGetName(p.func)) if int(p.func) else ok(drv.cuKernelGetName(p.kern))).decode()
+        found = re.search(r"\d(paged_[a-z_]+kernel)(I(?:L[ib]\d+E|\d*[a-zA-Z_]\w*?)*E)?", name)
+        cluster = ok(drv.cuGraphKernelNodeGetAttribute(
+            node, drv.CUlaunchAttributeID.CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION)).clusterDim.x
+        out.append((found.group(1), [int(x) for x in re.findall(r"Li(\d+)E", found.group(2) or "")], cluster))
+    return out
+
+
+def widened(table, columns):
+    wide = torch.full((table.shape[0], columns), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
+# lengths, KV heads, columns of the table (0: as the lengths need); what follows from them: CTAs of a row's cluster, or
+# the join and how many heads a CTA of it takes
+PATHS = {
+    "a CTA a row": ([150, 0, 33] * 8, 2, 0, 1),
+    "two CTAs a row": ([700, 0, 333, 1, 90, 1024] * 3, 2, 0, 2),
+    "four CTAs a row": ([900, 0, 1000, 17] * 3, 2, 0, 4),
+    "eight CTAs a row": ([3000, 0, 1777, 16], 2, 0, 8),
+    "sixteen CTAs a row": ([5000, 15], 2, 0, 16),
+    "joined by rows, a head a CTA": ([4000, 0, 9, 2500], 2, 60000, "one"),
+    "joined by rows, several heads a CTA": ([30, 0, 9, 50, 71, 18, 2000] * 45, 2, 0, "rows"),
+    "joined by cuts": ([70, 0, 9, 50, 71, 18, 1000] * 155, 2, 0, "cuts"),
+}
+
+
+@pytest.mark.parametrize("heads,D,qdt,cdt", [(4, 128, BF16, BF16), (7, 128, BF16, FP8), (8, 64, F16, F16),
+                                             (16, 64, BF16, FP8), (8, 256, F16, FP8), (11, 128, F16, F16),
+                                             (2, 256, BF16, BF16), (9, 64, BF16, BF16), (16, 256, BF16, BF16),
+                                             (12, 256, BF16, FP8), (10, 256, F16, F16), (13, 128, BF16, FP8)])
+@pytest.mark.parametrize("path", list(PATHS))
+def test_each_path_of_the_attention(cuda, path, heads, D, qdt, cdt):
+    """Each way of sharing the work out, seen to be the one that runs."""
+    if torch.cuda.get_device_properties(cuda).multi_processor_count != 148:
+        pytest.skip("the sizes are for 148 SMs")
+    lens, Hk, columns, want = PATHS[path]
+    q, kc, vc, table, clen, ks, vs = attention_inputs(lens, heads * Hk, Hk, D, 16 if heads % 2 else 8, qdt, cdt, heads)
+    if columns:
+        table = widened(table, columns)
+    on = [t.to(cuda) for t in (q, kc, vc, table, clen)]
+    got = launched(lambda: paged.paged_decode_attn(*on, 0.1, k_scale=ks, v_scale=vs))
+    assert got[0][0] == "paged_attn_tile_kernel"
+    if isinstance(want, int):
+        assert len(got) == 1 and max(1, got[0][2]) == want, got
+    else:
+        name, args, _ = got[1]
+        many = 4 if D == 256 else 8
+        if want == "cuts" or path == "joined by rows, several heads a CTA" and name.endswith("cuts_kernel") and heads > many:
+            assert name == "paged_tile_join_cuts_kernel", got  # (two groups of heads are twice as many CTAs)
+        else:
+            assert name == "paged_tile_join_kernel" and args[-1] == (1 if want == "one" else many), got
+    check_attention(q, kc, vc, table, clen, ks, vs, cuda)
+
+
+@pytest.mark.parametrize("qdt,cdt,D,block", [(F32, BF16, 128, 16), (BF16, F16, 128, 16), (F16, F16, 96, 16), (BF16, BF16, 64, 12)])
+def test_what_the_tiles_cannot_take_goes_to_the_general_form(cuda, qdt, cdt, D, block):
+    q, kc, vc, table, clen, ks, vs = attention_inputs([50, 0, 700], 6, 2, D, block, qdt, cdt, 61)
+    on = [t.to(cuda) for t in (q, kc, vc, table, clen)]
+    assert [x[0] for x in launched(lambda: paged.paged_decode_attn(*on, 0.1))] == ["paged_attn_generic_kernel", "paged_join_kernel"]
+    check_attention(q, kc, vc, table, clen, ks, vs, cuda)
+
+
+# -------------------------------------------------------------------------- tables, pages, types
+@pytest.mark.parametrize("D,cdt", [(128, BF16), (64, FP8), (40, F32)])
+def test_choice_and_summaries_at_a_wide_table(cuda, D, cdt):
+    """A table far wider than the lengths, as a loop that replays a graph has it: summaries, choice and chained attention
+    as at a table of their own width."""
+    lens = [700, 20, 0, 1, 5000]
+    q, kc, vc, table, clen, ks, vs = attention_inputs(lens, 8, 2, D, 16, F32 if cdt == F32 else BF16, cdt, 71)
+    gq, gk, gv, gl = (t.to(cuda) for t in (q, kc, vc, clen))
+    both = []
+    for t in (table, widened(table, 9000), widened(table, 70000)):
+        gt = t.to(cuda)
+        code, scale = paged.new_block_summary(gk)
+        paged.paged_block_summary(gk, gt, gl, code, scale, k_scale=ks)
+        out, sel = paged.paged_sparse_decode_attn(gq, gk, gv, code, scale, gt, gl, 6, 0.1, sink_blocks=1, recent_blocks=2,
+                                                  k_scale=ks, v_scale=vs, return_selected=True)
+        both.append((code, scale, sel, out))
+    want = plain.select(q, both[0][0].cpu(), both[0][1].cpu(), table, clen, 6, 16, 1, 2)
+    for code, scale, sel, out in both:
+        assert torch.equal(code, both[0][0]) and torch.equal(scale, both[0][1])
+        assert torch.equal(sel.cpu(), want)
+        # (how the rows are shared out, and with that the order of the sums, follows from the chosen pages alone)
+        assert torch.equal(bits(out), bits(both[0][3]))
+
+
+def touched(lens, new, block, columns, packed):
+    """Pages of each sequence that an append of new[b] tokens lies in."""
+    out = []
+    for n, m in zip(lens, new):
+        last = (n - 1) // block if n > 0 else -1
+        if last >= columns:
+            last = columns - 1 if packed else -1
+        out.append(range(max(n - m, 0) // block, last + 1) if m else range(0))
+    return out
+
+
+@pytest.mark.parametrize("Hk,D,block,cdt", [(4, 128, 16, FP8), (3, 64, 32, F16), (2, 256, 8, BF16), (2, 40, 5, F32),
+                                            (1, 64, 16, FP8), (2, 96, 12, F16)])
+@pytest.mark.parametrize("packed", [True, False])
+def test_append_keeps_summaries_of_every_type(cuda, packed, Hk, D, block, cdt):
+    """The touched pages' summaries are the rebuild's, all others stay; some tokens have no place."""
+    new = [1, 3 * block + 2, 0, block, 7, 2] if packed else [1] * 6
+    past = [block - 1, 3, 30, 2 * block, 4 * block - 2, block]
+    lens = [a + b for a, b in zip(new, past)]
+    if not packed:
+        lens[2] = 0  # idle
+    g = gen(D + block)
+    table, nb = table_for(lens, block, g, extra_columns=0)
+    table = table[:, :4]              # sequences that reach past it
+    table[3, 2] = -1                  # a page that is none
+    qdt = {FP8: BF16, F16: F16, BF16: BF16, F32: F32}[cdt]
+    ks, vs = (0.25, 0.5) if cdt == FP8 else (1.0, 1.0)
+    kc, vc = (to_cache(torch.randn(nb, Hk, block, D, generator=g), cdt, 1.0).to(cuda) for _ in "kv")
+    k, v = (torch.randn(sum(new), Hk, D, generator=g).to(qdt).to(cuda) for _ in "kv")
+    code, scale = paged.new_block_summary(kc)
+    code.fill_(77)
+    scale.fill_(-1.0)
+    cu = torch.tensor([0] + new).cumsum(0).int().to(cuda) if packed else None
+    gt, gl = table.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+    paged.paged_append(k, v, kc, vc, gt, gl, cu_seqlens=cu, k_scale=ks, v_scale=vs, summary=code, summary_scale=scale)
+    every = paged.new_block_summary(kc)
+    paged.paged_block_summary(kc, gt, gl, *every, k_scale=ks)
+    pages = [int(table[b, j]) for b, r in enumerate(touched(lens, new, block, 4, packed)) for j in r]
+    pages = sorted(p for p in pages if 0 <= p < nb)
+    assert pages
+    others = [p for p in range(nb) if p not in pages]
+    assert torch.equal(code[pages], every[0][pages]) and torch.equal(scale[pages], every[1][pages])
+    assert (code[others] == 77).all() and (scale[others] == -1).all()
+    # and the rebuild's are the plain form's
+    want = torch.zeros(nb, Hk, 2, D, dtype=torch.int8), torch.zeros(nb, Hk)
+    expected_summary(kc.cpu(), table, [min(n, 4 * block) for n in lens], block, torch.tensor(ks, dtype=F32), *want)
+    assert torch.equal(every[0].cpu(), want[0]) and torch.equal(every[1].cpu(), want[1])
+
+
+def test_choice_and_summaries_past_32_bit_offsets(cuda):
+    """Summaries of more than 2^32 bytes over a cache of more than 2^31: pages at the far end."""
+    nb, Hk, block, D = 140000, 64, 1, 256
+    kc = torch.zeros(nb, Hk, block, D, dtype=FP8, device=cuda)
+    far = [nb - 1, 3, nb - 7, nb // 2 + 1, nb - 2]
+    g = gen(81)
+    for p in far:
+        kc[p] = to_cache(torch.randn(Hk, block, D, generator=g), FP8, 1.0).to(cuda)
+    code, scale = paged.new_block_summary(kc)
+    table, lens = torch.tensor([far], dtype=torch.int32), torch.tensor([5], dtype=torch.int32)
+    paged.paged_block_summary(kc, table.to(cuda), lens.to(cuda), code, scale)
+    small = torch.zeros(5, Hk, 2, D, dtype=torch.int8), torch.zeros(5, Hk)
+    local = torch.arange(5, dtype=torch.int32)[None]
+    expected_summary(kc[far].cpu(), local, [5], block, torch.tensor(1.0), *small)
+    assert torch.equal(code[far].cpu(), small[0]) and torch.equal(scale[far].cpu(), small[1])
+    q = torch.randn(1, 2 * Hk, D, generator=g).bfloat16()
+    for budget in (2, 4):
+        got = paged.paged_select_blocks(q.to(cuda), code, scale, table.to(cuda), lens.to(cuda), budget, block, recent_blocks=0)
+        assert torch.equal(got.cpu(), plain.select(q, *small, local, lens, budget, block, 0, 0))
+    # summaries with rows that no vector load can take
+    odd = code.view(nb, Hk, -1).new_zeros(16, Hk, 2 * D + 1)
+    assert odd[..., 1:].unflatten(2, (2, D)).stride(1) % 16  # (the general form; its offsets are the same products)
+    at = odd[..., 1:].unflatten(2, (2, D))
+    at[:5] = small[0].to(cuda)
+    s = torch.zeros(16, Hk, device=cuda)
+    s[:5] = small[1].to(cuda)
+    got = paged.paged_select_blocks(q.to(cuda), at, s, local.to(cuda), lens.to(cuda), 3, block, recent_blocks=0)
+    assert torch.equal(got.cpu(), plain.select(q, *small, local, lens, 3, block, 0, 0))
