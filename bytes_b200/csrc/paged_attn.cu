@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
         }
         // ---- running maximum and sum; P^T fragments
         const bool v0 = g < nv0, v1 = g < nv1;
-        uint32_t pb[NT][2];
+        uint32_t pb[NT][2], pr[NT][2];  // pr: the weights' remainders
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float a[2], c[2], mx[2], pv[4];
@@ -754,14 +754,29 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
             pv[2 + j] = fast_exp2(c[j] - ref);
             lrow[nt][j] += pv[j] + pv[2 + j];
           }
-          // the weights as the matrix product takes them: rounded once to 16 bits (to 2^-9 of themselves, in f16 2^-12), an
-          // error that the output's own rounding to 16 bits covers; their sum is taken before
+          // The weights as the matrix product takes them, in 16 bits; their sum is taken before. Of 16-bit caches a second
+          // product takes what the rounding left (bf16 rounds by up to 2^-8 of a weight, the two together by 2^-16; f16 by
+          // 2^-11 and 2^-22), so that the output's error is that of its own rounding: with one product it was up to 11 %
+          // larger. 8 sequences of 131072 tokens 330 us against 327, 64 of 33 to 8192 74.7 against 74.3. 8-bit caches, whose
+          // values are rounded by 2^-4 themselves, stay with one (in f16; a second costs 5 % at 64 channels, 7 to 11 % with
+          // 16 heads a pass, and leaves the error against 64 bits where it is).
           if (KIND == kBf16) {
-            pb[nt][0] = movmatrix_trans(pack_bf16x2(pv[0], pv[1]));
-            pb[nt][1] = movmatrix_trans(pack_bf16x2(pv[2], pv[3]));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t w = pack_bf16x2(pv[2 * i], pv[2 * i + 1]);
+              pb[nt][i] = movmatrix_trans(w);
+              pr[nt][i] = movmatrix_trans(pack_bf16x2(pv[2 * i] - __uint_as_float(w << 16),
+                                                      pv[2 * i + 1] - __uint_as_float(w & 0xffff0000u)));
+            }
           } else {
-            pb[nt][0] = movmatrix_trans(pack_f16x2(pv[0], pv[1]));
-            pb[nt][1] = movmatrix_trans(pack_f16x2(pv[2], pv[3]));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t w = pack_f16x2(pv[2 * i], pv[2 * i + 1]);
+              pb[nt][i] = movmatrix_trans(w);
+              if (FP8) continue;
+              const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w));
+              pr[nt][i] = movmatrix_trans(pack_f16x2(pv[2 * i] - x.x, pv[2 * i + 1] - x.y));
+            }
           }
         }
         // ---- O^T += V^T P^T
@@ -773,8 +788,13 @@ __global__ void __launch_bounds__(TileShape<D, KIND, NT>::WARPS * 32, 1)
             ldmatrix_x4_trans(a0, a1, a2, a3, from + (mt * 32 / T::SW) * slab + ((mt * 32 % T::SW) ^ (hi ^ x)));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              if (KIND == kBf16) mma_bf16(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-              else mma_f16(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+              if (KIND == kBf16) {
+                mma_bf16(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                mma_bf16(o[mt][nt], a0, a1, a2, a3, pr[nt][0], pr[nt][1]);
+              } else {
+                mma_f16(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                mma_f16(o[mt][nt], a0, a1, a2, a3, pr[nt][0], pr[nt][1]);
+              }
           }
         } else {
           const uint32_t from = vs + ((lane >> 3) & 1) * step8 + (lane & 7) * T::SW, hi = uint32_t(lane >> 4) * 16;

@@ -248,6 +248,21 @@ def test_choice_for_queries_and_keys_that_are_not_numbers(cuda, Hk, D, block, cd
         assert torch.equal(got.cpu(), plain.select(q, code.cpu(), scale.cpu(), table, clen, budget, block, 0, 1))
 
 
+@pytest.mark.parametrize("heads,D,cdt", [(4, 128, BF16), (12, 128, BF16), (8, 64, BF16), (3, 256, BF16), (16, 256, F16),
+                                         (4, 128, F16), (10, 64, F16)])
+@pytest.mark.parametrize("lens", [[700, 1, 40], [9000, 300] + [150] * 60])
+def test_weights_over_16_bit_caches_keep_more_than_16_bits(cuda, heads, D, cdt, lens):
+    """test_gpu_paged.py's bound with the weights' rounding at 2^-16 (bf16: 2^-8 twice over) and 2^-22 (f16) in place of
+    2^-8 and 2^-11: where a row's values cancel, the output's own rounding does not hide it."""
+    q, kc, vc, table, clen, ks, vs = attention_inputs(lens, 2 * heads, 2, D, 16, cdt, cdt, 91)
+    want, _, weight, reach = plain.decode_attn(q, kc, vc, table, clen, D ** -0.5)
+    got = paged.paged_decode_attn(*(t.to(cuda) for t in (q, kc, vc, table, clen)), D ** -0.5).double().cpu()
+    score = (D + 4) * 2.0 ** -23 * reach[..., None]
+    p = 2.0 ** -16 if cdt == BF16 else 2.0 ** -22
+    tol = (p + 2 * score + 2.0 ** -16) * weight + torch.finfo(cdt).eps / 2 * want.abs() * 1.01 + 2.0 ** -25
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
 # ----------------------------------------------------------------------- streams, host threads
 def select_through_c(q, code, scale, table, lens, block, out, ws, stream):
     """A call of the C entry point itself: ctypes lets other host threads run meanwhile, the Python layer's glue does not."""
