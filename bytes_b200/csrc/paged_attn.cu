@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const AttnParams p) {
 // shares for all of the cluster's warps, and adds up what they have over its shared memory.
 //
 // Bound by memory once there is enough of it: 8 sequences of 131072 tokens (28 heads over 4, 128 channels, bf16) 2148
-// MB in 323 us, 6.65 TB/s, what a copy reaches; 64 of 33 to 8192 tokens (32 over 8) 400 MB in 74 us, 5.4 TB/s. The
+// MB in 329 us, 6.5 TB/s, what a copy reaches; 64 of 33 to 8192 tokens (32 over 8) 400 MB in 74 us, 5.4 TB/s. The
 // difference is some 8 us for the launch, the way to the first units, and the join. 8-bit caches are issue-bound as well,
 // since a byte costs twice the work: 8 sequences of 32768 tokens 268 MB in 55 us, 4.9 TB/s. One sequence of 777 tokens
 // takes 7.9 us, all of it latency: a launch, the reads of length, table, page and query, a sum over the cluster, a write.
@@ -178,15 +178,17 @@ struct TileShape {
   static constexpr int SW = ROWB < 128 ? ROWB : 128;  // bytes of a row in one slab (the swizzle's span)
   static constexpr int SLABS = ROWB / SW;
   static constexpr int HALF = kUnit * ROWB;           // keys (or values) of a unit
-  // As many warps as keep their sums in registers and 4 units or more each in flight. Heads 9 to 16 of a KV head
-  // take a second n of the products (NT 2). 32 heads over 2, 300 MB of cache, us with this, with fewer, with more:
+  // As many warps as keep their sums in registers, with what units of theirs in flight 200 KB hold: 2 each (16-bit of 256
+  // channels, and of 128 with NT 1), 3 or 4 (others), 6 (8-bit of 64). Heads 9 to 16 of a KV head take a second n
+  // of the products (NT 2). 32 heads over 2, 300 MB of cache, us with this, with fewer, with more warps (the weights in one
+  // product, see below):
   // D 64 57.6 (12 warps), 67.8 (8), 60.8 (16); fp8 87.4 (16), 96.5 (12); D 128 59.8 (8), 59.6 (10); fp8 74.0 (12), 81.6 (8).
   // D 256 64.0 and fp8 75.9, against 93.0 and 90.9 as two chunks of 8 heads, which read the cache twice.
   static constexpr int WARPS = KIND == kFp8 ? (D == 256 ? 8 : D == 128 && NT == 2 ? 12 : 16)
                                             : (D == 256 ? 6 : D == 128 && NT == 2 ? 8 : D == 64 && NT == 1 ? 16 : 12);
   static constexpr int FIT = 200 * 1024 / (WARPS * HALF * 2);
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
-  static_assert(STAGES >= 2, "a unit in flight beside the one at hand");
+  static_assert(STAGES >= 2, "one unit's copy under way while another is worked off");
   static constexpr int SMEM = WARPS * STAGES * HALF * 2 + WARPS * STAGES * 12 + 1024;
 };
 
@@ -269,8 +271,10 @@ struct ListSums {
 
 // The list's shares: equal ones for the grid's CTAs (the first few get one slot more), and of a CTA's
 // share equal ones for its warps: warp w has slots [begin(w), begin(w + 1)). A short list goes to as
-// many CTAs as it has kMinSlots: spread over the SMs it is there sooner, in fewer parts it is joined sooner
-// (one sequence of 777 tokens, 28 heads over 4: 12.5, 9.5, 9.2, 9.8 us for 1, 2, 4, 8).
+// many CTAs as it has kMinSlots: spread over the SMs it is there sooner, in fewer parts it is joined sooner. Short rows take
+// the list at a table far wider than they are; 8192 columns, 28 heads over 4, us for 1, 2, 4, 8: one sequence of 300
+// tokens 9.3, 9.1, 8.9, 9.4, of 777 12.0, 9.5, 9.3, 9.4, of 2000 12.6, 12.6, 9.8, 9.7, of 4000 13.6, 13.6, 13.7, 11.2; 4 of
+// 300 10.8, 10.9, 9.1, 9.5; 16 of 50 9.5, 9.5, 10.5, 11.0.
 constexpr int kMinSlots = 4;
 
 // A border inside a row of up to `whole` slots, half a share or 7 units, moves to the nearer end of the row: so
@@ -1246,6 +1250,10 @@ void plan_tiles(AttnParams* p) {
   // 19.9, 19.1; 4 of 2000 10.6, 13.5, of 8000 18.2, 17.1; 8 of 4000 14.3, 17.0, of 100 to 4000 13.5, 14.9; 32 over 8, 16
   // of 1900 25.0, 29.8, of 1 to 1900 15.0, 13.7, of 3000 35.7, 40.5, of 100 to 3000 20.7, 16.9. 32 over 2 (16 heads a
   // pass), one of 777 10.2, 9.4, 4000 12.4, 11.3, 8000 14.5, 17.2.
+  // A compromise, since only the table's width is known here: rows of one length are better off in clusters, rows of very
+  // unlike ones in the list, and where the table is far wider than the rows the list takes them whatever they are (one
+  // of 777 at 8192 columns 9.4). The steps of `most` are where the two sides crossed: the more of the SMs the clusters
+  // have, the longer a row may be before what waits for it costs more than a join.
   const int64_t rows = int64_t(p->g.B) * p->g.Hk * p->chunks;
   const int64_t units = rows ? most_slots(*p, p->chunks) / rows - kRowCost : 0;
   // as many CTAs as leave each of them 8 units or more; one for up to two units a warp (one sequence of 300 tokens: 7.5 us

@@ -9,7 +9,7 @@ layer:
     out = paged.paged_decode_attn(q, k_cache, v_cache, block_table, context_lens, D ** -0.5)
 
 or, with page summaries (``new_block_summary``) kept by the append, attention over the pages whose
-8-bit key bounds score highest:
+8-bit key minima and maxima score highest:
 
     out = paged.paged_sparse_decode_attn(q, k_cache, v_cache, summary, summary_scale, block_table,
                                          context_lens, 64, D ** -0.5)
@@ -66,7 +66,8 @@ def paged_block_summary(k_cache, block_table, context_lens, summary, summary_sca
     int8 codes rint(x / s), s = max|x| / 127. Keys that are NaN do not count (a channel of nothing else is
     zero); the largest finite fp32 number stands for an infinite max|x|. ``paged_append`` keeps them page by page; this rebuilds
     them for pages that came from elsewhere (a copied prefix, a swapped-in sequence). A page that several
-    sequences share is summarised once for each of them, so it should be full in all.
+    sequences share is summarised once for each of them, so it should be full in all. Every column of the
+    table is visited: pass it cut to the longest sequence where that is known.
     """
     rc = N.glue().paged_block_summary(k_cache, block_table,
                                       context_lens, k_scale, summary, summary_scale)
@@ -83,9 +84,10 @@ def paged_select_blocks(q, summary, summary_scale, block_table, context_lens, bu
                         recent_blocks=1):
     """Logical pages for one new token of each sequence, int32 [B, H_k, budget], ascending, -1 after the last.
 
-    The ``sink_blocks`` first and ``recent_blocks`` last pages, then those with the largest bound of q.k over
-    the page (8-bit q and summaries, the largest over the KV head's query heads, the lower page on ties). A q
-    that is NaN counts as zero, an infinite one as the largest finite fp32 number.
+    The ``sink_blocks`` first and ``recent_blocks`` last pages, then those with the largest estimate of q.k's
+    maximum over the page (8-bit q and summaries, rounded to the nearest; the largest over the KV head's query
+    heads, the lower page on ties). A q that is NaN counts as zero, an infinite one as the largest finite fp32
+    number.
     """
     _check_row(q)
     if budget < 1:
