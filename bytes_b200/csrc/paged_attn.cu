@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(kGenWarps * 32) paged_attn_generic_kernel(cons
     }
     const int64_t at = (int64_t(b) * p.Hq + hk * p.G + h0 + h) * p.n_splits + split;
     p.part_o[at * D + d] = O;
-    if (d == 0) { p.part_m[at] = L != L ? 0.f : M; p.part_l[at] = L; }  // a sum that is NaN is not passed over for its maximum
+    // a sum that is NaN is not passed over for its maximum
+    if (d == 0) { p.part_m[at] = L != L ? 0.f : M; p.part_l[at] = L; }
   }
 }
 

@@ -428,9 +428,9 @@ template <> struct Pair<__half> {
 // second the maxima.
 //
 // Bound by memory, and nearly by its instructions (2.3 of 4 a cycle): the keys are read once, and of a page of 16 rows
-// 1/15 as many bytes written. 8 sequences of 30001 to
-// 32768 tokens, four KV heads of 128 channels, bf16: 273 MB in 50 us, 5.4 TB/s, 83 % of what a copy reaches. Two
-// CTAs of 8 warps an SM, each with eight 16-byte loads a lane in flight, are 64 KB an SM.
+// 1/15 as many bytes written. 8 sequences of 30001 to 32768 tokens, four KV heads of 128 channels, bf16: 273 MB in 50 us,
+// 5.4 TB/s, 83 % of what a copy reaches. Two CTAs of 8 warps an SM, each with eight 16-byte loads a lane in flight, are
+// 64 KB an SM.
 template <typename T, bool FP8, int LPR>
 __global__ void __launch_bounds__(256, 2) paged_summary_kernel(const SummaryParams p, int64_t pages) {
   using P = Pair<T>;
